@@ -1,0 +1,778 @@
+// serve_attn.cuh - softmax attention of packed queries on mma.sync tiles, for
+// packed prompts and for trees of drafted tokens over a paged cache.
+//
+//   o_i = sum_{j in M(i)} e_ij v_j / (sum_{j in M(i)} e_ij + e^sink / e^m_i),
+//   e_ij = exp(scale q_i.k_j - m_i), m_i the running maximum over M(i).
+//
+// A tile is BM rows of one key head: row r is (token r / G, head r % G) of the
+// G query heads that share it, so grouped heads read a key once. The keys come
+// in blocks of BN through cp.async into 16-byte-swizzled shared memory, two
+// stages ahead where they fit; scores, the softmax statistics (fp32, exp2 of
+// log2-scaled scores) and the output stay in registers over one pass.
+//
+// Warps: WM x WN. WM splits the rows. With WN = 1 a warp owns its rows' whole
+// score strip and output, and the weights go from the score accumulators to
+// the second product's operand without leaving registers. Head dims above
+// 128 do not fit that (an output row of 512 columns is 256 registers a thread
+// at 16 rows), so there WN warps share the rows: each scores BN / WN keys over
+// the whole head dim, row maxima and weights cross through shared memory, and
+// each accumulates D / WN output columns.
+//
+// fp32 queries (TERMS = 3) over a bf16 cache enter as three bf16 terms
+// q = t0 + t1 + t2, which carry all 24 significand bits, and so do the
+// weights: products are those of fp32 and only the fp32 accumulation rounds.
+// 16-bit queries use the weights rounded to the cache's type (2^-9 of each
+// weight in bf16, 2^-12 in f16: the size of the output's own rounding).
+//
+// Masked entries: a masked score is -inf whatever its key holds. A masked
+// value row is multiplied by a weight of exactly 0, which is only harmless
+// when the value is finite; blocks that a mask crosses (with three weight terms,
+// whose last ones may be 0, all blocks) look for non-finite values, and a tile that meets one is computed again by serve_slow_rows,
+// which touches visible keys only. Rows outside a sequence and pages outside
+// the pool arrive as zeros (cp.async with a source size of 0) and are masked.
+#pragma once
+
+#include <limits.h>
+
+#include "serve.h"
+
+namespace dsv4cu {
+
+constexpr int SA_MAX_NODES = 128;
+constexpr float SA_LOG2E = 1.4426950408889634f;
+enum { SA_BAD_NODES = 75 };           // a tree with more nodes than max_nodes (dsv4cu_ctx_status)
+
+struct SaArgs {
+    const void *q, *k, *v;            // packed rows; v == NULL: the key rows are the values
+    void *o;
+    const float *sink;                // [hq] or NULL
+    long ldq, ldk, ldv, ldo;          // elements between tokens
+    const int *cu;                    // [n_req + 1]
+    int n_req, nt, hq, hkv, G;
+    int window;                       // keys a row may look back over, INT_MAX: all
+    float scale2;                     // scale * log2 e
+    // tree
+    const void *kc, *vc;              // [n_pages][page_size][hkv][D]
+    const int *table, *ctx_len, *parent;
+    int page_size, page_log2, n_pages, max_pages;   // page_log2 < 0: not a power of two
+    int max_nodes, row_tiles, splits;
+    float *pm, *pl, *po;              // partials [splits][nt * hq](, D), splits > 1
+    int *status;
+    int nst;                          // key stages in shared memory (1 or 2)
+};
+
+DSV4CU_DEV uint32_t sa_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+DSV4CU_DEV void sa_cp16(void *dst, const void *src, bool there)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sa_smem(dst)), "l"(src), "r"(there ? 16 : 0)
+                 : "memory");
+}
+DSV4CU_DEV void sa_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+DSV4CU_DEV void sa_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+DSV4CU_DEV void sa_ldsm4(uint32_t (&r)[4], const void *p)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(sa_smem(p)) : "memory");
+}
+DSV4CU_DEV void sa_ldsm4_t(uint32_t (&r)[4], const void *p)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(sa_smem(p)) : "memory");
+}
+template <bool F16>
+DSV4CU_DEV void sa_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    if constexpr (F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+                     "{%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+                     "{%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+DSV4CU_DEV float sa_exp2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool F16>
+DSV4CU_DEV uint32_t sa_pack(float x, float y)
+{
+    if constexpr (F16) {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+// Two values as TERMS packed words (bf16 terms, each the rounding of what the
+// ones before left over; the subtractions are exact).
+template <int TERMS, bool F16>
+DSV4CU_DEV void sa_split(float x, float y, uint32_t (&w)[TERMS])
+{
+#pragma unroll
+    for (int t = 0; t < TERMS; t++) {
+        w[t] = sa_pack<F16>(x, y);
+        if (t + 1 < TERMS) {
+            x -= __uint_as_float(w[t] << 16);
+            y -= __uint_as_float(w[t] & 0xFFFF0000u);
+        }
+    }
+}
+template <bool F16>
+DSV4CU_DEV float sa_float(uint16_t b)
+{
+    if constexpr (F16) return __half2float(__ushort_as_half(b));
+    else return __uint_as_float((uint32_t)b << 16);
+}
+template <bool F16>
+DSV4CU_DEV bool sa_nonfinite(uint32_t w)
+{
+    constexpr uint32_t E = F16 ? 0x7C00u : 0x7F80u;
+    return (w & E) == E || (w & (E << 16)) == (E << 16);
+}
+// Element (row, col) of a swizzled tile of D columns; col a multiple of 8.
+template <int D>
+DSV4CU_DEV uint16_t *sa_at(uint16_t *base, int row, int col)
+{
+    return base + row * D + ((((col >> 3) ^ (row & 7)) << 3) | (col & 7));
+}
+
+// The rows and keys of one CTA.
+struct SaTile {
+    int begin, len;       // token range of the request / sequence
+    int r0, rows;         // first row of the tile, rows in it
+    int kvh;
+    int ctx, key0;        // tree: cached tokens, first key of the first cached block
+    int nblk_c, blk0, blk1;   // cached blocks; this CTA's range of blocks (cached first, then nodes)
+    int split;
+    const int *table;
+};
+
+// Sequence and tile of prompt tile `id`: the tiles of sequence b are
+// ceil(len * G / BM). All lanes of the warp return the same; begin < 0: no such tile.
+DSV4CU_DEV void sa_find(const int *cu, int n_req, int nt, int G, int BM, int id, int &begin, int &len, int &tile)
+{
+    const int lane = threadIdx.x & 31;
+    begin = -1;
+    len = tile = 0;
+    int before = 0;
+    for (int b0 = 0; b0 < n_req; b0 += 32) {
+        const int b = b0 + lane;
+        int lo = 0, n = 0;
+        if (b < n_req) {
+            lo = max(0, min(__ldg(cu + b), nt));
+            n = max(lo, min(__ldg(cu + b + 1), nt)) - lo;
+        }
+        const int mine = (int)(((int64_t)n * G + BM - 1) / BM);
+        int pre = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xFFFFFFFFu, pre, o);
+            if (lane >= o) pre += y;
+        }
+        const unsigned hit = __ballot_sync(0xFFFFFFFFu, id < before + pre);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            begin = __shfl_sync(0xFFFFFFFFu, lo, l);
+            len = __shfl_sync(0xFFFFFFFFu, n, l);
+            tile = id - before - __shfl_sync(0xFFFFFFFFu, pre - mine, l);
+            return;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, pre, 31);
+    }
+}
+
+// Row of cached key j, or NULL where its page is not in the pool.
+DSV4CU_DEV const uint16_t *sa_cached(const SaArgs &a, const SaTile &t, const void *cache, int j, int D)
+{
+    const int pg = a.page_log2 >= 0 ? j >> a.page_log2 : j / a.page_size;
+    if (pg >= a.max_pages) return nullptr;
+    const int id = __ldg(t.table + pg);
+    if (id < 0 || id >= a.n_pages) return nullptr;
+    const size_t slot = (size_t)id * a.page_size + (j - pg * a.page_size);
+    return reinterpret_cast<const uint16_t *>(cache) + (slot * a.hkv + t.kvh) * D;
+}
+
+template <bool F16, bool QF32>
+DSV4CU_DEV float sa_load_q(const SaArgs &a, size_t at)
+{
+    if constexpr (QF32) return __ldg(reinterpret_cast<const float *>(a.q) + at);
+    else return sa_float<F16>(__ldg(reinterpret_cast<const uint16_t *>(a.q) + at));
+}
+template <bool F16, bool OF32>
+DSV4CU_DEV void sa_store_o(const SaArgs &a, size_t at, float x)
+{
+    if constexpr (OF32) reinterpret_cast<float *>(a.o)[at] = x;
+    else reinterpret_cast<uint16_t *>(a.o)[at] = (uint16_t)(sa_pack<F16>(x, 0.0f) & 0xFFFFu);
+}
+// 1 / (l + sink term); a row without any visible key gives 0.
+DSV4CU_DEV float sa_inv(float l, float m, const float *sink, int head)
+{
+    if (sink) l += sa_exp2(__ldg(sink + head) * SA_LOG2E - m);
+    return l == 0.0f ? 0.0f : 1.0f / l;
+}
+
+// The tile's rows one by one, a warp per row and a lane per key, visible keys
+// only, everything in fp32: the form that a tile falls back to when a value
+// behind a mask is not finite. vis(token, block, key in block) and
+// row(block, key in block, values) are the tile kernel's own mask and addresses.
+template <int D, bool F16, bool QF32, class Vis, class Row>
+__device__ __noinline__ void serve_slow_rows(const SaArgs &a, const SaTile &t, int BN, int warps, Vis vis, Row row)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int E = D / 32;
+    for (int r = warp; r < t.rows; r += warps) {
+        const int tok = (t.r0 + r) / a.G, head = t.kvh * a.G + (t.r0 + r) % a.G;
+        const size_t qat = (size_t)(t.begin + tok) * a.ldq + (size_t)head * D;
+        float m = -INFINITY, l = 0.0f, o[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = 0.0f;
+        for (int blk = t.blk0; blk < t.blk1; blk++)
+            for (int j0 = 0; j0 < BN; j0 += 32) {
+                const int j = j0 + lane;
+                const bool see = j < BN && vis(tok, blk, j);
+                float s = -INFINITY;
+                if (see) {
+                    const uint16_t *k = row(blk, j, false);
+                    float dot = 0.0f;
+                    for (int d = 0; d < D; d++) dot = fmaf(sa_load_q<F16, QF32>(a, qat + d), sa_float<F16>(__ldg(k + d)), dot);
+                    s = dot * a.scale2;
+                }
+                float top = s;
+#pragma unroll
+                for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+                const float nm = fmaxf(m, top), use = nm == -INFINITY ? 0.0f : nm;
+                const float alpha = sa_exp2(m - use), p = see ? sa_exp2(s - use) : 0.0f;
+                m = nm;
+                float ps = p;
+#pragma unroll
+                for (int x = 16; x > 0; x >>= 1) ps += __shfl_xor_sync(0xFFFFFFFFu, ps, x);
+                l = l * alpha + ps;
+#pragma unroll
+                for (int e = 0; e < E; e++) o[e] *= alpha;
+                unsigned todo = __ballot_sync(0xFFFFFFFFu, see);
+                while (todo) {
+                    const int jj = __ffs(todo) - 1;
+                    todo &= todo - 1;
+                    const float w = __shfl_sync(0xFFFFFFFFu, p, jj);
+                    const uint16_t *v = row(blk, j0 + jj, true);
+#pragma unroll
+                    for (int e = 0; e < E; e++) o[e] = fmaf(w, sa_float<F16>(__ldg(v + lane + 32 * e)), o[e]);
+                }
+            }
+        if (a.splits > 1) {
+            const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + tok) * a.hq + head;
+#pragma unroll
+            for (int e = 0; e < E; e++) a.po[id * D + lane + 32 * e] = o[e];
+            if (lane == 0) {
+                a.pm[id] = m;
+                a.pl[id] = l;
+            }
+        } else {
+            const float inv = sa_inv(l, m, a.sink, head);
+            const size_t at = (size_t)(t.begin + tok) * a.ldo + (size_t)head * D;
+#pragma unroll
+            for (int e = 0; e < E; e++) sa_store_o<F16, QF32>(a, at + lane + 32 * e, o[e] * inv);
+        }
+    }
+}
+
+template <int D, int WM, int WN, int BN, int TERMS, bool F16, bool TREE>
+__global__ void __launch_bounds__(32 * WM * WN) serve_attn_kernel(const __grid_constant__ SaArgs a)
+{
+    constexpr int BM = 16 * WM, THREADS = 32 * WM * WN, C16 = D / 8;
+    constexpr int KW = BN / WN, NT = KW / 8;             // keys and score n tiles of a warp
+    constexpr int DW = D / WN, ON = DW / 8;              // output columns and n tiles of a warp
+    constexpr int PS = BN + 8;
+    constexpr bool QF32 = TERMS > 1;
+    static_assert(!(QF32 && F16), "three terms are bf16 terms");
+    extern __shared__ __align__(128) uint16_t sa_sm[];
+    __shared__ int s_par[TREE ? SA_MAX_NODES : 1], s_depth[TREE ? SA_MAX_NODES : 1];
+    __shared__ unsigned long long s_anc[TREE ? SA_MAX_NODES : 1][2];
+    __shared__ int s_bad[2];
+    __shared__ uint8_t s_there[2][BN];
+    __shared__ float s_red[WN][BM];
+    const bool shared_v = a.v == nullptr;
+    uint16_t *qs = sa_sm;                                // [TERMS][BM][D]
+    uint16_t *kvs = qs + TERMS * BM * D;                 // [nst][shared_v ? 1 : 2][BN][D]
+    const int stage_el = (shared_v ? 1 : 2) * BN * D;
+    uint16_t *ps = kvs + a.nst * stage_el;               // [TERMS][BM][PS], WN > 1
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp % WM, wn = warp / WM;
+    const int g = lane >> 2, c = lane & 3;
+
+    // ---- which rows and keys
+    SaTile t;
+    t.ctx = t.key0 = t.nblk_c = t.split = 0;
+    t.table = nullptr;
+    t.kvh = blockIdx.y;
+    if constexpr (TREE) {
+        const int b = blockIdx.z, tile = blockIdx.x % a.row_tiles;
+        t.split = blockIdx.x / a.row_tiles;
+        const int lo = __ldg(a.cu + b), hi = __ldg(a.cu + b + 1);
+        t.begin = max(0, min(lo, a.nt));
+        t.len = max(t.begin, min(hi, a.nt)) - t.begin;
+        if (t.len > a.max_nodes) {                       // refused whole: its rows are left as they were
+            if (tid == 0) atomicCAS(a.status, 0, SA_BAD_NODES);
+            return;
+        }
+        t.r0 = tile * BM;
+        t.ctx = max(0, __ldg(a.ctx_len + b));
+        t.table = a.table + (size_t)b * a.max_pages;
+        // no row looks further back than the shallowest one, at position ctx
+        const int first = a.window > t.ctx ? 0 : t.ctx - a.window + 1;
+        t.key0 = first / BN * BN;
+        t.nblk_c = (t.ctx - t.key0 + BN - 1) / BN;
+        const int nblk = t.nblk_c + (t.len + BN - 1) / BN, per = (nblk + a.splits - 1) / a.splits;
+        t.blk0 = min(nblk, t.split * per);
+        t.blk1 = min(nblk, t.blk0 + per);
+    } else {
+        int tile;
+        sa_find(a.cu, a.n_req, a.nt, a.G, BM, gridDim.x - 1 - blockIdx.x, t.begin, t.len, tile);
+        if (t.begin < 0) return;
+        t.r0 = tile * BM;
+    }
+    t.rows = min(BM, t.len * a.G - t.r0);
+    if (t.rows <= 0) return;
+    const int t_lo = t.r0 / a.G, t_hi = (t.r0 + t.rows - 1) / a.G;
+    if constexpr (!TREE) {
+        const int first = a.window > t_lo ? 0 : t_lo - a.window + 1;
+        t.blk0 = first / BN;
+        t.blk1 = t_hi / BN + 1;
+    }
+    if constexpr (TREE) {
+        // ancestors-or-self as bit sets, depths; a parent that does not come
+        // before its child counts as the root's (none)
+        for (int i = tid; i < t.len; i += THREADS) s_par[i] = __ldg(a.parent + t.begin + i);
+        __syncthreads();
+        for (int i = tid; i < t.len; i += THREADS) {
+            unsigned long long set[2] = {0, 0};
+            int d = -1, x = i;
+            for (;;) {
+                set[x >> 6] |= 1ull << (x & 63);
+                d++;
+                const int p = s_par[x];
+                if (p < 0 || p >= x) break;
+                x = p;
+            }
+            s_anc[i][0] = set[0];
+            s_anc[i][1] = set[1];
+            s_depth[i] = d;
+        }
+        if (tid < 2) s_bad[tid] = -1;
+        __syncthreads();
+    }
+    // a key of block blk: its address, and whether token tok sees it (by
+    // value: the fallback's call must not pin the tile to local memory)
+    const SaArgs &a0 = a;
+    auto row = [t, shared_v, ap = &a0](int blk, int j, bool values) -> const uint16_t * {
+        const SaArgs &a = *ap;
+        const bool vv = values && !shared_v;
+        if (TREE && blk < t.nblk_c) {
+            const int key = t.key0 + blk * BN + j;
+            return key < t.ctx ? sa_cached(a, t, vv ? a.vc : a.kc, key, D) : nullptr;
+        }
+        const int key = (TREE ? blk - t.nblk_c : blk) * BN + j;
+        if (key >= t.len) return nullptr;
+        return reinterpret_cast<const uint16_t *>(vv ? a.v : a.k) + (size_t)(t.begin + key) * (vv ? a.ldv : a.ldk) +
+               (size_t)t.kvh * D;
+    };
+    auto vis = [t, row, ap = &a0](int tok, int blk, int j) -> bool {
+        const SaArgs &a = *ap;
+        if constexpr (TREE) {
+            if (blk < t.nblk_c) {
+                const int key = t.key0 + blk * BN + j;
+                return key < t.ctx && t.ctx - key + s_depth[tok] < a.window && row(blk, j, false) != nullptr;
+            }
+            const int x = (blk - t.nblk_c) * BN + j;
+            return x < t.len && (s_anc[tok][x >> 6] >> (x & 63) & 1) && s_depth[tok] - s_depth[x] < a.window;
+        } else {
+            const int key = blk * BN + j;
+            return key <= tok && tok - key < a.window;
+        }
+    };
+    auto issue = [&](int blk) {
+        const int st = (blk - t.blk0) % a.nst;
+        uint16_t *kd = kvs + st * stage_el;
+        for (int i = tid; i < BN * C16; i += THREADS) {
+            const int j = i / C16, ch = i - j * C16;
+            const uint16_t *k = row(blk, j, false);
+            sa_cp16(sa_at<D>(kd, j, 8 * ch), k ? k + 8 * ch : (const uint16_t *)a.q, k != nullptr);
+            if (!shared_v) {
+                const uint16_t *v = row(blk, j, true);
+                sa_cp16(sa_at<D>(kd + BN * D, j, 8 * ch), v ? v + 8 * ch : (const uint16_t *)a.q, v != nullptr);
+            }
+            if (TREE && ch == 0) {
+                s_there[st][j] = k != nullptr;
+                if (!k) s_bad[st] = blk;
+            }
+        }
+        sa_commit();
+    };
+    if (t.blk0 < t.blk1) issue(t.blk0);
+
+    // ---- queries, as terms of the cache's type
+    for (int i = tid; i < BM * C16; i += THREADS) {
+        const int r = i / C16, ch = i - r * C16;
+        uint4 w[TERMS];
+#pragma unroll
+        for (int x = 0; x < TERMS; x++) w[x] = make_uint4(0, 0, 0, 0);
+        if (r < t.rows) {
+            const int tok = (t.r0 + r) / a.G, head = t.kvh * a.G + (t.r0 + r) % a.G;
+            const size_t at = (size_t)(t.begin + tok) * a.ldq + (size_t)head * D + 8 * ch;
+            if constexpr (QF32) {
+                const float4 *p = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.q) + at);
+                const float4 x = __ldg(p), y = __ldg(p + 1);
+                const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint32_t s[TERMS];
+                    sa_split<TERMS, F16>(f[2 * e], f[2 * e + 1], s);
+#pragma unroll
+                    for (int x2 = 0; x2 < TERMS; x2++) reinterpret_cast<uint32_t *>(&w[x2])[e] = s[x2];
+                }
+            } else {
+                w[0] = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + at));
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < TERMS; x++) *reinterpret_cast<uint4 *>(sa_at<D>(qs + x * BM * D, r, 8 * ch)) = w[x];
+    }
+
+    const int arow = (lane & 7) + 8 * ((lane >> 3) & 1), acol = 8 * (lane >> 4);
+    const int brow = (lane & 7) + 8 * (lane >> 4), bcol = 8 * ((lane >> 3) & 1);
+    const bool live = 16 * wm < t.rows;                  // this warp has rows
+    int tok[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) tok[h] = (t.r0 + min(t.rows - 1, 16 * wm + g + 8 * h)) / a.G;
+    float o[ON][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int n = 0; n < ON; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    bool odd = false;                                    // met a non-finite value in a masked block
+
+    for (int blk = t.blk0; blk < t.blk1; blk++) {
+        const int st = (blk - t.blk0) % a.nst;
+        if (a.nst == 2 && blk + 1 < t.blk1) {
+            issue(blk + 1);
+            sa_wait<1>();
+        } else {
+            sa_wait<0>();
+        }
+        __syncthreads();
+        uint16_t *kt = kvs + st * stage_el, *vt = shared_v ? kt : kt + BN * D;
+        bool full;
+        if constexpr (TREE) {
+            const int e = t.key0 + (blk + 1) * BN;
+            full = blk < t.nblk_c && e <= t.ctx && s_bad[st] != blk && t.ctx + t.len - (e - BN) <= a.window;
+        } else {
+            full = (blk + 1) * BN - 1 <= t_lo && t_hi - blk * BN < a.window;
+        }
+        float s[NT][4];
+        if (live) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+            if constexpr (NT >= 2) {
+#pragma unroll
+                for (int kk = 0; kk < D / 16; kk++) {
+                    uint32_t qa[TERMS][4];
+#pragma unroll
+                    for (int x = 0; x < TERMS; x++) sa_ldsm4(qa[x], sa_at<D>(qs + x * BM * D, 16 * wm + arow, 16 * kk + acol));
+#pragma unroll
+                    for (int n = 0; n < NT; n += 2) {
+                        uint32_t b[4];
+                        sa_ldsm4(b, sa_at<D>(kt, KW * wn + 8 * n + brow, 16 * kk + bcol));
+#pragma unroll
+                        for (int x = TERMS - 1; x >= 0; x--) {
+                            sa_mma<F16>(s[n], qa[x], b[0], b[1]);
+                            sa_mma<F16>(s[n + 1], qa[x], b[2], b[3]);
+                        }
+                    }
+                }
+            } else {                                     // one n tile: four 8-wide k pieces per load
+#pragma unroll
+                for (int k2 = 0; k2 < D / 32; k2++) {
+                    uint32_t b[4];
+                    sa_ldsm4(b, sa_at<D>(kt, KW * wn + (lane & 7), 32 * k2 + 8 * (lane >> 3)));
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+#pragma unroll
+                        for (int x = TERMS - 1; x >= 0; x--) {
+                            uint32_t qa[4];
+                            sa_ldsm4(qa, sa_at<D>(qs + x * BM * D, 16 * wm + arow, 32 * k2 + 16 * h + acol));
+                            sa_mma<F16>(s[0], qa, b[2 * h], b[2 * h + 1]);
+                        }
+                    }
+                }
+            }
+            // ---- scaled scores and their row maxima
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float x = s[n][e] * a.scale2;
+                    if (!full) {
+                        const int j = KW * wn + 8 * n + 2 * c + (e & 1);
+                        bool see;
+                        if constexpr (TREE) {
+                            if (blk < t.nblk_c)
+                                see = s_there[st][j] && t.ctx - (t.key0 + blk * BN + j) + s_depth[tok[e >> 1]] < a.window;
+                            else
+                                see = vis(tok[e >> 1], blk, j);
+                        } else {
+                            see = vis(tok[e >> 1], blk, j);
+                        }
+                        if (!see) x = -INFINITY;
+                    }
+                    s[n][e] = x;
+                    top[e >> 1] = fmaxf(top[e >> 1], x);
+                }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                top[h] = fmaxf(top[h], __shfl_xor_sync(0xFFFFFFFFu, top[h], 1));
+                top[h] = fmaxf(top[h], __shfl_xor_sync(0xFFFFFFFFu, top[h], 2));
+            }
+            if constexpr (WN > 1) {
+                if (c == 0) {
+                    s_red[wn][16 * wm + g] = top[0];
+                    s_red[wn][16 * wm + g + 8] = top[1];
+                }
+            } else {
+                s_red[0][0] = 0.0f;                      // unused
+            }
+            if constexpr (WN == 1) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) top[h] = fmaxf(top[h], m[h]);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float use = top[h] == -INFINITY ? 0.0f : top[h], alpha = sa_exp2(m[h] - use);
+                    m[h] = top[h];
+                    l[h] *= alpha;
+#pragma unroll
+                    for (int n = 0; n < ON; n++) {
+                        o[n][2 * h] *= alpha;
+                        o[n][2 * h + 1] *= alpha;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int e = 2 * h; e < 2 * h + 2; e++) {
+                            s[n][e] = sa_exp2(s[n][e] - use);
+                            l[h] += s[n][e];
+                        }
+                }
+            }
+        }
+        if constexpr (WN > 1) {
+            __syncthreads();
+            if (live) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float top = m[h];
+#pragma unroll
+                    for (int w = 0; w < WN; w++) top = fmaxf(top, s_red[w][16 * wm + g + 8 * h]);
+                    const float use = top == -INFINITY ? 0.0f : top, alpha = sa_exp2(m[h] - use);
+                    m[h] = top;
+                    l[h] *= alpha;
+#pragma unroll
+                    for (int n = 0; n < ON; n++) {
+                        o[n][2 * h] *= alpha;
+                        o[n][2 * h + 1] *= alpha;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const float x = sa_exp2(s[n][2 * h] - use), y = sa_exp2(s[n][2 * h + 1] - use);
+                        l[h] += x + y;
+                        uint32_t w[TERMS];
+                        sa_split<TERMS, F16>(x, y, w);
+#pragma unroll
+                        for (int i = 0; i < TERMS; i++)
+                            *reinterpret_cast<uint32_t *>(ps + (i * BM + 16 * wm + g + 8 * h) * PS + KW * wn + 8 * n +
+                                                          2 * c) = w[i];
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (live) {
+#pragma unroll
+            for (int kk = 0; kk < BN / 16; kk++) {
+                uint32_t pa[TERMS][4];
+                if constexpr (WN > 1) {
+#pragma unroll
+                    for (int x = 0; x < TERMS; x++) sa_ldsm4(pa[x], ps + (x * BM + 16 * wm + arow) * PS + 16 * kk + acol);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {        // rows g / g + 8, keys 2c.. / 2c + 8..
+                        uint32_t w[TERMS];
+                        const int n = (2 * kk + (e >> 1)) % NT;
+                        sa_split<TERMS, F16>(s[n][2 * (e & 1)], s[n][2 * (e & 1) + 1], w);
+#pragma unroll
+                        for (int x = 0; x < TERMS; x++) pa[x][e] = w[x];
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < ON; n += 2) {
+                    uint32_t b[4];
+                    sa_ldsm4_t(b, sa_at<D>(vt, 16 * kk + arow, DW * wn + 8 * n + acol));
+                    if (TERMS > 1 || !full)              // a weight's zero terms times infinity are NaN as well
+                        odd = odd || sa_nonfinite<F16>(b[0]) || sa_nonfinite<F16>(b[1]) || sa_nonfinite<F16>(b[2]) ||
+                              sa_nonfinite<F16>(b[3]);
+#pragma unroll
+                    for (int x = TERMS - 1; x >= 0; x--) {
+                        sa_mma<F16>(o[n], pa[x], b[0], b[1]);
+                        sa_mma<F16>(o[n + 1], pa[x], b[2], b[3]);
+                    }
+                }
+            }
+        }
+        __syncthreads();                                 // this stage and the weights are free
+        if (a.nst == 1 && blk + 1 < t.blk1) issue(blk + 1);
+    }
+    if (__syncthreads_or(odd)) {
+        serve_slow_rows<D, F16, QF32>(a, t, BN, WM * WN, vis, row);
+        return;
+    }
+    // ---- exp-sums over the quad, and over the warps that share the rows
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
+    }
+    if constexpr (WN > 1) {
+        if (c == 0) {
+            s_red[wn][16 * wm + g] = l[0];
+            s_red[wn][16 * wm + g + 8] = l[1];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            l[h] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WN; w++) l[h] += s_red[w][16 * wm + g + 8 * h];
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int r = 16 * wm + g + 8 * h;
+        if (r >= t.rows) continue;
+        const int head = t.kvh * a.G + (t.r0 + r) % a.G, col = DW * wn + 2 * c;
+        if (a.splits > 1) {
+            const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + tok[h]) * a.hq + head;
+#pragma unroll
+            for (int n = 0; n < ON; n++)
+                *reinterpret_cast<float2 *>(a.po + id * D + col + 8 * n) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+            if (wn == 0 && c == 0) {
+                a.pm[id] = m[h];
+                a.pl[id] = l[h];
+            }
+        } else {
+            const float inv = sa_inv(l[h], m[h], a.sink, head);
+            const size_t at = (size_t)(t.begin + tok[h]) * a.ldo + (size_t)head * D + col;
+#pragma unroll
+            for (int n = 0; n < ON; n++) {
+                const float x = o[n][2 * h] * inv, y = o[n][2 * h + 1] * inv;
+                if constexpr (QF32) *reinterpret_cast<float2 *>(reinterpret_cast<float *>(a.o) + at + 8 * n) = make_float2(x, y);
+                else *reinterpret_cast<uint32_t *>(reinterpret_cast<uint16_t *>(a.o) + at + 8 * n) = sa_pack<F16>(x, y);
+            }
+        }
+    }
+}
+
+// Joins the splits of a tree's rows, a warp per row: the partial outputs
+// rescaled to the row's largest maximum and divided by the joint exp-sum (with
+// the sink), in split order.
+template <int D, bool F16, bool QF32>
+__global__ void __launch_bounds__(256) serve_join_kernel(const SaArgs a)
+{
+    pdl_wait();
+    const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int lo = __ldg(a.cu + b), hi = __ldg(a.cu + b + 1);
+    const int begin = max(0, min(lo, a.nt)), len = max(begin, min(hi, a.nt)) - begin;
+    const int r = blockIdx.x * 8 + warp;
+    if (len > a.max_nodes || r >= len * a.hq) return;
+    const int head = r % a.hq;
+    const size_t id = (size_t)(begin + r / a.hq) * a.hq + head, step = (size_t)a.nt * a.hq;
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; s++) m = fmaxf(m, a.pm[id + s * step]);
+    constexpr int E = D / 32;
+    float l = 0.0f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = 0.0f;
+    const float use = m == -INFINITY ? 0.0f : m;
+    for (int s = 0; s < a.splits; s++) {
+        const float ms = a.pm[id + s * step];
+        if (ms == -INFINITY) continue;                   // a split without a visible key wrote zeros
+        const float f = sa_exp2(ms - use);
+        l = fmaf(a.pl[id + s * step], f, l);
+        const float *src = a.po + (id + s * step) * D + lane;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = fmaf(src[32 * e], f, o[e]);
+    }
+    const float inv = sa_inv(l, m, a.sink, head);
+    const size_t at = (size_t)(begin + r / a.hq) * a.ldo + (size_t)head * D;
+#pragma unroll
+    for (int e = 0; e < E; e++) sa_store_o<F16, QF32>(a, at + lane + 32 * e, o[e] * inv);
+}
+
+// Tile shape of a head dim: rows, keys per block and warps.
+template <int D>
+struct SaShape {
+    static constexpr int WM = D <= 128 ? 4 : 2, WN = D <= 128 ? 1 : 4, BN = D <= 128 ? 64 : 32;
+    static constexpr int BM = 16 * WM;
+};
+
+constexpr int SA_SMEM_MAX = 220 * 1024;      // of 227 KB: the static arrays come on top
+
+template <int D, int TERMS, bool F16, bool TREE>
+int serve_attn_launch(SaArgs a, cudaStream_t st)
+{
+    using S = SaShape<D>;
+    auto kern = serve_attn_kernel<D, S::WM, S::WN, S::BN, TERMS, F16, TREE>;
+    const size_t stage = (size_t)(a.v ? 2 : 1) * S::BN * D * 2;
+    const size_t rest = (size_t)TERMS * S::BM * D * 2 + (S::WN > 1 ? (size_t)TERMS * S::BM * (S::BN + 8) * 2 : 0);
+    a.nst = rest + 2 * stage <= SA_SMEM_MAX ? 2 : 1;
+    const size_t smem = rest + a.nst * stage;
+    static SmemLimit lim;
+    DSV4CU_CUDA_TRY(smem_limit(lim, (const void *)kern, (int)smem));
+    dim3 grid;
+    if (TREE) {
+        grid = dim3(a.row_tiles * a.splits, a.hkv, a.n_req);
+    } else {
+        const int64_t tiles = (int64_t)a.nt * a.G / S::BM + min(a.n_req, a.nt);
+        if (tiles > INT_MAX) return dsv4cu_set_error(DSV4CU_ERR_ARG, "prompt_attn: %lld row tiles", (long long)tiles);
+        grid = dim3((unsigned)tiles, a.hkv, 1);
+    }
+    kern<<<grid, 32 * S::WM * S::WN, smem, st>>>(a);
+    DSV4CU_LAUNCH_CHECK();
+    if (TREE && a.splits > 1) {
+        auto join = serve_join_kernel<D, F16, (TERMS > 1)>;
+        const dim3 jg((unsigned)(((int64_t)a.max_nodes * a.hq + 7) / 8), a.n_req, 1);
+        DSV4CU_CUDA_TRY(launch_pdl(join, jg, dim3(256), 0, st, a));
+    }
+    return DSV4CU_OK;
+}
+
+// One translation unit per operand kind.
+int serve_attn_bf16(const SaArgs &a, int D, bool tree, cudaStream_t st);
+int serve_attn_f16(const SaArgs &a, int D, bool tree, cudaStream_t st);
+int serve_attn_f32(const SaArgs &a, int D, bool tree, cudaStream_t st);
+
+template <int TERMS, bool F16>
+int serve_attn_pick(const SaArgs &a, int D, bool tree, cudaStream_t st)
+{
+    switch (D) {
+    case 64: return tree ? serve_attn_launch<64, TERMS, F16, true>(a, st) : serve_attn_launch<64, TERMS, F16, false>(a, st);
+    case 128: return tree ? serve_attn_launch<128, TERMS, F16, true>(a, st) : serve_attn_launch<128, TERMS, F16, false>(a, st);
+    case 256: return tree ? serve_attn_launch<256, TERMS, F16, true>(a, st) : serve_attn_launch<256, TERMS, F16, false>(a, st);
+    default: return tree ? serve_attn_launch<512, TERMS, F16, true>(a, st) : serve_attn_launch<512, TERMS, F16, false>(a, st);
+    }
+}
+
+}  // namespace dsv4cu

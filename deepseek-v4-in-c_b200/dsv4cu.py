@@ -143,6 +143,15 @@ def lib() -> C.CDLL:
             "dsv4cu_trunk_resident_bytes": (C.c_int64, [vp]),
             "dsv4cu_trunk_free": (None, [vp]),
             "dsv4cu_head": (i, [vp, vp, vp, vp, vp, i, vp]),
+            "dsv4cu_page_plan_workspace": (sz, [i]),
+            "dsv4cu_page_plan": (i, [vp, vp, vp]),
+            "dsv4cu_paged_write": (i, [vp, vp, vp, i, vp, vp, i, C.c_long, C.c_long, vp, i, i, i, i, vp]),
+            "dsv4cu_prompt_attn": (i, [vp, vp, vp]),
+            "dsv4cu_tree_attn_workspace": (sz, [vp, vp]),
+            "dsv4cu_tree_attn": (i, [vp, vp, vp]),
+            "dsv4cu_verify_greedy": (i, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i, i, vp]),
+            "dsv4cu_verify_sample": (i, [vp, vp, vp, vp, vp, vp, vp, vp, C.c_long, vp, C.c_long, vp, i, vp, vp, i, i,
+                                         vp]),
             "dsv4cu_quantize_fp8": (i, [vp, vp, vp, i, i, vp]),
             "dsv4cu_quantize_fp4": (i, [vp, vp, vp, i, i, vp]),
             "dsv4cu_fill_normal": (i, [vp, sz, C.c_uint64, f, f, vp]),
@@ -345,6 +354,33 @@ class FfnDesc(C.Structure):
                [("ep", C.c_void_p)]
 
 
+class PagePlanArgs(C.Structure):
+    """dsv4cu_page_plan_args (include/dsv4cu.h): device pointers."""
+    _fields_ = [(n, C.c_int) for n in ("n_req", "page_size", "n_pages", "max_pages", "nt_cap")] + \
+               [(n, C.c_void_p) for n in ("seq_len", "new_len", "held", "held_out", "table", "ring", "ring_pos",
+                                          "ring_pos_out", "cu", "slot", "pos", "req")]
+
+
+class PromptAttnArgs(C.Structure):
+    """dsv4cu_prompt_attn_args (include/dsv4cu.h): device pointers."""
+    _fields_ = [(n, C.c_void_p) for n in ("o", "q", "k", "v")] + \
+               [(n, C.c_long) for n in ("ldo", "ldq", "ldk", "ldv")] + \
+               [("q_type", C.c_int), ("kv_type", C.c_int), ("cu", C.c_void_p)] + \
+               [(n, C.c_int) for n in ("n_req", "nt", "n_heads", "n_kv", "head_dim", "window")] + \
+               [("scale", C.c_float), ("sink", C.c_void_p)]
+
+
+class TreeAttnArgs(C.Structure):
+    """dsv4cu_tree_attn_args (include/dsv4cu.h): device pointers."""
+    _fields_ = [(n, C.c_void_p) for n in ("o", "q", "k", "v", "k_cache", "v_cache")] + \
+               [(n, C.c_long) for n in ("ldo", "ldq", "ldk", "ldv")] + \
+               [("q_type", C.c_int), ("kv_type", C.c_int)] + \
+               [(n, C.c_void_p) for n in ("table", "ctx_len", "cu", "parent")] + \
+               [(n, C.c_int) for n in ("n_req", "nt", "n_heads", "n_kv", "head_dim", "page_size", "n_pages",
+                                       "max_pages", "max_nodes", "max_ctx", "window")] + \
+               [("scale", C.c_float), ("sink", C.c_void_p)]
+
+
 class Device:
     """The native dsv4cu_* entry points on one CUDA device."""
 
@@ -357,6 +393,7 @@ class Device:
         torch.cuda.set_device(device)
         check(self.L.dsv4cu_ctx_create(C.byref(h), device), "ctx_create")
         self.ctx = h
+        self._elem = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
     def close(self):
         if self.ctx:
@@ -690,6 +727,173 @@ class Device:
         check(self.L.dsv4cu_sparse_attn(self.ctx, self.ptr(o), self.ptr(q), self.ptr(kv), kv_bf16,
                                         self.ptr(sink), self.ptr(idxs), h, d, topk, scale,
                                         self.stream()), "dsv4cu_sparse_attn")
+
+    # ---- paged serving
+    def _ints(self, what, n, *tensors):
+        """Every tensor is contiguous int32 on this device with n elements (None passes)."""
+        i32, device = self.torch.int32, self.device
+        for t in tensors:
+            if t is not None and (t.dtype is not i32 or t.get_device() != device or t.numel() != n or
+                                  not t.is_contiguous()):
+                raise DSV4CUError(f"{what}: needs contiguous int32 tensors of {n} elements on cuda:{device}, got "
+                                  f"{t.dtype} {tuple(t.shape)} on {t.device}")
+
+    def _rows(self, what, t, heads, dim, dtype=None):
+        """Packed token rows [nt][heads][dim], any stride between tokens: that stride in elements."""
+        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.get_device() != self.device or \
+                t.dtype not in self._elem or (dtype is not None and t.dtype is not dtype):
+            raise DSV4CUError(f"{what}: needs rows [tokens][{heads}][{dim}] on cuda:{self.device}, got {t.dtype} "
+                              f"{tuple(t.shape)} on {t.device}")
+        step, head, one = t.stride()
+        if (one != 1 and dim > 1) or (head != dim and heads > 1):
+            raise DSV4CUError(f"{what}: the heads of a token must be contiguous, got strides {t.stride()}")
+        return step if t.shape[0] > 1 else heads * dim
+
+    def _sink(self, what, sink, heads):
+        if sink is not None and (sink.dtype is not self.torch.float32 or sink.numel() != heads or
+                                 sink.get_device() != self.device or not sink.is_contiguous()):
+            raise DSV4CUError(f"{what}: sink needs {heads} contiguous float32 on cuda:{self.device}")
+
+    def _caches(self, what, k_cache, v_cache):
+        if k_cache.dim() != 4 or not k_cache.is_contiguous() or k_cache.get_device() != self.device or \
+                k_cache.dtype not in self._elem or \
+                (v_cache is not None and (v_cache.shape != k_cache.shape or v_cache.dtype is not k_cache.dtype or
+                                          not v_cache.is_contiguous() or v_cache.get_device() != self.device)):
+            raise DSV4CUError(f"{what}: caches are contiguous [pages][page_size][kv heads][head_dim] of one type on "
+                              f"cuda:{self.device}")
+
+    def page_plan(self, table, held, ring, ring_pos, seq_len, new_len, page_size: int, cu, slot, pos=None, req=None,
+                  held_out=None, ring_pos_out=None):
+        """Block tables and slot maps from request lengths (dsv4cu_page_plan). table [n_req][max_pages], held,
+        seq_len and new_len [n_req], ring [n_pages], cu [n_req + 1], slot / pos / req [nt_cap]: int32; ring_pos [2]
+        int64. held_out / ring_pos_out None: held and ring_pos are updated in place."""
+        held_out = held if held_out is None else held_out
+        ring_pos_out = ring_pos if ring_pos_out is None else ring_pos_out
+        n, cap = seq_len.numel(), slot.numel()
+        self._ints("page_plan", n, seq_len, new_len, held, held_out)
+        self._ints("page_plan", cap, slot, pos, req)
+        self._ints("page_plan", n + 1, cu)
+        self._ints("page_plan", ring.numel(), ring)
+        if table.dim() != 2 or table.shape[0] != n:
+            raise DSV4CUError(f"page_plan: table needs {n} rows, got {tuple(table.shape)}")
+        self._ints("page_plan", table.numel(), table)
+        for t in (ring_pos, ring_pos_out):
+            if t.dtype is not self.torch.int64 or t.numel() != 2 or t.get_device() != self.device or \
+                    not t.is_contiguous():
+                raise DSV4CUError("page_plan: ring_pos needs two contiguous int64 on this device")
+        p = self.ptr
+        a = PagePlanArgs(n, page_size, ring.numel(), table.shape[1], cap, p(seq_len), p(new_len), p(held), p(held_out),
+                         p(table), p(ring), p(ring_pos), p(ring_pos_out), p(cu), p(slot), p(pos), p(req))
+        check(self.L.dsv4cu_page_plan(self.ctx, C.byref(a), self.stream()), "dsv4cu_page_plan")
+
+    def paged_write(self, k_cache, v_cache, k, v, slot):
+        """k_cache / v_cache [pages][page_size][kv heads][head_dim] at slot[t] = row t of k / v
+        [nt][kv heads][head_dim] (dsv4cu_paged_write); v_cache and v None: keys only."""
+        self._caches("paged_write", k_cache, v_cache)
+        pages, page, kv, dim = k_cache.shape
+        nt = k.shape[0]
+        ldk = self._rows("paged_write", k, kv, dim)
+        ldv = 0
+        if v is not None:
+            ldv = self._rows("paged_write", v, kv, dim, k.dtype)
+            if v.shape[0] != nt:
+                raise DSV4CUError(f"paged_write: {nt} key rows and {v.shape[0]} value rows")
+        self._ints("paged_write", nt, slot)
+        check(self.L.dsv4cu_paged_write(self.ctx, self.ptr(k_cache), self.ptr(v_cache), self._elem[k_cache.dtype],
+                                        self.ptr(k), self.ptr(v), self._elem[k.dtype], ldk, ldv, self.ptr(slot), nt,
+                                        pages * page, kv, dim, self.stream()), "dsv4cu_paged_write")
+
+    def prompt_attn(self, o, q, k, v, cu, scale: float, window: int = 0, sink=None):
+        """Causal attention of packed prompts (dsv4cu_prompt_attn): o / q [nt][heads][dim], k / v [nt][kv heads][dim]
+        (v None: the keys are the values), cu int32 [n_req + 1], sink float32 [heads] or None."""
+        what = "prompt_attn"
+        nt, heads, dim = q.shape
+        kv = k.shape[1]
+        ldq, ldo = self._rows(what, q, heads, dim), self._rows(what, o, heads, dim, q.dtype)
+        ldk = self._rows(what, k, kv, dim)
+        ldv = 0 if v is None else self._rows(what, v, kv, dim, k.dtype)
+        if o.shape[0] != nt or k.shape[0] != nt or (v is not None and v.shape[0] != nt):
+            raise DSV4CUError(f"{what}: q, k, v and o must have the same number of tokens")
+        self._ints(what, cu.numel(), cu)
+        self._sink(what, sink, heads)
+        p = self.ptr
+        a = PromptAttnArgs(p(o), p(q), p(k), p(v), ldo, ldq, ldk, ldv, self._elem[q.dtype], self._elem[k.dtype], p(cu),
+                           cu.numel() - 1, nt, heads, kv, dim, window, scale, p(sink))
+        check(self.L.dsv4cu_prompt_attn(self.ctx, C.byref(a), self.stream()), "dsv4cu_prompt_attn")
+
+    def _tree_args(self, o, q, k, v, k_cache, v_cache, table, ctx_len, cu, parent, scale, max_nodes, max_ctx, window,
+                   sink):
+        what = "tree_attn"
+        nt, heads, dim = q.shape
+        self._caches(what, k_cache, v_cache)
+        pages, page, kv, _ = k_cache.shape
+        ldq, ldo = self._rows(what, q, heads, dim), self._rows(what, o, heads, dim, q.dtype)
+        ldk = self._rows(what, k, kv, dim, k_cache.dtype)
+        ldv = 0 if v is None else self._rows(what, v, kv, dim, k_cache.dtype)
+        if k_cache.shape[3] != dim or (v is None) != (v_cache is None) or o.shape[0] != nt or k.shape[0] != nt or \
+                (v is not None and v.shape[0] != nt):
+            raise DSV4CUError(f"{what}: q, k, v, o and the caches do not fit together")
+        n = ctx_len.numel()
+        self._ints(what, n, ctx_len)
+        self._ints(what, n + 1, cu)
+        self._ints(what, nt, parent)
+        if table.dim() != 2 or table.shape[0] != n:
+            raise DSV4CUError(f"{what}: table needs {n} rows, got {tuple(table.shape)}")
+        self._ints(what, table.numel(), table)
+        self._sink(what, sink, heads)
+        p = self.ptr
+        return TreeAttnArgs(p(o), p(q), p(k), p(v), p(k_cache), p(v_cache), ldo, ldq, ldk, ldv, self._elem[q.dtype],
+                            self._elem[k.dtype], p(table), p(ctx_len), p(cu), p(parent), n, nt, heads, kv, dim, page,
+                            pages, table.shape[1], max_nodes, max_ctx, window, scale, p(sink))
+
+    def tree_attn(self, o, q, k, v, k_cache, v_cache, table, ctx_len, cu, parent, scale: float, max_nodes: int,
+                  max_ctx: int, window: int = 0, sink=None):
+        """Attention of drafted trees over a paged cache (dsv4cu_tree_attn): o / q [nt][heads][dim], k / v
+        [nt][kv heads][dim] the nodes' own rows, caches [pages][page_size][kv heads][dim] through table
+        [n_req][max_pages], ctx_len [n_req], cu [n_req + 1], parent [nt]: int32."""
+        a = self._tree_args(o, q, k, v, k_cache, v_cache, table, ctx_len, cu, parent, scale, max_nodes, max_ctx,
+                            window, sink)
+        check(self.L.dsv4cu_tree_attn(self.ctx, C.byref(a), self.stream()), "dsv4cu_tree_attn")
+
+    def tree_attn_workspace(self, *args, window: int = 0, sink=None) -> int:
+        """Workspace bytes of the tree_attn call with these arguments (dsv4cu_tree_attn_workspace)."""
+        return self.L.dsv4cu_tree_attn_workspace(self.ctx, C.byref(self._tree_args(*args, window, sink)))
+
+    def _verify(self, what, accepted, next_token, path, tokens, parent, cu, slot, slot_out):
+        n, nt = cu.numel() - 1, tokens.numel()
+        self._ints(what, n, accepted, next_token)
+        self._ints(what, n + 1, cu)
+        self._ints(what, nt, tokens, path, parent, slot, slot_out)
+        return n, nt
+
+    def verify_greedy(self, accepted, next_token, path, tokens, parent, cu, best, slot=None, slot_out=None):
+        """Drafted trees against the target's greedy picks best [nt] (dsv4cu_verify_greedy)."""
+        n, nt = self._verify("verify_greedy", accepted, next_token, path, tokens, parent, cu, slot, slot_out)
+        self._ints("verify_greedy", nt, best)
+        p = self.ptr
+        check(self.L.dsv4cu_verify_greedy(self.ctx, p(accepted), p(next_token), p(path), p(tokens), p(parent), p(cu),
+                                          p(best), p(slot), p(slot_out), n, nt, self.stream()), "dsv4cu_verify_greedy")
+
+    def verify_sample(self, accepted, next_token, path, tokens, parent, cu, probs, u, draft=None, slot=None,
+                      slot_out=None):
+        """Drafted trees against the target's probabilities probs [nt][vocab] from uniform numbers u [nt], draft
+        [nt][vocab] or None for certain drafts (dsv4cu_verify_sample)."""
+        n, nt = self._verify("verify_sample", accepted, next_token, path, tokens, parent, cu, slot, slot_out)
+        f32, device = self.torch.float32, self.device
+        if probs.dim() != 2 or u.numel() != nt or not u.is_contiguous():
+            raise DSV4CUError("verify_sample: probs [nt][vocab] and contiguous u [nt] are needed")
+        for t in (probs, draft):
+            if t is not None and (t.shape != probs.shape or t.shape[0] != nt or t.dtype is not f32 or
+                                  t.get_device() != device or (t.shape[1] > 1 and t.stride(1) != 1)):
+                raise DSV4CUError("verify_sample: probabilities are float32 [nt][vocab] on this device")
+        if u.dtype is not f32 or u.get_device() != device:
+            raise DSV4CUError("verify_sample: u is float32 on this device")
+        vocab = probs.shape[1]
+        step = lambda t: vocab if t is None or nt < 2 else t.stride(0)  # noqa: E731
+        p = self.ptr
+        check(self.L.dsv4cu_verify_sample(self.ctx, p(accepted), p(next_token), p(path), p(tokens), p(parent), p(cu),
+                                          p(probs), step(probs), p(draft), step(draft), p(u), vocab, p(slot),
+                                          p(slot_out), n, nt, self.stream()), "dsv4cu_verify_sample")
 
     def quantize_fp8(self, w, s, src, rows, cols):
         check(self.L.dsv4cu_quantize_fp8(self.ptr(w), self.ptr(s), self.ptr(src), rows, cols,

@@ -620,6 +620,144 @@ int dsv4cu_argmax(int *best, const float *logits, int n, int nt, void *stream);
 int dsv4cu_head(dsv4cu_ctx *ctx, float *logits, int *best, const float *x, const dsv4cu_qmat *head, int nt,
                 void *stream);
 
+/* ---- paged serving: a key / value cache of fixed-size pages shared by many
+ * requests, packed prompts, and drafted tokens with their verification. No
+ * counterpart in the reference, which serves one request at a time from one
+ * host array and decodes greedily; these stand beside dsv4cu_sparse_attn
+ * (one token over index lists) and dsv4cu_argmax. A serving step is
+ *   page_plan -> prompt_attn, paged_write                   (prompts)
+ *   page_plan -> tree_attn -> head -> verify -> paged_write (decoding)
+ * Every call runs on its context's device whichever device is current, is
+ * enqueued on the stream and can be captured in a CUDA graph. Calls that use
+ * the context workspace (page_plan, tree_attn) share it with the context's
+ * other calls: reserve it (dsv4cu_ctx_reserve) before capturing, do not let
+ * it grow while captured graphs are alive, and give streams or graphs that
+ * run at the same time a context each. Index arrays are device int32; what
+ * they hold is clamped or skipped, never read or written through. */
+enum { DSV4CU_F32 = 0, DSV4CU_BF16 = 1, DSV4CU_F16 = 2 };   /* element types */
+
+/* Block tables and slot maps from request lengths. Request b holds held[b]
+ * pages, table[b][0 .. held[b] - 1]; page ids are < n_pages. Free pages are
+ * ring[i mod n_pages] for ring_pos[0] <= i < ring_pos[1] (head and tail, both
+ * >= 0, growing without end). A step appends new_len[b] tokens behind
+ * seq_len[b]: requests in order take the pages they lack from the head and
+ * enter them in the table. new_len[b] < 0: the request is over, its pages go
+ * back to the tail in table order and it holds none. Then, packed by request,
+ * cu [n_req + 1] = first token row of each, and for token rows t < nt_cap
+ * slot[t] = page * page_size + offset, pos[t] = its position, req[t] = its
+ * request (pos and req may be NULL); rows behind the last token get -1.
+ * held_out / ring_pos_out may be held / ring_pos. Only table entries of newly
+ * granted pages and ring entries of released ones are written, so the same
+ * call on the same held and ring_pos writes the same again. Status codes
+ * (dsv4cu_ctx_status): 71 the ring ran out (requests in order got what was
+ * there, slots on missing pages are -1), 72 more tokens than nt_cap (the rest
+ * has no row), 73 a request needs more than max_pages pages (slots behind
+ * them are -1). */
+typedef struct {
+    int n_req, page_size, n_pages, max_pages, nt_cap;
+    const int *seq_len, *new_len;       /* [n_req] */
+    const int *held;                    /* [n_req] */
+    int *held_out;                      /* [n_req] */
+    int *table;                         /* [n_req][max_pages] */
+    int *ring;                          /* [n_pages] */
+    const int64_t *ring_pos;            /* [2] */
+    int64_t *ring_pos_out;              /* [2] */
+    int *cu, *slot, *pos, *req;
+} dsv4cu_page_plan_args;
+size_t dsv4cu_page_plan_workspace(int n_req);
+int dsv4cu_page_plan(dsv4cu_ctx *ctx, const dsv4cu_page_plan_args *args, void *stream);
+
+/* cache[slot[t]] = row t for nt rows of n_kv * head_dim elements, keys and
+ * (v, v_cache not NULL) values, ldk / ldv elements between source rows. The
+ * cache is bf16 or f16 [n_slots][n_kv][head_dim]; rows are fp32 (rounded to
+ * nearest) or of the cache's type. Slots outside [0, n_slots) are skipped; no
+ * slot may appear twice. head_dim % 8 == 0, everything 16-byte aligned. */
+int dsv4cu_paged_write(dsv4cu_ctx *ctx, void *k_cache, void *v_cache, int cache_type, const void *k, const void *v,
+                       int src_type, long ldk, long ldv, const int *slot, int nt, int n_slots, int n_kv, int head_dim,
+                       void *stream);
+
+/* Causal attention over whole prompts of different lengths, packed: sequence b
+ * is token rows cu[b] .. cu[b + 1] - 1 of nt. n_heads query heads in groups of
+ * n_heads / n_kv per key head; token i sees token j of its sequence when
+ * j <= i and (window > 0) i - j < window; scale > 0; sink [n_heads] fp32 or
+ * NULL joins the denominator only, as in dsv4cu_sparse_attn. q / o of q_type,
+ * k / v of kv_type (bf16 or f16); q_type = kv_type, or fp32 with bf16 keys
+ * (then only fp32 accumulation rounds; 16-bit queries use weights rounded to
+ * kv_type). v NULL: the key rows are the values. head_dim 64, 128, 256 or 512.
+ * ld*: elements between token rows, heads contiguous; rows 16-byte aligned. A
+ * key or value that is not finite reaches only rows that see it. Token rows
+ * outside every sequence are not written. */
+typedef struct {
+    void *o;
+    const void *q, *k, *v;
+    long ldo, ldq, ldk, ldv;
+    int q_type, kv_type;
+    const int *cu;                      /* [n_req + 1] */
+    int n_req, nt, n_heads, n_kv, head_dim;
+    int window;                         /* 0: no window */
+    float scale;
+    const float *sink;
+} dsv4cu_prompt_attn_args;
+int dsv4cu_prompt_attn(dsv4cu_ctx *ctx, const dsv4cu_prompt_attn_args *args, void *stream);
+
+/* Attention of drafted token trees over a paged cache. Request b's nodes are
+ * token rows cu[b] .. cu[b + 1] - 1 (at most max_nodes <= 128): node 0 the last
+ * committed token, parent[row] the index within the request of a node's
+ * parent, smaller than its own (-1, or any other value: none). A node sees the
+ * ctx_len[b] cached tokens, its ancestors and itself; its position is
+ * ctx_len[b] + depth, and a window counts by positions. One node per request
+ * is plain decoding. k / v are the nodes' own rows (they need not be in the
+ * cache); k_cache / v_cache [n_pages][page_size][n_kv][head_dim] are read
+ * through table [n_req][max_pages], where ids outside [0, n_pages) are masked.
+ * Types, heads, head dims, sink, v NULL (then v_cache NULL as well) and
+ * non-finite values as in dsv4cu_prompt_attn. max_ctx, an upper estimate of
+ * ctx_len, only chooses how many ways a cache is split. A request with more
+ * than max_nodes nodes is left out and sets status code 75. */
+typedef struct {
+    void *o;
+    const void *q, *k, *v, *k_cache, *v_cache;
+    long ldo, ldq, ldk, ldv;
+    int q_type, kv_type;
+    const int *table, *ctx_len;         /* [n_req][max_pages], [n_req] */
+    const int *cu, *parent;             /* [n_req + 1], [nt] */
+    int n_req, nt, n_heads, n_kv, head_dim, page_size, n_pages, max_pages, max_nodes, max_ctx;
+    int window;
+    float scale;
+    const float *sink;
+} dsv4cu_tree_attn_args;
+size_t dsv4cu_tree_attn_workspace(const dsv4cu_ctx *ctx, const dsv4cu_tree_attn_args *args);
+int dsv4cu_tree_attn(dsv4cu_ctx *ctx, const dsv4cu_tree_attn_args *args, void *stream);
+
+/* Verification of drafted trees (cu, parent as in dsv4cu_tree_attn, at most
+ * 128 nodes per request; more sets status code 76). The current node starts
+ * at node 0; a node in index order whose parent is the current node is tested
+ * and becomes the current node when accepted. accepted[b] = accepted nodes
+ * (node 0 not counted), next[b] = the token behind the last of them, path
+ * [nt]: rows cu[b] + i hold node 0 (i = 0) and the i-th accepted node, then -1.
+ * With slot [nt] (a page plan's slots for the request's rows) and slot_out
+ * [nt], slot_out of the d-th node of the path is slot[cu[b] + d] and -1 for
+ * every other node: the rows dsv4cu_paged_write commits. A request without
+ * nodes gets accepted 0 and next -1.
+ *
+ * verify_greedy: a node is accepted when tokens[row] == best[current row]
+ * (dsv4cu_argmax of the target's logits); next = best of the last one.
+ * verify_sample: p [nt][vocab] the target's probabilities behind each node,
+ * draft [nt][vocab] the distribution a node's children were drawn from (NULL:
+ * the drafts are certain), u [nt] uniform numbers of [0, 1): u of node 0 draws
+ * the next token, u of any other node tests it. With rest = p[cur], mass = 1
+ * at each new current node, a node of token x is accepted when
+ * u * mass * draft[cur][x] < rest[x]; refused, rest = max(rest - mass *
+ * draft[cur], 0) and mass = sum(rest) (certain drafts: mass -= rest[x],
+ * rest[x] = 0). next = the first x whose running sum of rest passes
+ * u * sum(rest); an empty rest falls back to p[cur], and -1 where that has no
+ * positive finite sum. In doubles. ldp / ldd: floats between rows. */
+int dsv4cu_verify_greedy(dsv4cu_ctx *ctx, int *accepted, int *next, int *path, const int *tokens, const int *parent,
+                         const int *cu, const int *best, const int *slot, int *slot_out, int n_req, int nt,
+                         void *stream);
+int dsv4cu_verify_sample(dsv4cu_ctx *ctx, int *accepted, int *next, int *path, const int *tokens, const int *parent,
+                         const int *cu, const float *p, long ldp, const float *draft, long ldd, const float *u,
+                         int vocab, const int *slot, int *slot_out, int n_req, int nt, void *stream);
+
 /* --------------------------------------------------- weight packing utility
  * Quantize fp32 [rows][cols] to the reference pack layouts: FP8 e4m3 with one
  * E8M0 scale per 128x128 block, or FP4 e2m1 with one E8M0 scale per 1x32
