@@ -4,6 +4,7 @@
 #include <math.h>
 
 #include "serve_attn.cuh"
+#include "serve_umma.cuh"
 
 namespace dsv4cu {
 
@@ -66,8 +67,23 @@ static SaArgs fill_common(const Common &c, const int *cu, const float *sink)
     return s;
 }
 
-static int serve_attn_run(const SaArgs &s, const Common &c, bool tree, cudaStream_t st)
+// The tcgen05 kernel takes 16-bit operands at head dims 64 and 128 where TMA
+// can copy the rows (strides below 2^40 bytes; cached pages of a power of two
+// of at least 8 rows, the swizzle's period, in fewer than 2^31 slots).
+static bool use_umma(const Common &c)
 {
+    return c.q_type != DSV4CU_F32 && c.head_dim <= 128 && c.ldk < (1l << 38) && (!c.v || c.ldv < (1l << 38));
+}
+static bool use_umma(const dsv4cu_tree_attn_args *a, const Common &c)
+{
+    return use_umma(c) && a->page_size >= 8 && (a->page_size & (a->page_size - 1)) == 0 &&
+           (int64_t)a->n_pages * a->page_size <= INT_MAX;
+}
+
+static int serve_attn_run(const SaArgs &s, const Common &c, bool tree, bool umma, cudaStream_t st)
+{
+    if (umma)
+        return c.q_type == DSV4CU_F16 ? serve_umma_f16(s, c.head_dim, tree, st) : serve_umma_bf16(s, c.head_dim, tree, st);
     if (c.q_type == DSV4CU_F32) return serve_attn_f32(s, c.head_dim, tree, st);
     return c.q_type == DSV4CU_F16 ? serve_attn_f16(s, c.head_dim, tree, st) : serve_attn_bf16(s, c.head_dim, tree, st);
 }
@@ -103,19 +119,35 @@ static int tree_check(const dsv4cu_tree_attn_args *a, const Common &c)
     return DSV4CU_OK;
 }
 
-// Row tiles and splits of a tree call: enough CTAs to fill the SMs twice, no
-// split of fewer than 4 key blocks.
-static void tree_shape(const dsv4cu_ctx *ctx, const dsv4cu_tree_attn_args *a, int &row_tiles, int &splits)
+// Row tiles, splits and blocks per split of a tree call. Splits only matter
+// for speed: they come from the estimate max_ctx, and the kernel spreads the
+// real blocks over them.
+struct TreeShape {
+    bool umma;
+    int two, row_tiles, splits, chunk;
+};
+static TreeShape tree_shape(const dsv4cu_ctx *ctx, const dsv4cu_tree_attn_args *a, const Common &c)
 {
-    const int G = a->n_heads / a->n_kv, BM = a->head_dim <= 128 ? 64 : 32, BN = a->head_dim <= 128 ? 64 : 32;
-    row_tiles = (int)(((int64_t)a->max_nodes * G + BM - 1) / BM);
-    const int64_t ctas = (int64_t)row_tiles * a->n_kv * a->n_req;
+    TreeShape s = {};
+    s.umma = use_umma(a, c);
+    const int64_t rows = (int64_t)a->max_nodes * (a->n_heads / a->n_kv);
+    s.two = s.umma && rows > 128;
+    const int BM = s.umma ? (s.two ? 256 : 128) : a->head_dim <= 128 ? 64 : 32;
+    const int BN = s.umma ? 128 : a->head_dim <= 128 ? 64 : 32;
+    s.row_tiles = (int)((rows + BM - 1) / BM);
+    const int64_t ctas = (int64_t)s.row_tiles * a->n_kv * a->n_req;
     const int seen = a->window && a->window < a->max_ctx ? a->window : a->max_ctx;
-    const int64_t most = seen / (4 * BN);
-    int64_t s = ctas > 0 ? (2 * (int64_t)ctx->sm_count + ctas - 1) / ctas : 1;
-    if (s > most) s = most;
-    if (s > 64) s = 64;
-    splits = s < 1 ? 1 : (int)s;
+    const int64_t blocks = (int64_t)seen / BN + 2;        // the cached ones and the nodes' own
+    // about 8 CTAs per SM in all; a split of few blocks costs more for its
+    // partial rows (4 (D + 2) bytes each, written and read) than it saves
+    int64_t least = min(rows, (int64_t)BM) / 8;
+    if (least < 2) least = 2;
+    int64_t chunk = (blocks * ctas + 8 * ctx->sm_count - 1) / (8 * ctx->sm_count);
+    if (chunk < least) chunk = least;
+    if (chunk < (blocks + 63) / 64) chunk = (blocks + 63) / 64;
+    s.chunk = (int)chunk;
+    s.splits = (int)((blocks + chunk - 1) / chunk);
+    return s;
 }
 
 static size_t tree_ws(const dsv4cu_tree_attn_args *a, int splits)
@@ -141,15 +173,13 @@ extern "C" int dsv4cu_prompt_attn(dsv4cu_ctx *ctx, const dsv4cu_prompt_attn_args
     DSV4CU_CUDA_TRY(guard.enter(ctx->device));
     SaArgs s = fill_common(c, a->cu, a->sink);
     s.status = ctx->status;
-    return serve_attn_run(s, c, false, (cudaStream_t)stream);
+    return serve_attn_run(s, c, false, use_umma(c), (cudaStream_t)stream);
 }
 
 extern "C" size_t dsv4cu_tree_attn_workspace(const dsv4cu_ctx *ctx, const dsv4cu_tree_attn_args *a)
 {
     if (!ctx || !a || tree_check(a, common_of(a)) || a->n_req == 0 || a->nt == 0) return 0;
-    int tiles, splits;
-    tree_shape(ctx, a, tiles, splits);
-    return tree_ws(a, splits);
+    return tree_ws(a, tree_shape(ctx, a, common_of(a)).splits);
 }
 
 extern "C" int dsv4cu_tree_attn(dsv4cu_ctx *ctx, const dsv4cu_tree_attn_args *a, void *stream)
@@ -175,7 +205,11 @@ extern "C" int dsv4cu_tree_attn(dsv4cu_ctx *ctx, const dsv4cu_tree_attn_args *a,
     s.max_pages = a->max_pages;
     s.max_nodes = a->max_nodes;
     s.status = ctx->status;
-    tree_shape(ctx, a, s.row_tiles, s.splits);
+    const TreeShape shape = tree_shape(ctx, a, c);
+    s.two = shape.two;
+    s.row_tiles = shape.row_tiles;
+    s.splits = shape.splits;
+    s.chunk = shape.chunk;
     if (s.splits > 1) {
         void *ws = nullptr;
         r = dsv4cu_ws_get(ctx, tree_ws(a, s.splits), &ws);
@@ -185,5 +219,5 @@ extern "C" int dsv4cu_tree_attn(dsv4cu_ctx *ctx, const dsv4cu_tree_attn_args *a,
         s.pl = (float *)((char *)ws + rows);
         s.po = (float *)((char *)ws + 2 * rows);
     }
-    return serve_attn_run(s, c, true, (cudaStream_t)stream);
+    return serve_attn_run(s, c, true, shape.umma, (cudaStream_t)stream);
 }

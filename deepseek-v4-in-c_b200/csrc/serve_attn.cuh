@@ -56,10 +56,36 @@ struct SaArgs {
     const int *table, *ctx_len, *parent;
     int page_size, page_log2, n_pages, max_pages;   // page_log2 < 0: not a power of two
     int max_nodes, row_tiles, splits;
+    int chunk;                        // key blocks of a split, at least
     float *pm, *pl, *po;              // partials [splits][nt * hq](, D), splits > 1
     int *status;
-    int nst;                          // key stages in shared memory (1 or 2)
+    int nst;                          // key stages in shared memory
+    int two, box_log2;                // tcgen05 kernel: two row tiles per CTA; rows of a cached copy's box
 };
+
+// The key blocks of request b of a tree call: blocks of BN cached keys from
+// key0 on (no row looks further back than the shallowest one, at position
+// ctx), then blocks of the request's own nodes; a split takes `per` of them
+// and `used` splits have any.
+struct SaSpan {
+    int begin, len, ctx, kend, key0, nblk_c, nblk, per, used;   // kend: cached keys that the table can hold
+};
+DSV4CU_DEV SaSpan sa_span(const SaArgs &a, int b, int BN)
+{
+    SaSpan s;
+    const int lo = __ldg(a.cu + b), hi = __ldg(a.cu + b + 1);
+    s.begin = max(0, min(lo, a.nt));
+    s.len = max(s.begin, min(hi, a.nt)) - s.begin;
+    s.ctx = max(0, min(__ldg(a.ctx_len + b), INT_MAX - (1 << 20)));   // positions stay in 32 bits
+    s.kend = (int)min((int64_t)s.ctx, (int64_t)a.max_pages * a.page_size);
+    const int first = a.window > s.ctx ? 0 : s.ctx - a.window + 1;
+    s.key0 = first / BN * BN;
+    s.nblk_c = max(0, s.kend - s.key0 + BN - 1) / BN;
+    s.nblk = s.nblk_c + (s.len + BN - 1) / BN;
+    s.per = max(a.chunk, (s.nblk + a.splits - 1) / a.splits);
+    s.used = (s.nblk + s.per - 1) / s.per;
+    return s;
+}
 
 DSV4CU_DEV uint32_t sa_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 DSV4CU_DEV void sa_cp16(void *dst, const void *src, bool there)
@@ -149,9 +175,9 @@ struct SaTile {
     int begin, len;       // token range of the request / sequence
     int r0, rows;         // first row of the tile, rows in it
     int kvh;
-    int ctx, key0;        // tree: cached tokens, first key of the first cached block
+    int ctx, kend, key0;  // tree: cached tokens, those that the table holds, first key of the first cached block
     int nblk_c, blk0, blk1;   // cached blocks; this CTA's range of blocks (cached first, then nodes)
-    int split;
+    int split, parts;     // tree: which split of how many
     const int *table;
 };
 
@@ -224,9 +250,10 @@ DSV4CU_DEV float sa_inv(float l, float m, const float *sink, int head)
 // behind a mask is not finite. vis(token, block, key in block) and
 // row(block, key in block, values) are the tile kernel's own mask and addresses.
 template <int D, bool F16, bool QF32, class Vis, class Row>
-__device__ __noinline__ void serve_slow_rows(const SaArgs &a, const SaTile &t, int BN, int warps, Vis vis, Row row)
+__device__ __noinline__ void serve_slow_rows(const SaArgs &a, const SaTile &t, int BN, int warp, int warps, Vis vis,
+                                             Row row)
 {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
     constexpr int E = D / 32;
     for (int r = warp; r < t.rows; r += warps) {
         const int tok = (t.r0 + r) / a.G, head = t.kvh * a.G + (t.r0 + r) % a.G;
@@ -267,7 +294,7 @@ __device__ __noinline__ void serve_slow_rows(const SaArgs &a, const SaTile &t, i
                     for (int e = 0; e < E; e++) o[e] = fmaf(w, sa_float<F16>(__ldg(v + lane + 32 * e)), o[e]);
                 }
             }
-        if (a.splits > 1) {
+        if (t.parts > 1) {
             const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + tok) * a.hq + head;
 #pragma unroll
             for (int e = 0; e < E; e++) a.po[id * D + lane + 32 * e] = o[e];
@@ -309,29 +336,30 @@ __global__ void __launch_bounds__(32 * WM * WN) serve_attn_kernel(const __grid_c
 
     // ---- which rows and keys
     SaTile t;
-    t.ctx = t.key0 = t.nblk_c = t.split = 0;
+    t.ctx = t.kend = t.key0 = t.nblk_c = t.split = 0;
+    t.parts = 1;
     t.table = nullptr;
     t.kvh = blockIdx.y;
     if constexpr (TREE) {
         const int b = blockIdx.z, tile = blockIdx.x % a.row_tiles;
+        const SaSpan sp = sa_span(a, b, BN);
         t.split = blockIdx.x / a.row_tiles;
-        const int lo = __ldg(a.cu + b), hi = __ldg(a.cu + b + 1);
-        t.begin = max(0, min(lo, a.nt));
-        t.len = max(t.begin, min(hi, a.nt)) - t.begin;
+        t.begin = sp.begin;
+        t.len = sp.len;
         if (t.len > a.max_nodes) {                       // refused whole: its rows are left as they were
             if (tid == 0) atomicCAS(a.status, 0, SA_BAD_NODES);
             return;
         }
+        if (t.split >= sp.used) return;
+        t.parts = sp.used;
         t.r0 = tile * BM;
-        t.ctx = max(0, __ldg(a.ctx_len + b));
+        t.ctx = sp.ctx;
+        t.kend = sp.kend;
         t.table = a.table + (size_t)b * a.max_pages;
-        // no row looks further back than the shallowest one, at position ctx
-        const int first = a.window > t.ctx ? 0 : t.ctx - a.window + 1;
-        t.key0 = first / BN * BN;
-        t.nblk_c = (t.ctx - t.key0 + BN - 1) / BN;
-        const int nblk = t.nblk_c + (t.len + BN - 1) / BN, per = (nblk + a.splits - 1) / a.splits;
-        t.blk0 = min(nblk, t.split * per);
-        t.blk1 = min(nblk, t.blk0 + per);
+        t.key0 = sp.key0;
+        t.nblk_c = sp.nblk_c;
+        t.blk0 = t.split * sp.per;
+        t.blk1 = min(sp.nblk, t.blk0 + sp.per);
     } else {
         int tile;
         sa_find(a.cu, a.n_req, a.nt, a.G, BM, gridDim.x - 1 - blockIdx.x, t.begin, t.len, tile);
@@ -376,7 +404,7 @@ __global__ void __launch_bounds__(32 * WM * WN) serve_attn_kernel(const __grid_c
         const bool vv = values && !shared_v;
         if (TREE && blk < t.nblk_c) {
             const int key = t.key0 + blk * BN + j;
-            return key < t.ctx ? sa_cached(a, t, vv ? a.vc : a.kc, key, D) : nullptr;
+            return key < t.kend ? sa_cached(a, t, vv ? a.vc : a.kc, key, D) : nullptr;
         }
         const int key = (TREE ? blk - t.nblk_c : blk) * BN + j;
         if (key >= t.len) return nullptr;
@@ -388,7 +416,7 @@ __global__ void __launch_bounds__(32 * WM * WN) serve_attn_kernel(const __grid_c
         if constexpr (TREE) {
             if (blk < t.nblk_c) {
                 const int key = t.key0 + blk * BN + j;
-                return key < t.ctx && t.ctx - key + s_depth[tok] < a.window && row(blk, j, false) != nullptr;
+                return key < t.kend && t.ctx - key + s_depth[tok] < a.window && row(blk, j, false) != nullptr;
             }
             const int x = (blk - t.nblk_c) * BN + j;
             return x < t.len && (s_anc[tok][x >> 6] >> (x & 63) & 1) && s_depth[tok] - s_depth[x] < a.window;
@@ -469,7 +497,7 @@ __global__ void __launch_bounds__(32 * WM * WN) serve_attn_kernel(const __grid_c
         bool full;
         if constexpr (TREE) {
             const int e = t.key0 + (blk + 1) * BN;
-            full = blk < t.nblk_c && e <= t.ctx && s_bad[st] != blk && t.ctx + t.len - (e - BN) <= a.window;
+            full = blk < t.nblk_c && e <= t.kend && s_bad[st] != blk && t.ctx + t.len - (e - BN) <= a.window;
         } else {
             full = (blk + 1) * BN - 1 <= t_lo && t_hi - blk * BN < a.window;
         }
@@ -636,7 +664,7 @@ __global__ void __launch_bounds__(32 * WM * WN) serve_attn_kernel(const __grid_c
         if (a.nst == 1 && blk + 1 < t.blk1) issue(blk + 1);
     }
     if (__syncthreads_or(odd)) {
-        serve_slow_rows<D, F16, QF32>(a, t, BN, WM * WN, vis, row);
+        serve_slow_rows<D, F16, QF32>(a, t, BN, warp, WM * WN, vis, row);
         return;
     }
     // ---- exp-sums over the quad, and over the warps that share the rows
@@ -663,7 +691,7 @@ __global__ void __launch_bounds__(32 * WM * WN) serve_attn_kernel(const __grid_c
         const int r = 16 * wm + g + 8 * h;
         if (r >= t.rows) continue;
         const int head = t.kvh * a.G + (t.r0 + r) % a.G, col = DW * wn + 2 * c;
-        if (a.splits > 1) {
+        if (t.parts > 1) {
             const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + tok[h]) * a.hq + head;
 #pragma unroll
             for (int n = 0; n < ON; n++)
@@ -689,26 +717,26 @@ __global__ void __launch_bounds__(32 * WM * WN) serve_attn_kernel(const __grid_c
 // rescaled to the row's largest maximum and divided by the joint exp-sum (with
 // the sink), in split order.
 template <int D, bool F16, bool QF32>
-__global__ void __launch_bounds__(256) serve_join_kernel(const SaArgs a)
+__global__ void __launch_bounds__(256) serve_join_kernel(const SaArgs a, int BN)
 {
     pdl_wait();
-    const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int lo = __ldg(a.cu + b), hi = __ldg(a.cu + b + 1);
-    const int begin = max(0, min(lo, a.nt)), len = max(begin, min(hi, a.nt)) - begin;
-    const int r = blockIdx.x * 8 + warp;
-    if (len > a.max_nodes || r >= len * a.hq) return;
+    const SaSpan sp = sa_span(a, blockIdx.y, BN);
+    const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (sp.len > a.max_nodes || r >= sp.len * a.hq || sp.used <= 1) return;   // one split writes its rows itself
     const int head = r % a.hq;
-    const size_t id = (size_t)(begin + r / a.hq) * a.hq + head, step = (size_t)a.nt * a.hq;
+    const size_t id = (size_t)(sp.begin + r / a.hq) * a.hq + head, step = (size_t)a.nt * a.hq;
     float m = -INFINITY;
-    for (int s = 0; s < a.splits; s++) m = fmaxf(m, a.pm[id + s * step]);
+    for (int s = lane; s < sp.used; s += 32) m = fmaxf(m, a.pm[id + s * step]);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
     constexpr int E = D / 32;
     float l = 0.0f, o[E];
 #pragma unroll
     for (int e = 0; e < E; e++) o[e] = 0.0f;
     const float use = m == -INFINITY ? 0.0f : m;
-    for (int s = 0; s < a.splits; s++) {
+    for (int s = 0; s < sp.used; s++) {
         const float ms = a.pm[id + s * step];
-        if (ms == -INFINITY) continue;                   // a split without a visible key wrote zeros
+        if (ms == -INFINITY) continue;                   // a split without a visible key
         const float f = sa_exp2(ms - use);
         l = fmaf(a.pl[id + s * step], f, l);
         const float *src = a.po + (id + s * step) * D + lane;
@@ -716,9 +744,18 @@ __global__ void __launch_bounds__(256) serve_join_kernel(const SaArgs a)
         for (int e = 0; e < E; e++) o[e] = fmaf(src[32 * e], f, o[e]);
     }
     const float inv = sa_inv(l, m, a.sink, head);
-    const size_t at = (size_t)(begin + r / a.hq) * a.ldo + (size_t)head * D;
+    const size_t at = (size_t)(sp.begin + r / a.hq) * a.ldo + (size_t)head * D;
 #pragma unroll
     for (int e = 0; e < E; e++) sa_store_o<F16, QF32>(a, at + lane + 32 * e, o[e] * inv);
+}
+
+// Launches the join behind a split tree pass of key blocks of BN.
+template <int D, bool F16, bool QF32>
+int serve_join_launch(const SaArgs &a, int BN, cudaStream_t st)
+{
+    const dim3 grid((unsigned)(((int64_t)a.max_nodes * a.hq + 7) / 8), a.n_req, 1);
+    DSV4CU_CUDA_TRY(launch_pdl(serve_join_kernel<D, F16, QF32>, grid, dim3(256), 0, st, a, BN));
+    return DSV4CU_OK;
 }
 
 // Tile shape of a head dim: rows, keys per block and warps.
@@ -751,11 +788,7 @@ int serve_attn_launch(SaArgs a, cudaStream_t st)
     }
     kern<<<grid, 32 * S::WM * S::WN, smem, st>>>(a);
     DSV4CU_LAUNCH_CHECK();
-    if (TREE && a.splits > 1) {
-        auto join = serve_join_kernel<D, F16, (TERMS > 1)>;
-        const dim3 jg((unsigned)(((int64_t)a.max_nodes * a.hq + 7) / 8), a.n_req, 1);
-        DSV4CU_CUDA_TRY(launch_pdl(join, jg, dim3(256), 0, st, a));
-    }
+    if (TREE && a.splits > 1) return serve_join_launch<D, F16, (TERMS > 1)>(a, S::BN, st);
     return DSV4CU_OK;
 }
 

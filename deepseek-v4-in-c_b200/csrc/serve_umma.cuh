@@ -1,0 +1,728 @@
+// serve_umma.cuh - softmax attention of packed queries on tcgen05, for head
+// dims 64 and 128 in 16 bits: packed prompts, and drafted trees over a paged
+// cache whose pages TMA can copy. The mathematics, the packing of grouped
+// heads into rows and the masks are those of serve_attn.cuh.
+//
+// A CTA works on two strips of 128 rows with their scores S (128 fp32 columns)
+// and outputs O (D columns) in TMEM; keys come in blocks of 128.
+//   warp 0       TMA of key and value blocks, two rings of stages
+//   warp 1       TMEM and the single MMA thread: S = Q K^T, then O += P V with
+//                P read from TMEM and V as it lies (its rows are the
+//                contraction: a transposed operand, nothing is moved)
+//   warps 4-7    the first strip's softmax, a thread per row: no shuffles, the
+//   warps 8-11   second strip's. A thread reads its row of S, writes it back as
+//                16-bit weights over S, and holds the running maximum and sum.
+// The two strips take turns: while one is in its softmax the tensor core runs
+// the other's products, so neither waits for the other for long.
+//
+// What a strip is: with more than 128 rows, rows 0-127 and 128-255 over the
+// same key blocks (a block is read once for both); with fewer, the same rows
+// twice, even blocks and odd blocks, joined at the end - so a single strip
+// (decoding) also overlaps its products with its softmax.
+//
+// The running maximum moves only when a row's new one is more than 8 (in
+// log2) above it: weights stay below 2^8, sums and products are exact to the
+// same relative rounding, and the outputs in TMEM are seldom rescaled.
+//
+// Bound by: the exponentials (16 per clock and SM against 128 x 128 scores per
+// block and strip: 1024 clocks, as long as the strip's two products at head
+// dim 128), then the tensor core; for trees of few rows the cache's bytes.
+#pragma once
+
+#include <cuda.h>
+
+#include "serve_attn.cuh"
+#include "tma_gemv.cuh"
+#include "tmap.h"
+#include "umma.cuh"
+
+namespace dsv4cu {
+
+constexpr int SU_BN = 128;                // keys per block
+constexpr int SU_THREADS = 384;
+constexpr int SU_SUB = 128 * 128;         // bytes of a 128-row x 64-column operand tile
+constexpr int SU_MAX_STAGES = 4;
+constexpr int SU_REGS_FEW = 72, SU_REGS_MANY = 216;   // per thread: copy and product warps, softmax warps
+constexpr float SU_LAZY = 8.0f;           // log2 units the running maximum may fall behind
+enum { SUE_KEMPTY = 81, SUE_VEMPTY, SUE_KFULL, SUE_VFULL, SUE_S, SUE_P, SUE_O, SUE_Q, SUE_DRAIN };
+
+// Instruction descriptor of kind::f16: fp32 accumulator, both operands of one
+// 16-bit type (0 f16, 1 bf16), N >> 3 in bits 17-22, M >> 4 in bits 24-28; bit
+// 16 = B with its rows as the contraction.
+__host__ __device__ constexpr uint32_t su_idesc(bool f16, int N, bool bt)
+{
+    return (1u << 4) | ((f16 ? 0u : 1u) << 7) | ((f16 ? 0u : 1u) << 10) | ((bt ? 1u : 0u) << 16) |
+           ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+// The value tile [128 keys][64 columns] x D / 64 read with keys as the
+// contraction: 8-key groups 1024 bytes apart (stride byte offset), 64-column
+// groups one operand tile apart (leading byte offset).
+DSV4CU_DEV uint64_t su_desc_v(const void *p)
+{
+    const uint64_t a = umma::saddr(p);
+    return ((a >> 4) & 0x3FFFull) | ((uint64_t)(SU_SUB >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+DSV4CU_DEV void su_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// The same with A in TMEM: lane = row, 16-bit pairs per column.
+DSV4CU_DEV void su_mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// 32 consecutive columns of this thread's lane.
+DSV4CU_DEV void su_ld32(uint32_t taddr, uint32_t *r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(taddr) : "memory");
+}
+DSV4CU_DEV void su_st32(uint32_t taddr, const uint32_t *r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
+}
+DSV4CU_DEV void su_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+DSV4CU_DEV void su_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+DSV4CU_DEV void su_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+template <int N>
+DSV4CU_DEV void su_bar(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory"); }
+template <int R>
+DSV4CU_DEV void su_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
+template <int R>
+DSV4CU_DEV void su_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
+
+// Box of a [row][head][column] map; x = column (a multiple of 64).
+DSV4CU_DEV void su_tma(void *dst, const CUtensorMap *map, int x, int head, int row, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+                 " [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(umma::saddr(dst)), "l"(map), "r"(x), "r"(head), "r"(row), "r"(umma::saddr(bar)) : "memory");
+}
+// Bounded poll for the single-thread roles.
+DSV4CU_DEV bool su_spin(uint64_t *bar, uint32_t parity, int *err, int code)
+{
+    const uint32_t a = umma::saddr(bar);
+    uint64_t t0 = 0;
+    for (uint32_t i = 0;; i++) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\t"
+                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                     "selp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(a), "r"(parity) : "memory");
+        if (ok) return true;
+        if ((i & 255u) == 0u) {
+            const uint64_t now = globaltimer_ns();
+            if (i == 0) t0 = now;
+            else if (now - t0 > MBAR_TIMEOUT_NS) break;
+        }
+    }
+    atomicCAS(err, 0, code);
+    return false;
+}
+
+// Bits lo .. hi of 128 as four words (empty where lo > hi).
+DSV4CU_DEV uint32_t su_range(int lo, int hi, int word)
+{
+    const int l = max(0, lo - 32 * word), h = min(31, hi - 32 * word);
+    return l > h ? 0u : (0xFFFFFFFFu << l) & (0xFFFFFFFFu >> (31 - h));
+}
+
+template <int D, bool F16, bool TREE>
+__global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_constant__ CUtensorMap mk,
+                                                                   const __grid_constant__ CUtensorMap mv,
+                                                                   const __grid_constant__ CUtensorMap mkc,
+                                                                   const __grid_constant__ CUtensorMap mvc,
+                                                                   const __grid_constant__ SaArgs a)
+{
+    constexpr int DC = D / 64, KVB = DC * SU_SUB;        // operand tiles and bytes of a block
+    extern __shared__ uint8_t su_raw[];
+    __shared__ __align__(8) uint64_t kfull[SU_MAX_STAGES], kempty[SU_MAX_STAGES], vfull[SU_MAX_STAGES],
+        vempty[SU_MAX_STAGES], sfull[2], pfull[2], ofull[2], qfull, drain;
+    __shared__ uint32_t tmem_holder;
+    __shared__ int s_par[TREE ? SA_MAX_NODES : 1], s_depth[TREE ? SA_MAX_NODES : 1];
+    __shared__ uint32_t s_anc[TREE ? SA_MAX_NODES : 1][4];
+    __shared__ int s_odd[2];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)su_raw + 1023) & ~(uintptr_t)1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rows_cta = a.two ? 256 : 128;
+
+    // ---- which rows and keys
+    SaTile t;
+    t.ctx = t.kend = t.key0 = t.nblk_c = t.split = 0;
+    t.parts = 1;
+    t.table = nullptr;
+    t.kvh = blockIdx.y;
+    if constexpr (TREE) {
+        const int b = blockIdx.z;
+        const SaSpan sp = sa_span(a, b, SU_BN);
+        t.split = blockIdx.x / a.row_tiles;
+        t.begin = sp.begin;
+        t.len = sp.len;
+        if (t.len > a.max_nodes) {
+            if (threadIdx.x == 0) atomicCAS(a.status, 0, SA_BAD_NODES);
+            return;
+        }
+        if (t.split >= sp.used) return;
+        t.parts = sp.used;
+        t.r0 = blockIdx.x % a.row_tiles * rows_cta;
+        t.ctx = sp.ctx;
+        t.kend = sp.kend;
+        t.table = a.table + (size_t)b * a.max_pages;
+        t.key0 = sp.key0;
+        t.nblk_c = sp.nblk_c;
+        t.blk0 = t.split * sp.per;
+        t.blk1 = min(sp.nblk, t.blk0 + sp.per);
+    } else {
+        int tile;
+        sa_find(a.cu, a.n_req, a.nt, a.G, rows_cta, gridDim.x - 1 - blockIdx.x, t.begin, t.len, tile);
+        if (t.begin < 0) return;
+        t.r0 = tile * rows_cta;
+    }
+    t.rows = min(rows_cta, t.len * a.G - t.r0);
+    if (t.rows <= 0) return;
+    const int tok_end = (t.r0 + t.rows - 1) / a.G;       // the CTA's last token
+    const bool alt = t.rows <= 128;                      // one strip: even and odd blocks
+    // strip s: rows [row0, row0 + n), key blocks from `first` to `end` by `step`
+    auto strip_first = [&](int s) {
+        if constexpr (TREE) return t.blk0 + (alt ? s : 0);
+        const int tok = (t.r0 + (alt ? 0 : 128 * s)) / a.G, lo = a.window > tok ? 0 : tok - a.window + 1;
+        return lo / SU_BN + (alt ? s : 0);
+    };
+    auto strip_end = [&](int s) {
+        if constexpr (TREE) return t.blk1;
+        return (alt || s ? tok_end : (t.r0 + 127) / a.G) / SU_BN + 1;
+    };
+    const int f0 = strip_first(0), f1 = strip_first(1), e0 = strip_end(0), e1 = strip_end(1), step = alt ? 2 : 1;
+    if constexpr (!TREE) {
+        t.blk0 = f0;
+        t.blk1 = e1;
+    }
+    const int c0 = f0, c1 = e1;                          // all blocks of the CTA: the second strip ends last
+    auto uses = [&](int s, int b) {
+        return s ? b >= f1 && b < e1 && (!alt || ((b - f1) & 1) == 0) : b >= f0 && b < e0 && (!alt || ((b - f0) & 1) == 0);
+    };
+
+    uint8_t *qs = smem, *ks = qs + (a.two ? 2 : 1) * KVB, *vs = ks + a.nst * KVB;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < SU_MAX_STAGES; s++) {
+            mbar_init(&kfull[s], 1);
+            mbar_init(&kempty[s], 1);
+            mbar_init(&vfull[s], 1);
+            mbar_init(&vempty[s], 1);
+        }
+        for (int s = 0; s < 2; s++) {
+            mbar_init(&sfull[s], 1);
+            mbar_init(&pfull[s], 4);
+            mbar_init(&ofull[s], 1);
+            s_odd[s] = 0;
+        }
+        mbar_init(&qfull, 8);
+        mbar_init(&drain, 1);
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        umma::tmem_alloc(&tmem_holder, 512);
+        umma::tmem_relinquish();
+    }
+    int lost = 0;                                        // a page of these blocks is not in the pool
+    if constexpr (TREE) {
+        const int k_lo = t.key0 + t.blk0 * SU_BN, k_hi = min(t.kend, t.key0 + min(t.blk1, t.nblk_c) * SU_BN);
+        if (k_lo < k_hi)
+            for (int pg = k_lo / a.page_size + threadIdx.x; pg <= (k_hi - 1) / a.page_size; pg += SU_THREADS) {
+                const int id = __ldg(t.table + pg);
+                lost |= id < 0 || id >= a.n_pages;
+            }
+        for (int i = threadIdx.x; i < t.len; i += SU_THREADS) s_par[i] = __ldg(a.parent + t.begin + i);
+    }
+    umma::fence_before();
+    lost = __syncthreads_or(lost);
+    umma::fence_after();
+    if constexpr (TREE) {
+        for (int i = threadIdx.x; i < t.len; i += SU_THREADS) {
+            uint32_t set[4] = {0, 0, 0, 0};
+            int d = -1, x = i;
+            for (;;) {
+#pragma unroll
+                for (int w = 0; w < 4; w++) set[w] |= (x >> 5) == w ? 1u << (x & 31) : 0u;
+                d++;
+                const int p = s_par[x];
+                if (p < 0 || p >= x) break;
+                x = p;
+            }
+#pragma unroll
+            for (int w = 0; w < 4; w++) s_anc[i][w] = set[w];
+            s_depth[i] = d;
+        }
+        __syncthreads();
+    }
+    const uint32_t tmem = tmem_holder;
+    const uint32_t tm_s = tmem, tm_o = tmem + 256;       // strip s: S at + 128 s, O at + 128 s
+
+    if (warp < 4) {
+        su_regs_dec<SU_REGS_FEW>();
+        if (warp == 0) {
+            // ------------------------------------------------ copies
+            const int boxes = TREE ? SU_BN >> a.box_log2 : 1;
+            bool ok = true;
+            int n = 0;
+            for (int b = c0; b < c1 && ok; b++, n++) {
+                const int st = n % a.nst, u = n / a.nst;
+                const bool cached = TREE && b < t.nblk_c;
+                int row = 0;
+                bool mine = lane == 0;
+                if (cached) {
+                    const int key = t.key0 + b * SU_BN + (lane << a.box_log2);
+                    mine = lane < boxes && key < t.kend;
+                    if (mine) {
+                        const int pg = key >> a.page_log2, id = __ldg(t.table + pg);
+                        mine = id >= 0 && id < a.n_pages;
+                        row = id * a.page_size + (key - (pg << a.page_log2));
+                    }
+                } else {
+                    row = t.begin + (b - t.nblk_c) * SU_BN;
+                }
+                const unsigned go = __ballot_sync(0xFFFFFFFFu, mine);
+                const uint32_t off = cached ? (uint32_t)lane << (a.box_log2 + 7) : 0u;   // this box's first row
+                const uint32_t bytes = cached ? (uint32_t)__popc(go) * DC << (a.box_log2 + 7) : (uint32_t)KVB;
+#pragma unroll
+                for (int kv = 0; kv < 2; kv++) {
+                    uint64_t *full = kv ? &vfull[st] : &kfull[st], *empty = kv ? &vempty[st] : &kempty[st];
+                    if (lane == 0 && u > 0) ok = su_spin(empty, (u - 1) & 1, a.status, kv ? SUE_VEMPTY : SUE_KEMPTY);
+                    ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive_expect_tx(full, bytes);
+                    __syncwarp();
+                    uint8_t *dst = (kv ? vs : ks) + st * KVB + off;
+                    const CUtensorMap *map = cached ? (kv ? &mvc : &mkc) : (kv ? &mv : &mk);
+                    if (mine)
+#pragma unroll
+                        for (int c = 0; c < DC; c++) su_tma(dst + c * SU_SUB, map, 64 * c, t.kvh, row, full);
+                }
+            }
+            // every issued copy lands before the CTA can exit
+            if (lane == 0)
+                for (int j = max(0, n - a.nst); j < n; j++) {
+                    mbar_wait(&kfull[j % a.nst], (j / a.nst) & 1, nullptr, 0);
+                    mbar_wait(&vfull[j % a.nst], (j / a.nst) & 1, nullptr, 0);
+                }
+        } else if (warp == 1 && lane == 0) {
+            // ------------------------------------------------ products
+            constexpr uint32_t id_s = su_idesc(F16, SU_BN, false), id_o = su_idesc(F16, D, true);
+            bool ok = su_spin(&qfull, 0, a.status, SUE_Q);
+            umma::fence_after();
+            uint32_t once = 0;                           // blocks that one of their two strips has scored
+            auto scores = [&](int s, int b) {
+                const int n = b - c0, st = n % a.nst;
+                ok = ok && su_spin(&kfull[st], (n / a.nst) & 1, a.status, SUE_KFULL);
+                if (!ok) return;
+                umma::fence_after();
+                const uint8_t *q = qs + (alt ? 0 : s) * KVB, *k = ks + st * KVB;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; kk++) {
+                    const int at = (kk >> 2) * SU_SUB + 32 * (kk & 3);
+                    su_mma(tm_s + 128 * s, umma::desc_sw128(q + at), umma::desc_sw128(k + at), id_s, kk > 0);
+                }
+                umma::commit(&sfull[s]);
+                const uint32_t bit = 1u << (b & 31);
+                if (uses(s ^ 1, b) && !(once & bit)) {
+                    once |= bit;
+                } else {                                 // its last reader
+                    once &= ~bit;
+                    umma::commit(&kempty[st]);
+                }
+            };
+            if (f0 < e0) scores(0, f0);
+            if (f1 < e1) scores(1, f1);
+            uint32_t turn[2] = {0, 0};
+            for (int b = c0; b < c1 && ok; b++)
+                for (int s = 0; s < 2 && ok; s++) {
+                    if (!uses(s, b)) continue;
+                    const int n = b - c0, st = n % a.nst;
+                    ok = su_spin(&pfull[s], turn[s] & 1, a.status, SUE_P) &&
+                         su_spin(&vfull[st], (n / a.nst) & 1, a.status, SUE_VFULL);
+                    if (!ok) break;
+                    umma::fence_after();
+                    const uint8_t *v = vs + st * KVB;
+#pragma unroll
+                    for (int kk = 0; kk < SU_BN / 16; kk++)
+                        su_mma_ta(tm_o + 128 * s, tm_s + 128 * s + 8 * kk, su_desc_v(v + 2048 * kk), id_o,
+                                  (turn[s] > 0 || kk > 0) ? 1u : 0u);
+                    turn[s]++;
+                    if (s || !uses(1, b)) umma::commit(&vempty[st]);   // strip 1 comes second
+                    if (b + step < (s ? e1 : e0)) scores(s, b + step);
+                    else umma::commit(&ofull[s]);
+                }
+            // the products in flight complete before TMEM is released
+            umma::commit(&drain);
+            mbar_wait(&drain, 0, a.status, SUE_DRAIN);
+        }
+    } else {
+        su_regs_inc<SU_REGS_MANY>();
+        // ------------------------------------------------ softmax
+        const int s = (warp - 4) >> 2, i = (threadIdx.x - 128) & 127;    // strip; row, and key in prepared values
+        const int row0 = alt ? 0 : 128 * s, rows = min(128, t.rows - row0);
+        {
+            // queries: strip s by its own warps, a single strip by all
+            const int r_n = alt ? 256 : 128, r_i = alt ? threadIdx.x - 128 : i;
+            for (int x = r_i; x < 128 * (D / 8); x += r_n) {
+                const int r = x / (D / 8), ch = x - r * (D / 8);
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (r < rows) {
+                    const int pr = t.r0 + row0 + r, tok = pr / a.G, head = t.kvh * a.G + pr - tok * a.G;
+                    w = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) +
+                                                              (size_t)(t.begin + tok) * a.ldq + (size_t)head * D + 8 * ch));
+                }
+                *reinterpret_cast<uint4 *>(qs + (alt ? 0 : s) * KVB + (ch >> 3) * SU_SUB + r * 128 +
+                                           (((ch & 7) ^ (r & 7)) << 4)) = w;
+            }
+            su_fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&qfull);
+        }
+        const int first = s ? f1 : f0, end = s ? e1 : e0;
+        const bool live = 32 * (warp & 3) < rows;        // this warp has rows
+        const int pr = t.r0 + row0 + min(i, max(0, rows - 1)), tok = pr / a.G, head = t.kvh * a.G + pr - tok * a.G;
+        const int tok_lo = (t.r0 + row0) / a.G, tok_hi = (t.r0 + row0 + rows - 1) / a.G;
+        const int depth = TREE ? s_depth[tok] : 0;
+        const uint32_t quarter = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t sp_s = tm_s + 128 * s + quarter, sp_o = tm_o + 128 * s + quarter;
+        float m = -INFINITY, l = 0.0f;
+        uint32_t turn = 0;
+        bool ok = true;
+        auto in_pool = [&](int key) {
+            if (key >= t.kend) return false;
+            const int id = __ldg(t.table + (key >> a.page_log2));
+            return id >= 0 && id < a.n_pages;
+        };
+        for (int b = first; b < end; b += step, turn++) {
+            // ---- the mask: whether any, whether it differs between rows
+            const bool cached = TREE && b < t.nblk_c;
+            const int base = (TREE ? (cached ? t.key0 + b * SU_BN : (b - t.nblk_c) * SU_BN) : b * SU_BN);
+            bool ragged, masked;
+            if (cached) {
+                ragged = t.ctx + t.len - base > a.window;
+                masked = ragged || lost || base + SU_BN > t.kend;
+            } else if (TREE) {
+                ragged = masked = true;
+            } else {
+                ragged = masked = base + SU_BN - 1 > tok_lo || tok_hi - base >= a.window;
+            }
+            uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+            // behind this block's scores lie the products of every block before
+            // it, so the value stage's last use is over and its barrier is at
+            // most one phase away: the parity below means this block
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sfull[s], turn & 1, a.status, SUE_S));
+            if (!ok) break;
+            if (masked) {
+                // key i of the block is there at all: in its page, before the CTA's last token
+                bool there;
+                if (cached) {
+                    there = in_pool(base + i);
+                } else {
+                    there = base + i <= (TREE ? t.len - 1 : tok_end);
+                }
+                const int n = b - c0, st = n % a.nst;
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&vfull[st], (n / a.nst) & 1, a.status, SUE_VFULL));
+                if (!ok) break;
+                // values of absent keys become zeros; the others must be finite
+                // where the mask keeps them from some rows only
+                uint8_t *v = vs + st * KVB + i * 128;
+                bool odd = false;
+#pragma unroll
+                for (int c = 0; c < DC; c++)
+#pragma unroll
+                    for (int x = 0; x < 8; x++) {
+                        uint4 *p = reinterpret_cast<uint4 *>(v + c * SU_SUB + 16 * x);
+                        if (!there) *p = make_uint4(0, 0, 0, 0);
+                        else if (ragged) {
+                            const uint4 w = *p;
+                            odd = odd || sa_nonfinite<F16>(w.x) || sa_nonfinite<F16>(w.y) || sa_nonfinite<F16>(w.z) ||
+                                  sa_nonfinite<F16>(w.w);
+                        }
+                    }
+                if (odd) s_odd[s] = 1;
+                su_fence_async();
+                if (cached) {
+                    const int pos = t.ctx + depth, lo = a.window > pos ? 0 : pos - a.window + 1 - base;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        vis[w] = su_range(lo, t.kend - 1 - base, w);
+                        if (lost) vis[w] &= __ballot_sync(0xFFFFFFFFu, in_pool(base + 32 * w + lane));
+                    }
+                } else if (TREE) {
+#pragma unroll
+                    for (int w = 0; w < 4; w++) vis[w] = s_anc[tok][w];
+                    if (depth >= a.window)
+                        for (int x = 0; x < t.len; x++)
+                            if (depth - s_depth[x] >= a.window) vis[x >> 5] &= ~(1u << (x & 31));
+                } else {
+                    const int lo = a.window > tok ? 0 : tok - a.window + 1 - base;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) vis[w] = su_range(lo, tok - base, w);
+                }
+            }
+            if (live) {
+                umma::fence_after();
+                uint32_t x[128];
+#pragma unroll
+                for (int c = 0; c < 4; c++) su_ld32(sp_s + 32 * c, x + 32 * c);
+                su_wait_ld();
+                if (masked) {
+#pragma unroll
+                    for (int k = 0; k < 128; k++)
+                        if (!((vis[k >> 5] >> (k & 31)) & 1u)) x[k] = 0xFF800000u;
+                }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int k = 0; k < 128; k++) top[k & 3] = fmaxf(top[k & 3], __uint_as_float(x[k]));
+                const float mrow = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale2;
+                const bool move = mrow > m + SU_LAZY || (m == -INFINITY && mrow > m);
+                if (__any_sync(0xFFFFFFFFu, move)) {
+                    const float to = move ? mrow : m, alpha = move ? sa_exp2(m - to) : 1.0f;
+                    m = to;
+                    l *= alpha;
+                    if (turn > 0) {                      // the products so far are complete: S came behind them
+#pragma unroll
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            su_ld32(sp_o + c, o);
+                            su_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                            su_st32(sp_o + c, o);
+                        }
+                    }
+                }
+                const float use = m == -INFINITY ? 0.0f : m;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < 128; k += 2) {
+                    const float p0 = sa_exp2(fmaf(__uint_as_float(x[k]), a.scale2, -use));
+                    const float p1 = sa_exp2(fmaf(__uint_as_float(x[k + 1]), a.scale2, -use));
+                    sum[(k >> 1) & 3] += p0 + p1;
+                    x[k >> 1] = sa_pack<F16>(p0, p1);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                su_st32(sp_s, x);
+                su_st32(sp_s + 32, x + 32);
+                su_wait_st();
+                umma::fence_before();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pfull[s]);
+        }
+        // ---- outputs
+        const bool any = first < end;
+        if (any) ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(&ofull[s], 0, a.status, SUE_O));
+        umma::fence_after();
+        const SaArgs &a0 = a;
+        auto row_of = [t, ap = &a0](int blk, int j, bool values) -> const uint16_t * {
+            const SaArgs &a = *ap;
+            const bool vv = values && a.v != nullptr;
+            if (TREE && blk < t.nblk_c) {
+                const int key = t.key0 + blk * SU_BN + j;
+                return key < t.kend ? sa_cached(a, t, vv ? a.vc : a.kc, key, D) : nullptr;
+            }
+            const int key = (TREE ? blk - t.nblk_c : blk) * SU_BN + j;
+            if (key >= t.len) return nullptr;
+            return reinterpret_cast<const uint16_t *>(vv ? a.v : a.k) + (size_t)(t.begin + key) * (vv ? a.ldv : a.ldk) +
+                   (size_t)t.kvh * D;
+        };
+        auto sees = [t, row_of, ap = &a0, dp = &s_depth[0], an = &s_anc[0]](int tok, int blk, int j) -> bool {
+            const SaArgs &a = *ap;
+            if constexpr (TREE) {
+                if (blk < t.nblk_c) {
+                    const int key = t.key0 + blk * SU_BN + j;
+                    return key < t.kend && t.ctx - key + dp[tok] < a.window && row_of(blk, j, false) != nullptr;
+                }
+                const int x = (blk - t.nblk_c) * SU_BN + j;
+                return x < t.len && (an[tok][x >> 5] >> (x & 31) & 1) && dp[tok] - dp[x] < a.window;
+            } else {
+                const int key = blk * SU_BN + j;
+                return key <= tok && tok - key < a.window;
+            }
+        };
+        if (alt) {
+            // the odd blocks' rows go through shared memory (every product has
+            // read its operands) to the even blocks' threads
+            constexpr int OS = D + 4;
+            float *xo = reinterpret_cast<float *>(ks), *xm = xo + 128 * OS, *xl = xm + 128;
+            const bool two = f1 < e1;
+            if (s && two) ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(&ofull[0], 0, a.status, SUE_O));
+            if (s && two && live) {
+#pragma unroll
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    su_ld32(sp_o + c, o);
+                    su_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4)
+                        *reinterpret_cast<uint4 *>(xo + i * OS + c + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                }
+                xm[i] = m;
+                xl[i] = l;
+            }
+            su_bar<256>(1);
+            if (s_odd[0] | s_odd[1]) {
+                serve_slow_rows<D, F16, false>(a, t, SU_BN, warp - 4, 8, sees, row_of);
+            } else if (s == 0 && live) {
+                float f_a = 1.0f, f_b = 0.0f;
+                if (two) {
+                    const float mb = xm[i], top = fmaxf(m, mb), use = top == -INFINITY ? 0.0f : top;
+                    f_a = sa_exp2(m - use);
+                    f_b = sa_exp2(mb - use);
+                    l = l * f_a + xl[i] * f_b;
+                    m = top;
+                }
+                const bool part = t.parts > 1;
+                const float inv = part ? 1.0f : sa_inv(l, m, a.sink, head);
+                const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + tok) * a.hq + head;
+                const size_t at = (size_t)(t.begin + tok) * a.ldo + (size_t)head * D;
+                if (part && i < rows) {
+                    a.pm[id] = m;
+                    a.pl[id] = l;
+                }
+#pragma unroll
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    su_ld32(sp_o + c, o);
+                    su_wait_ld();
+                    float y[32];
+#pragma unroll
+                    for (int k = 0; k < 32; k++) {
+                        y[k] = __uint_as_float(o[k]) * f_a;
+                        if (two) y[k] = fmaf(xo[i * OS + c + k], f_b, y[k]);
+                        y[k] *= inv;
+                    }
+                    if (i < rows) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8) {
+                            if (part) {
+                                float4 *d = reinterpret_cast<float4 *>(a.po + id * D + c + k);
+                                d[0] = make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]);
+                                d[1] = make_float4(y[k + 4], y[k + 5], y[k + 6], y[k + 7]);
+                            } else {
+                                *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.o) + at + c + k) =
+                                    make_uint4(sa_pack<F16>(y[k], y[k + 1]), sa_pack<F16>(y[k + 2], y[k + 3]),
+                                               sa_pack<F16>(y[k + 4], y[k + 5]), sa_pack<F16>(y[k + 6], y[k + 7]));
+                            }
+                        }
+                    }
+                }
+            }
+        } else {
+            su_bar<128>(2 + s);                          // every warp's finding in s_odd
+            if (s_odd[s]) {
+                SaTile ts = t;
+                ts.r0 = t.r0 + row0;
+                ts.rows = rows;
+                ts.blk0 = first;
+                ts.blk1 = end;
+                serve_slow_rows<D, F16, false>(a, ts, SU_BN, warp & 3, 4, sees, row_of);
+            } else if (live) {
+                const bool part = t.parts > 1;
+                const float inv = part ? 1.0f : sa_inv(l, m, a.sink, head);
+                const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + tok) * a.hq + head;
+                const size_t at = (size_t)(t.begin + tok) * a.ldo + (size_t)head * D;
+                if (part && i < rows) {
+                    a.pm[id] = m;
+                    a.pl[id] = l;
+                }
+#pragma unroll
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    su_ld32(sp_o + c, o);
+                    su_wait_ld();
+                    if (i < rows) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8) {
+                            float y[8];
+#pragma unroll
+                            for (int e = 0; e < 8; e++) y[e] = __uint_as_float(o[k + e]) * inv;
+                            if (part) {
+                                float4 *d = reinterpret_cast<float4 *>(a.po + id * D + c + k);
+                                d[0] = make_float4(y[0], y[1], y[2], y[3]);
+                                d[1] = make_float4(y[4], y[5], y[6], y[7]);
+                            } else {
+                                *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.o) + at + c + k) =
+                                    make_uint4(sa_pack<F16>(y[0], y[1]), sa_pack<F16>(y[2], y[3]),
+                                               sa_pack<F16>(y[4], y[5]), sa_pack<F16>(y[6], y[7]));
+                            }
+                        }
+                    }
+                }
+            }
+        }
+    }
+    umma::fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        umma::fence_after();
+        umma::tmem_dealloc(tmem, 512);
+    }
+}
+
+// Map of a [rows][heads][D] 16-bit tensor, boxes of 64 columns x 1 head x box_rows rows.
+static inline int su_map(CUtensorMap *map, const void *base, int D, int heads, int64_t rows, long ld, int box_rows,
+                         bool f16)
+{
+    return tmap_encode_rows(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, D, heads,
+                            rows, (uint64_t)D * 2, (uint64_t)ld * 2, 64, box_rows);
+}
+
+template <int D, bool F16>
+int serve_umma_launch(SaArgs a, bool tree, cudaStream_t st)
+{
+    constexpr int KVB = D / 64 * SU_SUB;
+    int r;
+    CUtensorMap mk, mv, mkc, mvc;
+    if ((r = su_map(&mk, a.k, D, a.hkv, a.nt, a.ldk, SU_BN, F16))) return r;
+    if ((r = su_map(&mv, a.v ? a.v : a.k, D, a.hkv, a.nt, a.v ? a.ldv : a.ldk, SU_BN, F16))) return r;
+    mkc = mk;
+    mvc = mv;
+    dim3 grid;
+    if (tree) {
+        a.box_log2 = a.page_log2 < 7 ? a.page_log2 : 7;
+        if (a.n_pages > 0) {
+            const int64_t slots = (int64_t)a.n_pages * a.page_size;
+            const long row = (long)a.hkv * D;
+            if ((r = su_map(&mkc, a.kc, D, a.hkv, slots, row, 1 << a.box_log2, F16))) return r;
+            if ((r = su_map(&mvc, a.vc ? a.vc : a.kc, D, a.hkv, slots, row, 1 << a.box_log2, F16))) return r;
+        }
+        grid = dim3(a.row_tiles * a.splits, a.hkv, a.n_req);
+    } else {
+        a.two = 1;
+        const int64_t tiles = (int64_t)a.nt * a.G / 256 + min(a.n_req, a.nt);
+        if (tiles > INT_MAX) return dsv4cu_set_error(DSV4CU_ERR_ARG, "prompt_attn: %lld row tiles", (long long)tiles);
+        grid = dim3((unsigned)tiles, a.hkv, 1);
+    }
+    a.nst = min(SU_MAX_STAGES, (SA_SMEM_MAX - (a.two ? 2 : 1) * KVB) / (2 * KVB));
+    const size_t smem = (size_t)((a.two ? 2 : 1) + 2 * a.nst) * KVB + 1024;
+    auto kern = tree ? serve_umma_kernel<D, F16, true> : serve_umma_kernel<D, F16, false>;
+    static SmemLimit lim[2];
+    DSV4CU_CUDA_TRY(smem_limit(lim[tree], (const void *)kern, (int)smem));
+    // the warps' register shares are taken from what the block is launched with
+    static int regs[2];
+    if (!regs[tree]) {
+        cudaFuncAttributes f;
+        DSV4CU_CUDA_TRY(cudaFuncGetAttributes(&f, (const void *)kern));
+        regs[tree] = f.numRegs;
+    }
+    if (regs[tree] * SU_THREADS < SU_REGS_FEW * 128 + SU_REGS_MANY * 256)
+        return dsv4cu_set_error(DSV4CU_ERR_UNSUPPORTED, "serving attention: launched with %d registers a thread", regs[tree]);
+    kern<<<grid, SU_THREADS, smem, st>>>(mk, mv, mkc, mvc, a);
+    DSV4CU_LAUNCH_CHECK();
+    return tree && a.splits > 1 ? serve_join_launch<D, F16, false>(a, SU_BN, st) : DSV4CU_OK;
+}
+
+int serve_umma_bf16(const SaArgs &a, int D, bool tree, cudaStream_t st);
+int serve_umma_f16(const SaArgs &a, int D, bool tree, cudaStream_t st);
+
+}  // namespace dsv4cu

@@ -43,6 +43,19 @@ int tmap_encode_2d(CUtensorMap *map, CUtensorMapDataType type, const void *base,
     return DSV4CU_OK;
 }
 
+int tmap_encode_rows(CUtensorMap *map, CUtensorMapDataType type, const void *base, uint64_t cols, uint64_t heads,
+                     uint64_t rows, uint64_t head_bytes, uint64_t row_bytes, uint32_t box_cols, uint32_t box_rows)
+{
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return dsv4cu_set_error(DSV4CU_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    cuuint64_t dims[3] = {cols, heads, rows}, strides[2] = {head_bytes, row_bytes};
+    cuuint32_t box[3] = {box_cols, 1, box_rows}, es[3] = {1, 1, 1};
+    CUresult r = enc(map, type, 3, const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return dsv4cu_set_error(DSV4CU_ERR_CUDA, "cuTensorMapEncodeTiled(rows): %d", (int)r);
+    return DSV4CU_OK;
+}
+
 bool tmap_weights_ok(const dsv4cu_qmat *q)
 {
     const int rb = row_bytes_of(q->wdt, q->cols);

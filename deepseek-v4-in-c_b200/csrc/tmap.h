@@ -30,4 +30,9 @@ int tmap_encode(const dsv4cu_qmat *q, CUtensorMap *wmap, CUtensorMap *smap, int 
 int tmap_encode_2d(CUtensorMap *map, CUtensorMapDataType type, const void *base, uint64_t inner, uint64_t outer,
                    uint64_t row_bytes, uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle);
 
+// A [rows][heads][cols] map with boxes of box_cols columns of one head over
+// box_rows rows, 128-byte swizzle, zero fill outside the tensor.
+int tmap_encode_rows(CUtensorMap *map, CUtensorMapDataType type, const void *base, uint64_t cols, uint64_t heads,
+                     uint64_t rows, uint64_t head_bytes, uint64_t row_bytes, uint32_t box_cols, uint32_t box_rows);
+
 }  // namespace dsv4cu
