@@ -132,8 +132,7 @@ static TreeShape tree_shape(const dsv4cu_ctx *ctx, const dsv4cu_tree_attn_args *
     s.umma = use_umma(a, c);
     const int64_t rows = (int64_t)a->max_nodes * (a->n_heads / a->n_kv);
     s.two = s.umma && rows > 128;
-    const int BM = s.umma ? (s.two ? 256 : 128) : a->head_dim <= 128 ? 64 : 32;
-    const int BN = s.umma ? 128 : a->head_dim <= 128 ? 64 : 32;
+    const int BM = s.umma ? (s.two ? 256 : 128) : SA_BM, BN = s.umma ? 128 : sa_block(a->head_dim, a->v == nullptr);
     s.row_tiles = (int)((rows + BM - 1) / BM);
     const int64_t ctas = (int64_t)s.row_tiles * a->n_kv * a->n_req;
     const int seen = a->window && a->window < a->max_ctx ? a->window : a->max_ctx;

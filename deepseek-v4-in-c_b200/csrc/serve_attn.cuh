@@ -1,35 +1,38 @@
-// serve_attn.cuh - softmax attention of packed queries on mma.sync tiles, for
-// packed prompts and for trees of drafted tokens over a paged cache.
+// serve_attn.cuh - softmax attention of packed queries, for packed prompts and
+// for trees of drafted tokens over a paged cache: what the two kernels share
+// (masks, rows, splits and their join) and the mma.sync kernel, which covers
+// every head dim, fp32 queries and any page size.
 //
 //   o_i = sum_{j in M(i)} e_ij v_j / (sum_{j in M(i)} e_ij + e^sink / e^m_i),
 //   e_ij = exp(scale q_i.k_j - m_i), m_i the running maximum over M(i).
 //
-// A tile is BM rows of one key head: row r is (token r / G, head r % G) of the
+// A tile is 32 rows of one key head: row r is (token r / G, head r % G) of the
 // G query heads that share it, so grouped heads read a key once. The keys come
 // in blocks of BN through cp.async into 16-byte-swizzled shared memory, two
-// stages ahead where they fit; scores, the softmax statistics (fp32, exp2 of
-// log2-scaled scores) and the output stay in registers over one pass.
-//
-// Warps: WM x WN. WM splits the rows. With WN = 1 a warp owns its rows' whole
-// score strip and output, and the weights go from the score accumulators to
-// the second product's operand without leaving registers. Head dims above
-// 128 do not fit that (an output row of 512 columns is 256 registers a thread
-// at 16 rows), so there WN warps share the rows: each scores BN / WN keys over
-// the whole head dim, row maxima and weights cross through shared memory, and
-// each accumulates D / WN output columns.
+// stages where they fit. The NW warps of a CTA each own D / NW of the head's
+// dims for the whole pass - of the queries (mma fragments in registers), of
+// the scores' contraction, and of the output's columns - so a head dim of 512
+// needs no more than 255 registers a thread, and where the values are the key
+// rows (this engine's latent cache) a warp reads the same slice of the same
+// tile for both products. Per block: partial scores over the warp's dims to
+// shared memory, their sum and the softmax by THREADS / 32 threads per row, the
+// weights back through shared memory, then the output.
 //
 // fp32 queries (TERMS = 3) over a bf16 cache enter as three bf16 terms
 // q = t0 + t1 + t2, which carry all 24 significand bits, and so do the
-// weights: products are those of fp32 and only the fp32 accumulation rounds.
-// 16-bit queries use the weights rounded to the cache's type (2^-9 of each
-// weight in bf16, 2^-12 in f16: the size of the output's own rounding).
+// weights: products are those of fp32. 16-bit queries use the weights rounded
+// to the cache's type (2^-9 of each weight in bf16, 2^-12 in f16: the size of
+// the output's own rounding). The tensor core's own additions cut off low bits
+// (toward zero, so they do not average out), therefore it only adds within a
+// block; blocks are added in fp32 with rounding to nearest.
 //
 // Masked entries: a masked score is -inf whatever its key holds. A masked
 // value row is multiplied by a weight of exactly 0, which is only harmless
 // when the value is finite; blocks that a mask crosses (with three weight terms,
-// whose last ones may be 0, all blocks) look for non-finite values, and a tile that meets one is computed again by serve_slow_rows,
-// which touches visible keys only. Rows outside a sequence and pages outside
-// the pool arrive as zeros (cp.async with a source size of 0) and are masked.
+// whose last ones may be 0, all blocks) look for non-finite values, and a tile
+// that meets one is computed again by serve_slow_rows, which touches visible
+// keys only. Rows outside a sequence and pages outside the pool arrive as zeros
+// (cp.async with a source size of 0) and are masked.
 #pragma once
 
 #include <limits.h>
@@ -311,28 +314,32 @@ __device__ __noinline__ void serve_slow_rows(const SaArgs &a, const SaTile &t, i
     }
 }
 
-template <int D, int WM, int WN, int BN, int TERMS, bool F16, bool TREE>
-__global__ void __launch_bounds__(32 * WM * WN) serve_attn_kernel(const __grid_constant__ SaArgs a)
+constexpr int SA_BM = 32;             // rows of a tile
+constexpr int sa_warps(int D) { return D >= 128 ? 8 : 4; }
+
+template <int D, int BN, int TERMS, bool F16, bool TREE>
+__global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const __grid_constant__ SaArgs a)
 {
-    constexpr int BM = 16 * WM, THREADS = 32 * WM * WN, C16 = D / 8;
-    constexpr int KW = BN / WN, NT = KW / 8;             // keys and score n tiles of a warp
-    constexpr int DW = D / WN, ON = DW / 8;              // output columns and n tiles of a warp
-    constexpr int PS = BN + 8;
+    constexpr int NW = sa_warps(D), THREADS = 32 * NW, BM = SA_BM, C16 = D / 8;
+    constexpr int DW = D / NW, KS = DW / 16, ON = DW / 8;   // dims of a warp, their k steps, their output n tiles
+    constexpr int OG = ON < 4 ? ON : 4;                  // output n tiles accumulated at a time
+    constexpr int SS = BN + 8, PS = BN + 8;              // row strides of partial scores and weights
+    constexpr int TPR = THREADS / BM, CPT = BN / TPR;    // softmax: threads per row, columns per thread
     constexpr bool QF32 = TERMS > 1;
     static_assert(!(QF32 && F16), "three terms are bf16 terms");
+    static_assert(KS >= 1 && ON % OG == 0 && OG % 2 == 0 && CPT % 4 == 0, "shape");
     extern __shared__ __align__(128) uint16_t sa_sm[];
     __shared__ int s_par[TREE ? SA_MAX_NODES : 1], s_depth[TREE ? SA_MAX_NODES : 1];
     __shared__ unsigned long long s_anc[TREE ? SA_MAX_NODES : 1][2];
-    __shared__ int s_bad[2];
-    __shared__ uint8_t s_there[2][BN];
-    __shared__ float s_red[WN][BM];
+    __shared__ const uint16_t *s_row[2][2][BN];          // [slot][keys, values]: rows of a block, NULL outside
+    __shared__ int s_bad[2];                             // block with a missing row
+    __shared__ float s_alpha[BM], s_m[BM], s_l[BM];
     const bool shared_v = a.v == nullptr;
-    uint16_t *qs = sa_sm;                                // [TERMS][BM][D]
-    uint16_t *kvs = qs + TERMS * BM * D;                 // [nst][shared_v ? 1 : 2][BN][D]
     const int stage_el = (shared_v ? 1 : 2) * BN * D;
-    uint16_t *ps = kvs + a.nst * stage_el;               // [TERMS][BM][PS], WN > 1
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp % WM, wn = warp / WM;
-    const int g = lane >> 2, c = lane & 3;
+    uint16_t *kvs = sa_sm;                               // [nst][shared_v ? 1 : 2][BN][D]
+    float *part = reinterpret_cast<float *>(kvs + a.nst * stage_el);   // [NW][BM][SS]
+    uint16_t *ps = reinterpret_cast<uint16_t *>(part + NW * BM * SS);  // [TERMS][BM][PS]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
 
     // ---- which rows and keys
     SaTile t;
@@ -341,7 +348,7 @@ __global__ void __launch_bounds__(32 * WM * WN) serve_attn_kernel(const __grid_c
     t.table = nullptr;
     t.kvh = blockIdx.y;
     if constexpr (TREE) {
-        const int b = blockIdx.z, tile = blockIdx.x % a.row_tiles;
+        const int b = blockIdx.z;
         const SaSpan sp = sa_span(a, b, BN);
         t.split = blockIdx.x / a.row_tiles;
         t.begin = sp.begin;
@@ -352,7 +359,7 @@ __global__ void __launch_bounds__(32 * WM * WN) serve_attn_kernel(const __grid_c
         }
         if (t.split >= sp.used) return;
         t.parts = sp.used;
-        t.r0 = tile * BM;
+        t.r0 = blockIdx.x % a.row_tiles * BM;
         t.ctx = sp.ctx;
         t.kend = sp.kend;
         t.table = a.table + (size_t)b * a.max_pages;
@@ -376,7 +383,7 @@ __global__ void __launch_bounds__(32 * WM * WN) serve_attn_kernel(const __grid_c
     }
     if constexpr (TREE) {
         // ancestors-or-self as bit sets, depths; a parent that does not come
-        // before its child counts as the root's (none)
+        // before its child counts as none
         for (int i = tid; i < t.len; i += THREADS) s_par[i] = __ldg(a.parent + t.begin + i);
         __syncthreads();
         for (int i = tid; i < t.len; i += THREADS) {
@@ -393,8 +400,6 @@ __global__ void __launch_bounds__(32 * WM * WN) serve_attn_kernel(const __grid_c
             s_anc[i][1] = set[1];
             s_depth[i] = d;
         }
-        if (tid < 2) s_bad[tid] = -1;
-        __syncthreads();
     }
     // a key of block blk: its address, and whether token tok sees it (by
     // value: the fallback's call must not pin the tile to local memory)
@@ -425,67 +430,80 @@ __global__ void __launch_bounds__(32 * WM * WN) serve_attn_kernel(const __grid_c
             return key <= tok && tok - key < a.window;
         }
     };
+    // rows of block blk into slot blk & 1 (a barrier before their use)
+    auto find_rows = [&](int blk) {
+        if (tid < BN) {
+            const uint16_t *k = row(blk, tid, false);
+            s_row[blk & 1][0][tid] = k;
+            if (!shared_v) s_row[blk & 1][1][tid] = row(blk, tid, true);
+            if (!k) s_bad[blk & 1] = blk;
+        }
+    };
     auto issue = [&](int blk) {
-        const int st = (blk - t.blk0) % a.nst;
-        uint16_t *kd = kvs + st * stage_el;
-        for (int i = tid; i < BN * C16; i += THREADS) {
-            const int j = i / C16, ch = i - j * C16;
-            const uint16_t *k = row(blk, j, false);
+        uint16_t *kd = kvs + (a.nst == 2 ? blk & 1 : 0) * stage_el;
+        const int ch = tid % C16;
+#pragma unroll
+        for (int j = tid / C16; j < BN; j += THREADS / C16) {
+            const uint16_t *k = s_row[blk & 1][0][j];
             sa_cp16(sa_at<D>(kd, j, 8 * ch), k ? k + 8 * ch : (const uint16_t *)a.q, k != nullptr);
             if (!shared_v) {
-                const uint16_t *v = row(blk, j, true);
+                const uint16_t *v = s_row[blk & 1][1][j];
                 sa_cp16(sa_at<D>(kd + BN * D, j, 8 * ch), v ? v + 8 * ch : (const uint16_t *)a.q, v != nullptr);
-            }
-            if (TREE && ch == 0) {
-                s_there[st][j] = k != nullptr;
-                if (!k) s_bad[st] = blk;
             }
         }
         sa_commit();
     };
-    if (t.blk0 < t.blk1) issue(t.blk0);
-
-    // ---- queries, as terms of the cache's type
-    for (int i = tid; i < BM * C16; i += THREADS) {
-        const int r = i / C16, ch = i - r * C16;
-        uint4 w[TERMS];
-#pragma unroll
-        for (int x = 0; x < TERMS; x++) w[x] = make_uint4(0, 0, 0, 0);
-        if (r < t.rows) {
-            const int tok = (t.r0 + r) / a.G, head = t.kvh * a.G + (t.r0 + r) % a.G;
-            const size_t at = (size_t)(t.begin + tok) * a.ldq + (size_t)head * D + 8 * ch;
-            if constexpr (QF32) {
-                const float4 *p = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.q) + at);
-                const float4 x = __ldg(p), y = __ldg(p + 1);
-                const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    uint32_t s[TERMS];
-                    sa_split<TERMS, F16>(f[2 * e], f[2 * e + 1], s);
-#pragma unroll
-                    for (int x2 = 0; x2 < TERMS; x2++) reinterpret_cast<uint32_t *>(&w[x2])[e] = s[x2];
-                }
-            } else {
-                w[0] = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + at));
-            }
-        }
-#pragma unroll
-        for (int x = 0; x < TERMS; x++) *reinterpret_cast<uint4 *>(sa_at<D>(qs + x * BM * D, r, 8 * ch)) = w[x];
+    if (tid < 2) s_bad[tid] = -1;
+    if (tid < BM) {
+        s_m[tid] = -INFINITY;
+        s_l[tid] = 0.0f;
     }
+    __syncthreads();
+    find_rows(t.blk0);
+    if (t.blk0 + 1 < t.blk1) find_rows(t.blk0 + 1);
+    __syncthreads();
+    issue(t.blk0);
+
+    // ---- this warp's dims of the queries as mma fragments: rows g / g + 8 of
+    // m tile mt, dims DW * warp + 16 kk + 2c.. / 2c + 8..
+    uint32_t qa[2][KS][TERMS][4];
+#pragma unroll
+    for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int r = 16 * mt + g + 8 * h, pr = t.r0 + min(r, t.rows - 1), tok = pr / a.G, head = t.kvh * a.G + pr % a.G;
+            const size_t at = (size_t)(t.begin + tok) * a.ldq + (size_t)head * D + DW * warp + 2 * c;
+#pragma unroll
+            for (int kk = 0; kk < KS; kk++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    uint32_t w[TERMS];
+                    if constexpr (QF32) {
+                        const float2 x = __ldg(reinterpret_cast<const float2 *>(reinterpret_cast<const float *>(a.q) + at +
+                                                                                16 * kk + 8 * e));
+                        sa_split<TERMS, F16>(x.x, x.y, w);
+                    } else {
+                        w[0] = __ldg(reinterpret_cast<const uint32_t *>(reinterpret_cast<const uint16_t *>(a.q) + at +
+                                                                        16 * kk + 8 * e));
+                    }
+#pragma unroll
+                    for (int x = 0; x < TERMS; x++) qa[mt][kk][x][2 * e + h] = w[x];
+                }
+        }
 
     const int arow = (lane & 7) + 8 * ((lane >> 3) & 1), acol = 8 * (lane >> 4);
     const int brow = (lane & 7) + 8 * (lane >> 4), bcol = 8 * ((lane >> 3) & 1);
-    const bool live = 16 * wm < t.rows;                  // this warp has rows
-    int tok[2];
+    const int d0 = DW * warp;
+    const bool second = t.rows > 16;                     // rows 16 .. 31 exist
+    const int srow = tid / TPR, scol = (tid % TPR) * CPT, stok = (t.r0 + min(srow, t.rows - 1)) / a.G;
+    float o[2][ON][4];
 #pragma unroll
-    for (int h = 0; h < 2; h++) tok[h] = (t.r0 + min(t.rows - 1, 16 * wm + g + 8 * h)) / a.G;
-    float o[ON][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    for (int mt = 0; mt < 2; mt++)
 #pragma unroll
-    for (int n = 0; n < ON; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-    bool odd = false;                                    // met a non-finite value in a masked block
+        for (int n = 0; n < ON; n++) o[mt][n][0] = o[mt][n][1] = o[mt][n][2] = o[mt][n][3] = 0.0f;
+    bool odd = false;                                    // met a non-finite value that a mask or a zero term meets
 
     for (int blk = t.blk0; blk < t.blk1; blk++) {
-        const int st = (blk - t.blk0) % a.nst;
         if (a.nst == 2 && blk + 1 < t.blk1) {
             issue(blk + 1);
             sa_wait<1>();
@@ -493,224 +511,173 @@ __global__ void __launch_bounds__(32 * WM * WN) serve_attn_kernel(const __grid_c
             sa_wait<0>();
         }
         __syncthreads();
-        uint16_t *kt = kvs + st * stage_el, *vt = shared_v ? kt : kt + BN * D;
+        uint16_t *kt = kvs + (a.nst == 2 ? blk & 1 : 0) * stage_el, *vt = shared_v ? kt : kt + BN * D;
         bool full;
         if constexpr (TREE) {
             const int e = t.key0 + (blk + 1) * BN;
-            full = blk < t.nblk_c && e <= t.kend && s_bad[st] != blk && t.ctx + t.len - (e - BN) <= a.window;
+            full = blk < t.nblk_c && e <= t.kend && s_bad[blk & 1] != blk && t.ctx + t.len - (e - BN) <= a.window;
         } else {
             full = (blk + 1) * BN - 1 <= t_lo && t_hi - blk * BN < a.window;
         }
-        float s[NT][4];
-        if (live) {
+        // ---- partial scores over the warp's dims
 #pragma unroll
-            for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-            if constexpr (NT >= 2) {
+        for (int n = 0; n < BN / 8; n += 2) {
+            float s[2][2][4] = {};
 #pragma unroll
-                for (int kk = 0; kk < D / 16; kk++) {
-                    uint32_t qa[TERMS][4];
+            for (int kk = 0; kk < KS; kk++) {
+                uint32_t b[4];
+                sa_ldsm4(b, sa_at<D>(kt, 8 * n + brow, d0 + 16 * kk + bcol));
 #pragma unroll
-                    for (int x = 0; x < TERMS; x++) sa_ldsm4(qa[x], sa_at<D>(qs + x * BM * D, 16 * wm + arow, 16 * kk + acol));
+                for (int x = TERMS - 1; x >= 0; x--)
 #pragma unroll
-                    for (int n = 0; n < NT; n += 2) {
-                        uint32_t b[4];
-                        sa_ldsm4(b, sa_at<D>(kt, KW * wn + 8 * n + brow, 16 * kk + bcol));
-#pragma unroll
-                        for (int x = TERMS - 1; x >= 0; x--) {
-                            sa_mma<F16>(s[n], qa[x], b[0], b[1]);
-                            sa_mma<F16>(s[n + 1], qa[x], b[2], b[3]);
+                    for (int mt = 0; mt < 2; mt++)
+                        if (mt == 0 || second) {
+                            sa_mma<F16>(s[mt][0], qa[mt][kk][x], b[0], b[1]);
+                            sa_mma<F16>(s[mt][1], qa[mt][kk][x], b[2], b[3]);
                         }
-                    }
-                }
-            } else {                                     // one n tile: four 8-wide k pieces per load
-#pragma unroll
-                for (int k2 = 0; k2 < D / 32; k2++) {
-                    uint32_t b[4];
-                    sa_ldsm4(b, sa_at<D>(kt, KW * wn + (lane & 7), 32 * k2 + 8 * (lane >> 3)));
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-#pragma unroll
-                        for (int x = TERMS - 1; x >= 0; x--) {
-                            uint32_t qa[4];
-                            sa_ldsm4(qa, sa_at<D>(qs + x * BM * D, 16 * wm + arow, 32 * k2 + 16 * h + acol));
-                            sa_mma<F16>(s[0], qa, b[2 * h], b[2 * h + 1]);
-                        }
-                    }
-                }
             }
-            // ---- scaled scores and their row maxima
-            float top[2] = {-INFINITY, -INFINITY};
+            float *dst = part + (warp * BM + g) * SS + 8 * n + 2 * c;
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int mt = 0; mt < 2; mt++)
+                if (mt == 0 || second)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float x = s[n][e] * a.scale2;
-                    if (!full) {
-                        const int j = KW * wn + 8 * n + 2 * c + (e & 1);
-                        bool see;
-                        if constexpr (TREE) {
-                            if (blk < t.nblk_c)
-                                see = s_there[st][j] && t.ctx - (t.key0 + blk * BN + j) + s_depth[tok[e >> 1]] < a.window;
-                            else
-                                see = vis(tok[e >> 1], blk, j);
-                        } else {
-                            see = vis(tok[e >> 1], blk, j);
-                        }
-                        if (!see) x = -INFINITY;
+                    for (int u = 0; u < 2; u++) {
+                        *reinterpret_cast<float2 *>(dst + 16 * mt * SS + 8 * u) = make_float2(s[mt][u][0], s[mt][u][1]);
+                        *reinterpret_cast<float2 *>(dst + (16 * mt + 8) * SS + 8 * u) = make_float2(s[mt][u][2], s[mt][u][3]);
                     }
-                    s[n][e] = x;
-                    top[e >> 1] = fmaxf(top[e >> 1], x);
-                }
+        }
+        __syncthreads();
+        // ---- the row's scores (warp order), softmax
+        {
+            float x[CPT];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                top[h] = fmaxf(top[h], __shfl_xor_sync(0xFFFFFFFFu, top[h], 1));
-                top[h] = fmaxf(top[h], __shfl_xor_sync(0xFFFFFFFFu, top[h], 2));
+            for (int e = 0; e < CPT; e += 4) {
+                float4 y = *reinterpret_cast<const float4 *>(part + srow * SS + scol + e);
+#pragma unroll
+                for (int w = 1; w < NW; w++) {
+                    const float4 z = *reinterpret_cast<const float4 *>(part + (w * BM + srow) * SS + scol + e);
+                    y.x += z.x;
+                    y.y += z.y;
+                    y.z += z.z;
+                    y.w += z.w;
+                }
+                x[e] = y.x;
+                x[e + 1] = y.y;
+                x[e + 2] = y.z;
+                x[e + 3] = y.w;
             }
-            if constexpr (WN > 1) {
-                if (c == 0) {
-                    s_red[wn][16 * wm + g] = top[0];
-                    s_red[wn][16 * wm + g + 8] = top[1];
+            float top = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < CPT; e++) {
+                x[e] *= a.scale2;
+                if (!full) {
+                    bool see;
+                    if (TREE && blk < t.nblk_c)
+                        see = s_row[blk & 1][0][scol + e] != nullptr &&
+                              t.ctx - (t.key0 + blk * BN + scol + e) + s_depth[stok] < a.window;
+                    else
+                        see = vis(stok, blk, scol + e);
+                    if (!see) x[e] = -INFINITY;
                 }
-            } else {
-                s_red[0][0] = 0.0f;                      // unused
+                top = fmaxf(top, x[e]);
             }
-            if constexpr (WN == 1) {
 #pragma unroll
-                for (int h = 0; h < 2; h++) top[h] = fmaxf(top[h], m[h]);
+            for (int d = 1; d < TPR; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+            const float old = s_m[srow], m = fmaxf(old, top), use = m == -INFINITY ? 0.0f : m;
+            float sum = 0.0f;
+            uint32_t w[TERMS][CPT / 2];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const float use = top[h] == -INFINITY ? 0.0f : top[h], alpha = sa_exp2(m[h] - use);
-                    m[h] = top[h];
-                    l[h] *= alpha;
+            for (int e = 0; e < CPT; e += 2) {
+                const float y = sa_exp2(x[e] - use), z = sa_exp2(x[e + 1] - use);
+                sum += y + z;
+                uint32_t p[TERMS];
+                sa_split<TERMS, F16>(y, z, p);
 #pragma unroll
-                    for (int n = 0; n < ON; n++) {
-                        o[n][2 * h] *= alpha;
-                        o[n][2 * h + 1] *= alpha;
-                    }
+                for (int i = 0; i < TERMS; i++) w[i][e / 2] = p[i];
+            }
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
+            for (int i = 0; i < TERMS; i++)
 #pragma unroll
-                        for (int e = 2 * h; e < 2 * h + 2; e++) {
-                            s[n][e] = sa_exp2(s[n][e] - use);
-                            l[h] += s[n][e];
-                        }
-                }
+                for (int e = 0; e < CPT / 2; e += 2)
+                    *reinterpret_cast<uint2 *>(ps + (i * BM + srow) * PS + scol + 2 * e) = make_uint2(w[i][e], w[i][e + 1]);
+#pragma unroll
+            for (int d = 1; d < TPR; d <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+            if (tid % TPR == 0) {
+                const float alpha = sa_exp2(old - use);
+                s_alpha[srow] = alpha;
+                s_m[srow] = m;
+                s_l[srow] = s_l[srow] * alpha + sum;
             }
         }
-        if constexpr (WN > 1) {
-            __syncthreads();
-            if (live) {
+        __syncthreads();
+        // ---- output
+        const float al[2][2] = {{s_alpha[g], s_alpha[g + 8]}, {s_alpha[g + 16], s_alpha[g + 24]}};
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    float top = m[h];
-#pragma unroll
-                    for (int w = 0; w < WN; w++) top = fmaxf(top, s_red[w][16 * wm + g + 8 * h]);
-                    const float use = top == -INFINITY ? 0.0f : top, alpha = sa_exp2(m[h] - use);
-                    m[h] = top;
-                    l[h] *= alpha;
-#pragma unroll
-                    for (int n = 0; n < ON; n++) {
-                        o[n][2 * h] *= alpha;
-                        o[n][2 * h + 1] *= alpha;
-                    }
-#pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        const float x = sa_exp2(s[n][2 * h] - use), y = sa_exp2(s[n][2 * h + 1] - use);
-                        l[h] += x + y;
-                        uint32_t w[TERMS];
-                        sa_split<TERMS, F16>(x, y, w);
-#pragma unroll
-                        for (int i = 0; i < TERMS; i++)
-                            *reinterpret_cast<uint32_t *>(ps + (i * BM + 16 * wm + g + 8 * h) * PS + KW * wn + 8 * n +
-                                                          2 * c) = w[i];
-                    }
-                }
-            }
-            __syncthreads();
-        }
-        if (live) {
+        for (int n0 = 0; n0 < ON; n0 += OG) {
+            float acc[2][OG][4] = {};
 #pragma unroll
             for (int kk = 0; kk < BN / 16; kk++) {
-                uint32_t pa[TERMS][4];
-                if constexpr (WN > 1) {
+                uint32_t b[OG / 2][4];
 #pragma unroll
-                    for (int x = 0; x < TERMS; x++) sa_ldsm4(pa[x], ps + (x * BM + 16 * wm + arow) * PS + 16 * kk + acol);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {        // rows g / g + 8, keys 2c.. / 2c + 8..
-                        uint32_t w[TERMS];
-                        const int n = (2 * kk + (e >> 1)) % NT;
-                        sa_split<TERMS, F16>(s[n][2 * (e & 1)], s[n][2 * (e & 1) + 1], w);
-#pragma unroll
-                        for (int x = 0; x < TERMS; x++) pa[x][e] = w[x];
-                    }
-                }
-#pragma unroll
-                for (int n = 0; n < ON; n += 2) {
-                    uint32_t b[4];
-                    sa_ldsm4_t(b, sa_at<D>(vt, 16 * kk + arow, DW * wn + 8 * n + acol));
+                for (int n = 0; n < OG / 2; n++) {
+                    sa_ldsm4_t(b[n], sa_at<D>(vt, 16 * kk + arow, d0 + 8 * n0 + 16 * n + acol));
                     if (TERMS > 1 || !full)              // a weight's zero terms times infinity are NaN as well
-                        odd = odd || sa_nonfinite<F16>(b[0]) || sa_nonfinite<F16>(b[1]) || sa_nonfinite<F16>(b[2]) ||
-                              sa_nonfinite<F16>(b[3]);
-#pragma unroll
-                    for (int x = TERMS - 1; x >= 0; x--) {
-                        sa_mma<F16>(o[n], pa[x], b[0], b[1]);
-                        sa_mma<F16>(o[n + 1], pa[x], b[2], b[3]);
-                    }
+                        odd = odd || sa_nonfinite<F16>(b[n][0]) || sa_nonfinite<F16>(b[n][1]) ||
+                              sa_nonfinite<F16>(b[n][2]) || sa_nonfinite<F16>(b[n][3]);
                 }
+#pragma unroll
+                for (int mt = 0; mt < 2; mt++)
+                    if (mt == 0 || second)
+#pragma unroll
+                        for (int x = TERMS - 1; x >= 0; x--) {
+                            uint32_t pa[4];
+                            sa_ldsm4(pa, ps + (x * BM + 16 * mt + arow) * PS + 16 * kk + acol);
+#pragma unroll
+                            for (int n = 0; n < OG; n++) sa_mma<F16>(acc[mt][n], pa, b[n / 2][2 * (n & 1)], b[n / 2][2 * (n & 1) + 1]);
+                        }
             }
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int n = 0; n < OG; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[mt][n0 + n][e] = fmaf(o[mt][n0 + n][e], al[mt][e >> 1], acc[mt][n][e]);
         }
-        __syncthreads();                                 // this stage and the weights are free
+        if (blk + 2 < t.blk1) find_rows(blk + 2);        // this block's rows are used up (its mask is read)
+        __syncthreads();                                 // this stage, the weights and s_alpha are free
         if (a.nst == 1 && blk + 1 < t.blk1) issue(blk + 1);
     }
     if (__syncthreads_or(odd)) {
-        serve_slow_rows<D, F16, QF32>(a, t, BN, warp, WM * WN, vis, row);
+        serve_slow_rows<D, F16, QF32>(a, t, BN, warp, NW, vis, row);
         return;
     }
-    // ---- exp-sums over the quad, and over the warps that share the rows
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
-    }
-    if constexpr (WN > 1) {
-        if (c == 0) {
-            s_red[wn][16 * wm + g] = l[0];
-            s_red[wn][16 * wm + g + 8] = l[1];
-        }
-        __syncthreads();
+    for (int mt = 0; mt < 2; mt++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            l[h] = 0.0f;
+            const int r = 16 * mt + g + 8 * h;
+            if (r >= t.rows) continue;
+            const int pr = t.r0 + r, tok = pr / a.G, head = t.kvh * a.G + pr % a.G, col = d0 + 2 * c;
+            if (t.parts > 1) {
+                const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + tok) * a.hq + head;
 #pragma unroll
-            for (int w = 0; w < WN; w++) l[h] += s_red[w][16 * wm + g + 8 * h];
-        }
-    }
+                for (int n = 0; n < ON; n++)
+                    *reinterpret_cast<float2 *>(a.po + id * D + col + 8 * n) = make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
+                if (warp == 0 && c == 0) {
+                    a.pm[id] = s_m[r];
+                    a.pl[id] = s_l[r];
+                }
+            } else {
+                const float inv = sa_inv(s_l[r], s_m[r], a.sink, head);
+                const size_t at = (size_t)(t.begin + tok) * a.ldo + (size_t)head * D + col;
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int r = 16 * wm + g + 8 * h;
-        if (r >= t.rows) continue;
-        const int head = t.kvh * a.G + (t.r0 + r) % a.G, col = DW * wn + 2 * c;
-        if (t.parts > 1) {
-            const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + tok[h]) * a.hq + head;
-#pragma unroll
-            for (int n = 0; n < ON; n++)
-                *reinterpret_cast<float2 *>(a.po + id * D + col + 8 * n) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-            if (wn == 0 && c == 0) {
-                a.pm[id] = m[h];
-                a.pl[id] = l[h];
-            }
-        } else {
-            const float inv = sa_inv(l[h], m[h], a.sink, head);
-            const size_t at = (size_t)(t.begin + tok[h]) * a.ldo + (size_t)head * D + col;
-#pragma unroll
-            for (int n = 0; n < ON; n++) {
-                const float x = o[n][2 * h] * inv, y = o[n][2 * h + 1] * inv;
-                if constexpr (QF32) *reinterpret_cast<float2 *>(reinterpret_cast<float *>(a.o) + at + 8 * n) = make_float2(x, y);
-                else *reinterpret_cast<uint32_t *>(reinterpret_cast<uint16_t *>(a.o) + at + 8 * n) = sa_pack<F16>(x, y);
+                for (int n = 0; n < ON; n++) {
+                    const float x = o[mt][n][2 * h] * inv, y = o[mt][n][2 * h + 1] * inv;
+                    if constexpr (QF32) *reinterpret_cast<float2 *>(reinterpret_cast<float *>(a.o) + at + 8 * n) = make_float2(x, y);
+                    else *reinterpret_cast<uint32_t *>(reinterpret_cast<uint16_t *>(a.o) + at + 8 * n) = sa_pack<F16>(x, y);
+                }
             }
         }
-    }
 }
 
 // Joins the splits of a tree's rows, a warp per row: the partial outputs
@@ -758,22 +725,18 @@ int serve_join_launch(const SaArgs &a, int BN, cudaStream_t st)
     return DSV4CU_OK;
 }
 
-// Tile shape of a head dim: rows, keys per block and warps.
-template <int D>
-struct SaShape {
-    static constexpr int WM = D <= 128 ? 4 : 2, WN = D <= 128 ? 1 : 4, BN = D <= 128 ? 64 : 32;
-    static constexpr int BM = 16 * WM;
-};
-
 constexpr int SA_SMEM_MAX = 220 * 1024;      // of 227 KB: the static arrays come on top
+// Keys of a block: 64, or 32 where keys and values of 512 dims are apart (two
+// stages of both then take the same 128 KB).
+static inline int sa_block(int D, bool shared_v) { return D == 512 && !shared_v ? 32 : 64; }
 
-template <int D, int TERMS, bool F16, bool TREE>
+template <int D, int BN, int TERMS, bool F16, bool TREE>
 int serve_attn_launch(SaArgs a, cudaStream_t st)
 {
-    using S = SaShape<D>;
-    auto kern = serve_attn_kernel<D, S::WM, S::WN, S::BN, TERMS, F16, TREE>;
-    const size_t stage = (size_t)(a.v ? 2 : 1) * S::BN * D * 2;
-    const size_t rest = (size_t)TERMS * S::BM * D * 2 + (S::WN > 1 ? (size_t)TERMS * S::BM * (S::BN + 8) * 2 : 0);
+    auto kern = serve_attn_kernel<D, BN, TERMS, F16, TREE>;
+    constexpr int NW = sa_warps(D);
+    const size_t stage = (size_t)(a.v ? 2 : 1) * BN * D * 2;
+    const size_t rest = (size_t)NW * SA_BM * (BN + 8) * 4 + (size_t)TERMS * SA_BM * (BN + 8) * 2;
     a.nst = rest + 2 * stage <= SA_SMEM_MAX ? 2 : 1;
     const size_t smem = rest + a.nst * stage;
     static SmemLimit lim;
@@ -782,13 +745,13 @@ int serve_attn_launch(SaArgs a, cudaStream_t st)
     if (TREE) {
         grid = dim3(a.row_tiles * a.splits, a.hkv, a.n_req);
     } else {
-        const int64_t tiles = (int64_t)a.nt * a.G / S::BM + min(a.n_req, a.nt);
+        const int64_t tiles = (int64_t)a.nt * a.G / SA_BM + min(a.n_req, a.nt);
         if (tiles > INT_MAX) return dsv4cu_set_error(DSV4CU_ERR_ARG, "prompt_attn: %lld row tiles", (long long)tiles);
         grid = dim3((unsigned)tiles, a.hkv, 1);
     }
-    kern<<<grid, 32 * S::WM * S::WN, smem, st>>>(a);
+    kern<<<grid, 32 * NW, smem, st>>>(a);
     DSV4CU_LAUNCH_CHECK();
-    if (TREE && a.splits > 1) return serve_join_launch<D, F16, (TERMS > 1)>(a, S::BN, st);
+    if (TREE && a.splits > 1) return serve_join_launch<D, F16, (TERMS > 1)>(a, BN, st);
     return DSV4CU_OK;
 }
 
@@ -797,14 +760,15 @@ int serve_attn_bf16(const SaArgs &a, int D, bool tree, cudaStream_t st);
 int serve_attn_f16(const SaArgs &a, int D, bool tree, cudaStream_t st);
 int serve_attn_f32(const SaArgs &a, int D, bool tree, cudaStream_t st);
 
-template <int TERMS, bool F16>
-int serve_attn_pick(const SaArgs &a, int D, bool tree, cudaStream_t st)
+template <int TERMS, bool F16, bool TREE>
+int serve_attn_pick(const SaArgs &a, int D, cudaStream_t st)
 {
     switch (D) {
-    case 64: return tree ? serve_attn_launch<64, TERMS, F16, true>(a, st) : serve_attn_launch<64, TERMS, F16, false>(a, st);
-    case 128: return tree ? serve_attn_launch<128, TERMS, F16, true>(a, st) : serve_attn_launch<128, TERMS, F16, false>(a, st);
-    case 256: return tree ? serve_attn_launch<256, TERMS, F16, true>(a, st) : serve_attn_launch<256, TERMS, F16, false>(a, st);
-    default: return tree ? serve_attn_launch<512, TERMS, F16, true>(a, st) : serve_attn_launch<512, TERMS, F16, false>(a, st);
+    case 64: return serve_attn_launch<64, 64, TERMS, F16, TREE>(a, st);
+    case 128: return serve_attn_launch<128, 64, TERMS, F16, TREE>(a, st);
+    case 256: return serve_attn_launch<256, 64, TERMS, F16, TREE>(a, st);
+    default:
+        return a.v ? serve_attn_launch<512, 32, TERMS, F16, TREE>(a, st) : serve_attn_launch<512, 64, TERMS, F16, TREE>(a, st);
     }
 }
 

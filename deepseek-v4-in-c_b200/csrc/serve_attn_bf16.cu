@@ -4,6 +4,6 @@
 namespace dsv4cu {
 int serve_attn_bf16(const SaArgs &a, int D, bool tree, cudaStream_t st)
 {
-    return serve_attn_pick<1, false>(a, D, tree, st);
+    return tree ? serve_attn_pick<1, false, true>(a, D, st) : serve_attn_pick<1, false, false>(a, D, st);
 }
 }  // namespace dsv4cu

@@ -4,6 +4,6 @@
 namespace dsv4cu {
 int serve_attn_f16(const SaArgs &a, int D, bool tree, cudaStream_t st)
 {
-    return serve_attn_pick<1, true>(a, D, tree, st);
+    return tree ? serve_attn_pick<1, true, true>(a, D, st) : serve_attn_pick<1, true, false>(a, D, st);
 }
 }  // namespace dsv4cu

@@ -17,10 +17,13 @@
 // order of the sums is the kernel's own, and it is fixed.
 //
 // One cluster per request, CTA r on the r-th slice of the vocabulary. Every
-// CTA walks the tree by itself (a few gathers of p and q); what needs the
-// whole row is a sum that each CTA takes over its slice and reads from the
-// others through distributed shared memory. A row is read once from memory
-// for its sum; the rescan that finds the token touches one warp's segment.
+// CTA walks the tree by itself: the probabilities of every node's token in its
+// parent's rows are gathered up front by a thread each, so the walk waits for
+// no memory. What needs the whole row is a sum that each CTA takes over its
+// slice and stores into the others' shared memory (one cluster barrier per
+// sum; two sets of slots, so the next sum does not disturb readers). A row
+// comes from memory once; later sums and the rescan of the one warp's segment
+// that holds the token find it in L2.
 #include <math.h>
 
 #include <cooperative_groups.h>
@@ -31,7 +34,8 @@ namespace dsv4cu {
 namespace cg = cooperative_groups;
 
 constexpr int VER_MAX_NODES = 128;
-constexpr int VER_THREADS = 512;
+constexpr int VER_THREADS = 256;
+constexpr int VER_BATCH = 16;         // loads a lane has in flight
 constexpr int VER_WARPS = VER_THREADS / 32;
 constexpr int VER_CL = 8;             // CTAs per request: the largest portable cluster
 enum { VER_BAD_TREE = 76 };           // more than VER_MAX_NODES nodes (dsv4cu_ctx_status)
@@ -116,52 +120,75 @@ __global__ void __launch_bounds__(128) verify_greedy_kernel(const VerifyArgs a)
     ver_write(a, b, begin, n, line[warp], acc, lane, 32);
 }
 
-// The remainder of the current row after the refusals so far: coef[0 .. k - 1]
-// are the masses they were refused at (draft given).
+// The remainder of the current row after the refusals so far. With draft
+// probabilities the refusals' masses add up: max(max(p - c0 q, 0) - c1 q, 0) =
+// max(p - (c0 + c1) q, 0) for q >= 0.
 struct Rest {
     const float *p, *q;       // rows of the current node; q NULL without draft probabilities
-    const double *coef;
-    int k;
-    const int *gone;          // refused tokens (no draft)
+    double c;                 // sum of the masses refused at (with q)
+    const int *gone;          // refused tokens (without q)
+    int k;                    // refusals
 };
 
+DSV4CU_DEV double ver_less(float pv, float qv, double c)
+{
+    return fmax(__dsub_rn((double)pv, __dmul_rn(c, (double)qv)), 0.0);
+}
 DSV4CU_DEV double ver_rest(const Rest &r, float pv, float qv, int x)
 {
-    double v = (double)pv;
-    if (r.q) {
-        for (int i = 0; i < r.k; i++) v = fmax(__dsub_rn(v, __dmul_rn(r.coef[i], (double)qv)), 0.0);
-    } else {
-        for (int i = 0; i < r.k; i++)
-            if (r.gone[i] == x) v = 0.0;
-    }
-    return v;
+    if (r.q) return r.k ? ver_less(pv, qv, r.c) : (double)pv;
+    for (int i = 0; i < r.k; i++)
+        if (r.gone[i] == x) return 0.0;
+    return (double)pv;
 }
 
-// Sum of the remainder over elements [lo, hi) by one warp, 128 at a time in
-// lane order; every lane returns the sum. Elements outside add exact zeros.
+// Sum of the remainder over elements [lo, hi) by one warp; every lane returns
+// the sum. LESS: with a draft row to take off.
+template <bool LESS>
 DSV4CU_DEV double ver_segment(const Rest &r, int lo, int hi, int lane)
 {
-    double s = 0.0;
-    for (int x0 = lo; x0 < hi; x0 += 128) {
+    constexpr int B = LESS ? VER_BATCH / 2 : VER_BATCH;
+    double s[2] = {0.0, 0.0};
+    int x0 = lo;
+    bool plain = true;                           // no refused token lies in this segment
+    if (!LESS)
+        for (int i = 0; i < r.k; i++) plain = plain && (r.gone[i] < lo || r.gone[i] >= hi);
+    if (plain) {
+        const float *p = r.p + lo + lane, *q = r.q + lo + lane;
+        for (; x0 + 32 * B <= hi; x0 += 32 * B, p += 32 * B, q += 32 * B) {
+            float pv[B], qv[B];
+#pragma unroll
+            for (int j = 0; j < B; j++) {
+                pv[j] = __ldg(p + 32 * j);
+                if (LESS) qv[j] = __ldg(q + 32 * j);
+            }
+#pragma unroll
+            for (int j = 0; j < B; j++) s[j & 1] += LESS ? ver_less(pv[j], qv[j], r.c) : (double)pv[j];
+        }
+    }
+    for (; x0 < hi; x0 += 128) {                 // the rest (or a segment with a refused token), four at a time
         float pv[4], qv[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int x = x0 + 32 * j + lane;
             pv[j] = x < hi ? __ldg(r.p + x) : 0.0f;
-            qv[j] = x < hi && r.q && r.k ? __ldg(r.q + x) : 0.0f;
+            qv[j] = LESS && x < hi ? __ldg(r.q + x) : 0.0f;
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++) s += ver_rest(r, pv[j], qv[j], x0 + 32 * j + lane);
+        for (int j = 0; j < 4; j++) s[j & 1] += plain ? (LESS ? ver_less(pv[j], qv[j], r.c) : (double)pv[j])
+                                                      : ver_rest(r, pv[j], 0.0f, x0 + 32 * j + lane);
     }
+    double t = s[0] + s[1];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    return s;
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+    return t;
 }
 
-__global__ void __cluster_dims__(VER_CL, 1, 1) __launch_bounds__(VER_THREADS) verify_sample_kernel(const VerifyArgs a)
+__global__ void __cluster_dims__(VER_CL, 1, 1) __launch_bounds__(VER_THREADS, 4) verify_sample_kernel(const VerifyArgs a)
 {
-    __shared__ double part[VER_WARPS], slice_sum, coef[VER_MAX_NODES];
-    __shared__ double sums[VER_CL];
+    __shared__ double part[VER_WARPS];
+    __shared__ double slots[2][VER_CL];
+    __shared__ float s_p[VER_MAX_NODES], s_q[VER_MAX_NODES];
     __shared__ int s_par[VER_MAX_NODES], s_tok[VER_MAX_NODES], line[VER_MAX_NODES], gone[VER_MAX_NODES];
     __shared__ float s_u[VER_MAX_NODES];
     cg::cluster_group cluster = cg::this_cluster();
@@ -173,9 +200,13 @@ __global__ void __cluster_dims__(VER_CL, 1, 1) __launch_bounds__(VER_THREADS) ve
         return;
     }
     for (int i = tid; i < n; i += VER_THREADS) {
-        s_par[i] = __ldg(a.parent + begin + i);
-        s_tok[i] = __ldg(a.tokens + begin + i);
+        const int par = __ldg(a.parent + begin + i), x = __ldg(a.tokens + begin + i);
         s_u[i] = __ldg(a.u + begin + i);
+        s_par[i] = par;
+        s_tok[i] = x;
+        const bool in = i > 0 && par >= 0 && par < i && x >= 0 && x < a.vocab;
+        s_p[i] = in ? __ldg(a.p + (size_t)(begin + par) * a.ldp + x) : 0.0f;
+        s_q[i] = in && a.draft ? __ldg(a.draft + (size_t)(begin + par) * a.ldd + x) : 0.0f;
     }
     if (tid == 0) line[0] = 0;
     __syncthreads();
@@ -185,24 +216,26 @@ __global__ void __cluster_dims__(VER_CL, 1, 1) __launch_bounds__(VER_THREADS) ve
     const int seg = ((per + VER_WARPS - 1) / VER_WARPS + 31) & ~31;
     const int wlo = min(hi, lo + warp * seg), whi = min(hi, wlo + seg);
 
-    Rest r = {a.p + (size_t)begin * a.ldp, a.draft ? a.draft + (size_t)begin * a.ldd : nullptr, coef, 0, gone};
+    Rest r = {a.p + (size_t)begin * a.ldp, a.draft ? a.draft + (size_t)begin * a.ldd : nullptr, 0.0, gone, 0};
     double mass = 1.0;
     // Sum of the remainder over the row, the same bits in every thread of the
     // cluster: warps in order inside a slice, slices in order.
+    int set = 0;
     auto row_sum = [&]() -> double {
-        const double s = ver_segment(r, wlo, whi, lane);
+        const double s = r.q && r.k ? ver_segment<true>(r, wlo, whi, lane) : ver_segment<false>(r, wlo, whi, lane);
+        set ^= 1;
         if (lane == 0) part[warp] = s;
         __syncthreads();
-        if (tid == 0) {
+        if (tid < VER_CL) {
             double t = 0.0;
+#pragma unroll
             for (int w = 0; w < VER_WARPS; w++) t += part[w];
-            slice_sum = t;
+            *cluster.map_shared_rank(&slots[set][rank], tid) = t;
         }
         cluster.sync();
-        if (tid < VER_CL) sums[tid] = *cluster.map_shared_rank(&slice_sum, tid);
-        cluster.sync();                          // every read of slice_sum is done before the next sum writes it
         double t = 0.0;
-        for (int c = 0; c < VER_CL; c++) t += sums[c];
+#pragma unroll
+        for (int c = 0; c < VER_CL; c++) t += slots[set][c];
         return t;
     };
     int cur = 0, acc = 0;
@@ -212,28 +245,28 @@ __global__ void __cluster_dims__(VER_CL, 1, 1) __launch_bounds__(VER_THREADS) ve
         if (s_par[i] != cur) continue;
         const int x = s_tok[i];
         const bool in = x >= 0 && x < a.vocab;
-        const float pv = in ? __ldg(r.p + x) : 0.0f, qv = in && r.q ? __ldg(r.q + x) : 0.0f;
+        const float pv = s_p[i], qv = s_q[i];
         const double left = ver_rest(r, pv, qv, x);
         double bar = __dmul_rn((double)s_u[i], mass);
         if (r.q) bar = __dmul_rn(bar, (double)qv);
         if (in && bar < left) {
             cur = i;
             acc++;
-            __syncthreads();                     // line, coef and gone of the last node are read
             if (tid == 0) line[acc] = i;
             r.p = a.p + (size_t)(begin + i) * a.ldp;
             if (a.draft) r.q = a.draft + (size_t)(begin + i) * a.ldd;
             r.k = 0;
+            r.c = 0.0;
             mass = 1.0;
             have_total = false;
             continue;
         }
-        __syncthreads();
-        if (tid == 0) {
-            coef[r.k] = mass;
-            gone[r.k] = x;
+        r.c += mass;
+        if (!r.q) {
+            __syncthreads();                     // the last node's list is read
+            if (tid == 0) gone[r.k] = x;
+            __syncthreads();
         }
-        __syncthreads();
         r.k++;
         if (r.q) {
             mass = total = row_sum();
@@ -250,6 +283,7 @@ __global__ void __cluster_dims__(VER_CL, 1, 1) __launch_bounds__(VER_THREADS) ve
     }
     // the slice whose running sum passes the threshold, then the warp, then the element
     const double want = __dmul_rn((double)s_u[0], total);
+    const double *sums = slots[set];
     int owner = -1;
     double before = 0.0;
     if (total > 0.0) {
@@ -300,21 +334,31 @@ __global__ void __cluster_dims__(VER_CL, 1, 1) __launch_bounds__(VER_THREADS) ve
     if (warp != wsel) return;
     double base = wbefore;
     int found = -1, lastpos = -1;
-    for (int x0 = wlo; x0 < whi && found < 0; x0 += 32) {
-        const int x = x0 + lane;
-        const float pv = x < whi ? __ldg(r.p + x) : 0.0f, qv = x < whi && r.q && r.k ? __ldg(r.q + x) : 0.0f;
-        const double v = ver_rest(r, pv, qv, x);
-        double c = v;
+    for (int x1 = wlo; x1 < whi && found < 0; x1 += 256) {
+        float pw[8], qw[8];                      // eight steps' loads at once
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double y = __shfl_up_sync(0xFFFFFFFFu, c, o);
-            if (lane >= o) c += y;
+        for (int j = 0; j < 8; j++) {
+            const int x = x1 + 32 * j + lane;
+            pw[j] = x < whi ? __ldg(r.p + x) : 0.0f;
+            qw[j] = x < whi && r.q && r.k ? __ldg(r.q + x) : 0.0f;
         }
-        const unsigned pos = __ballot_sync(0xFFFFFFFFu, v > 0.0);
-        const unsigned hit = __ballot_sync(0xFFFFFFFFu, v > 0.0 && base + c > want);
-        if (hit) found = x0 + __ffs(hit) - 1;
-        if (pos) lastpos = x0 + 31 - __clz(pos);
-        base += __shfl_sync(0xFFFFFFFFu, c, 31);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int x0 = x1 + 32 * j;
+            if (x0 >= whi || found >= 0) break;
+            const double v = ver_rest(r, pw[j], qw[j], x0 + lane);
+            double c = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double y = __shfl_up_sync(0xFFFFFFFFu, c, o);
+                if (lane >= o) c += y;
+            }
+            const unsigned pos = __ballot_sync(0xFFFFFFFFu, v > 0.0);
+            const unsigned hit = __ballot_sync(0xFFFFFFFFu, v > 0.0 && base + c > want);
+            if (hit) found = x0 + __ffs(hit) - 1;
+            if (pos) lastpos = x0 + 31 - __clz(pos);
+            base += __shfl_sync(0xFFFFFFFFu, c, 31);
+        }
     }
     if (found < 0) found = lastpos;              // rounding of the segment's sum: its last token with mass
     if (lane == 0) a.next[b] = found;
