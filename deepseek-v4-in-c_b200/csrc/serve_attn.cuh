@@ -28,11 +28,12 @@
 //
 // Masked entries: a masked score is -inf whatever its key holds. A masked
 // value row is multiplied by a weight of exactly 0, which is only harmless
-// when the value is finite; blocks that a mask crosses (with three weight terms,
-// whose last ones may be 0, all blocks) look for non-finite values, and a tile
-// that meets one is computed again by serve_slow_rows, which touches visible
-// keys only. Rows outside a sequence and pages outside the pool arrive as zeros
-// (cp.async with a source size of 0) and are masked.
+// when the value is finite: 0 x infinity and 0 x NaN are NaN. So a tile whose
+// output is not finite looks (sa_suspect) for a non-finite value behind a mask
+// - with three weight terms, whose last ones may be 0, also for a visible
+// infinity - and if there is one, serve_slow_rows computes the tile again from
+// visible keys only. Rows outside a sequence and pages outside the pool arrive
+// as zeros (cp.async with a source size of 0) and are masked.
 #pragma once
 
 #include <limits.h>
@@ -246,6 +247,34 @@ DSV4CU_DEV float sa_inv(float l, float m, const float *sink, int head)
 {
     if (sink) l += sa_exp2(__ldg(sink + head) * SA_LOG2E - m);
     return l == 0.0f ? 0.0f : 1.0f / l;
+}
+
+// Whether a value of the tile's blocks could have made its output non-finite
+// against the mask: a value that is not finite in a block that a mask crosses
+// (full(block) false), or with ALL an infinite one anywhere. This thread's share
+// of the keys; rows are read from memory, D / 8 pieces each.
+template <int D, bool F16, bool ALL, class Full, class Row>
+DSV4CU_DEV bool sa_suspect(const SaTile &t, int BN, int thread, int threads, Full full, Row row)
+{
+    constexpr uint32_t E = F16 ? 0x7C00u : 0x7F80u, M = F16 ? 0x03FFu : 0x007Fu;
+    bool found = false;
+    for (int blk = t.blk0; blk < t.blk1; blk++) {
+        const bool masked = !full(blk);
+        if (!masked && !ALL) continue;
+        for (int x = thread; x < BN * (D / 8); x += threads) {
+            const int j = x / (D / 8);
+            const uint16_t *v = row(blk, j, true);
+            if (!v) continue;
+            const uint4 w = __ldg(reinterpret_cast<const uint4 *>(v + (x - j * (D / 8)) * 8));
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (masked) found = found || sa_nonfinite<F16>(u[e]);
+                else found = found || (u[e] & (E | M)) == E || ((u[e] >> 16) & (E | M)) == E;
+            }
+        }
+    }
+    return found;
 }
 
 // The tile's rows one by one, a warp per row and a lane per key, visible keys
@@ -501,7 +530,14 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
     for (int mt = 0; mt < 2; mt++)
 #pragma unroll
         for (int n = 0; n < ON; n++) o[mt][n][0] = o[mt][n][1] = o[mt][n][2] = o[mt][n][3] = 0.0f;
-    bool odd = false;                                    // met a non-finite value that a mask or a zero term meets
+    auto is_full = [t, t_lo, t_hi, ap = &a0](int blk) {   // no mask crosses the block (missing pages aside)
+        if constexpr (TREE) {
+            const int e = t.key0 + (blk + 1) * BN;
+            return blk < t.nblk_c && e <= t.kend && t.ctx + t.len - (e - BN) <= ap->window;
+        } else {
+            return (blk + 1) * BN - 1 <= t_lo && t_hi - blk * BN < ap->window;
+        }
+    };
 
     for (int blk = t.blk0; blk < t.blk1; blk++) {
         if (a.nst == 2 && blk + 1 < t.blk1) {
@@ -512,13 +548,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
         }
         __syncthreads();
         uint16_t *kt = kvs + (a.nst == 2 ? blk & 1 : 0) * stage_el, *vt = shared_v ? kt : kt + BN * D;
-        bool full;
-        if constexpr (TREE) {
-            const int e = t.key0 + (blk + 1) * BN;
-            full = blk < t.nblk_c && e <= t.kend && s_bad[blk & 1] != blk && t.ctx + t.len - (e - BN) <= a.window;
-        } else {
-            full = (blk + 1) * BN - 1 <= t_lo && t_hi - blk * BN < a.window;
-        }
+        const bool full = is_full(blk) && s_bad[blk & 1] != blk;
         // ---- partial scores over the warp's dims
 #pragma unroll
         for (int n = 0; n < BN / 8; n += 2) {
@@ -621,9 +651,6 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
 #pragma unroll
                 for (int n = 0; n < OG / 2; n++) {
                     sa_ldsm4_t(b[n], sa_at<D>(vt, 16 * kk + arow, d0 + 8 * n0 + 16 * n + acol));
-                    if (TERMS > 1 || !full)              // a weight's zero terms times infinity are NaN as well
-                        odd = odd || sa_nonfinite<F16>(b[n][0]) || sa_nonfinite<F16>(b[n][1]) ||
-                              sa_nonfinite<F16>(b[n][2]) || sa_nonfinite<F16>(b[n][3]);
                 }
 #pragma unroll
                 for (int mt = 0; mt < 2; mt++)
@@ -647,9 +674,19 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
         __syncthreads();                                 // this stage, the weights and s_alpha are free
         if (a.nst == 1 && blk + 1 < t.blk1) issue(blk + 1);
     }
-    if (__syncthreads_or(odd)) {
-        serve_slow_rows<D, F16, QF32>(a, t, BN, warp, NW, vis, row);
-        return;
+    {
+        bool odd = false;
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+            for (int n = 0; n < ON; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) odd = odd || (16 * mt + g + 8 * (e >> 1) < t.rows && !isfinite(o[mt][n][e]));
+        if (__syncthreads_or(odd) &&
+            __syncthreads_or(sa_suspect<D, F16, (TERMS > 1)>(t, BN, tid, THREADS, is_full, row))) {
+            serve_slow_rows<D, F16, QF32>(a, t, BN, warp, NW, vis, row);
+            return;
+        }
     }
 #pragma unroll
     for (int mt = 0; mt < 2; mt++)
@@ -696,19 +733,36 @@ __global__ void __launch_bounds__(256) serve_join_kernel(const SaArgs a, int BN)
     for (int s = lane; s < sp.used; s += 32) m = fmaxf(m, a.pm[id + s * step]);
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
-    constexpr int E = D / 32;
+    constexpr int E = D / 32, B = D >= 256 ? 4 : 8;      // columns of a lane; splits read at once
     float l = 0.0f, o[E];
 #pragma unroll
     for (int e = 0; e < E; e++) o[e] = 0.0f;
     const float use = m == -INFINITY ? 0.0f : m;
-    for (int s = 0; s < sp.used; s++) {
-        const float ms = a.pm[id + s * step];
-        if (ms == -INFINITY) continue;                   // a split without a visible key
-        const float f = sa_exp2(ms - use);
-        l = fmaf(a.pl[id + s * step], f, l);
-        const float *src = a.po + (id + s * step) * D + lane;
+    for (int s0 = 0; s0 < sp.used; s0 += 32) {
+        // a split's factor and sum by a lane each; one without a visible key has factor 0
+        const int n = min(32, sp.used - s0);
+        float f = 0.0f, ls = 0.0f;
+        if (lane < n) {
+            f = sa_exp2(a.pm[id + (s0 + lane) * step] - use);
+            ls = f > 0.0f ? a.pl[id + (s0 + lane) * step] : 0.0f;
+        }
+        for (int s = 0; s < n; s += B) {
+            float x[B][E], fs[B];
 #pragma unroll
-        for (int e = 0; e < E; e++) o[e] = fmaf(src[32 * e], f, o[e]);
+            for (int u = 0; u < B; u++) {
+                fs[u] = __shfl_sync(0xFFFFFFFFu, f, min(s + u, 31));
+                const float *src = a.po + (id + (s0 + s + u) * step) * D + lane;
+#pragma unroll
+                for (int e = 0; e < E; e++) x[u][e] = s + u < n && fs[u] != 0.0f ? __ldg(src + 32 * e) : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < B; u++) {
+                if (s + u >= n) break;
+                l = fmaf(__shfl_sync(0xFFFFFFFFu, ls, min(s + u, 31)), fs[u], l);
+#pragma unroll
+                for (int e = 0; e < E; e++) o[e] = fmaf(x[u][e], fs[u], o[e]);
+            }
+        }
     }
     const float inv = sa_inv(l, m, a.sink, head);
     const size_t at = (size_t)(sp.begin + r / a.hq) * a.ldo + (size_t)head * D;

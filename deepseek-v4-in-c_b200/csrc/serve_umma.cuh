@@ -396,59 +396,49 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
         float m = -INFINITY, l = 0.0f;
         uint32_t turn = 0;
         bool ok = true;
+        auto is_full = [t, tok_lo, tok_hi, w = a.window](int b) {   // no mask crosses the block (missing pages aside)
+            if constexpr (TREE) {
+                const int base = t.key0 + b * SU_BN;
+                return b < t.nblk_c && base + SU_BN <= t.kend && t.ctx + t.len - base <= w;
+            } else {
+                return b * SU_BN + SU_BN - 1 <= tok_lo && tok_hi - b * SU_BN < w;
+            }
+        };
         auto in_pool = [&](int key) {
             if (key >= t.kend) return false;
             const int id = __ldg(t.table + (key >> a.page_log2));
             return id >= 0 && id < a.n_pages;
         };
         for (int b = first; b < end; b += step, turn++) {
-            // ---- the mask: whether any, whether it differs between rows
+            // ---- the mask
             const bool cached = TREE && b < t.nblk_c;
             const int base = (TREE ? (cached ? t.key0 + b * SU_BN : (b - t.nblk_c) * SU_BN) : b * SU_BN);
-            bool ragged, masked;
-            if (cached) {
-                ragged = t.ctx + t.len - base > a.window;
-                masked = ragged || lost || base + SU_BN > t.kend;
-            } else if (TREE) {
-                ragged = masked = true;
-            } else {
-                ragged = masked = base + SU_BN - 1 > tok_lo || tok_hi - base >= a.window;
-            }
+            const bool masked = !is_full(b) || (cached && lost);
+            // keys that are not there: behind the sequence, the nodes or the
+            // cache, or on a missing page
+            const bool gaps = cached ? lost || base + SU_BN > t.kend : base + SU_BN > t.len;
             uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
-            // behind this block's scores lie the products of every block before
-            // it, so the value stage's last use is over and its barrier is at
-            // most one phase away: the parity below means this block
             ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sfull[s], turn & 1, a.status, SUE_S));
             if (!ok) break;
-            if (masked) {
-                // key i of the block is there at all: in its page, before the CTA's last token
-                bool there;
-                if (cached) {
-                    there = in_pool(base + i);
-                } else {
-                    there = base + i <= (TREE ? t.len - 1 : tok_end);
-                }
+            if (gaps) {
+                // values of absent keys become zeros (what the copies left, or
+                // brought from the next sequence, may be no number). Behind
+                // this block's scores lie the products of every block before
+                // it, so the stage's last use is over and its barrier is at
+                // most one phase away: the parity below means this block.
                 const int n = b - c0, st = n % a.nst;
                 ok = __all_sync(0xFFFFFFFFu, mbar_wait(&vfull[st], (n / a.nst) & 1, a.status, SUE_VFULL));
                 if (!ok) break;
-                // values of absent keys become zeros; the others must be finite
-                // where the mask keeps them from some rows only
-                uint8_t *v = vs + st * KVB + i * 128;
-                bool odd = false;
+                if (!(cached ? in_pool(base + i) : base + i < t.len)) {
+                    uint8_t *v = vs + st * KVB + i * 128;
 #pragma unroll
-                for (int c = 0; c < DC; c++)
+                    for (int c = 0; c < DC; c++)
 #pragma unroll
-                    for (int x = 0; x < 8; x++) {
-                        uint4 *p = reinterpret_cast<uint4 *>(v + c * SU_SUB + 16 * x);
-                        if (!there) *p = make_uint4(0, 0, 0, 0);
-                        else if (ragged) {
-                            const uint4 w = *p;
-                            odd = odd || sa_nonfinite<F16>(w.x) || sa_nonfinite<F16>(w.y) || sa_nonfinite<F16>(w.z) ||
-                                  sa_nonfinite<F16>(w.w);
-                        }
-                    }
-                if (odd) s_odd[s] = 1;
+                        for (int x = 0; x < 8; x++) *reinterpret_cast<uint4 *>(v + c * SU_SUB + 16 * x) = make_uint4(0, 0, 0, 0);
+                }
                 su_fence_async();
+            }
+            if (masked) {
                 if (cached) {
                     const int pos = t.ctx + depth, lo = a.window > pos ? 0 : pos - a.window + 1 - base;
 #pragma unroll
@@ -570,9 +560,8 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                 xl[i] = l;
             }
             su_bar<256>(1);
-            if (s_odd[0] | s_odd[1]) {
-                serve_slow_rows<D, F16, false>(a, t, SU_BN, warp - 4, 8, sees, row_of);
-            } else if (s == 0 && live) {
+            bool odd = false;
+            if (s == 0 && live) {
                 float f_a = 1.0f, f_b = 0.0f;
                 if (two) {
                     const float mb = xm[i], top = fmaxf(m, mb), use = top == -INFINITY ? 0.0f : top;
@@ -599,6 +588,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                     for (int k = 0; k < 32; k++) {
                         y[k] = __uint_as_float(o[k]) * f_a;
                         if (two) y[k] = fmaf(xo[i * OS + c + k], f_b, y[k]);
+                        odd = odd || (i < rows && !isfinite(y[k]));
                         y[k] *= inv;
                     }
                     if (i < rows) {
@@ -617,16 +607,17 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                     }
                 }
             }
+            // a row that is not finite: was it a value behind the mask?
+            if (odd) s_odd[0] = 1;
+            su_bar<256>(1);
+            if (s_odd[0]) {
+                if (sa_suspect<D, F16, false>(t, SU_BN, threadIdx.x - 128, 256, is_full, row_of)) s_odd[1] = 1;
+                su_bar<256>(1);
+                if (s_odd[1]) serve_slow_rows<D, F16, false>(a, t, SU_BN, warp - 4, 8, sees, row_of);
+            }
         } else {
-            su_bar<128>(2 + s);                          // every warp's finding in s_odd
-            if (s_odd[s]) {
-                SaTile ts = t;
-                ts.r0 = t.r0 + row0;
-                ts.rows = rows;
-                ts.blk0 = first;
-                ts.blk1 = end;
-                serve_slow_rows<D, F16, false>(a, ts, SU_BN, warp & 3, 4, sees, row_of);
-            } else if (live) {
+            bool odd = false;
+            if (live) {
                 const bool part = t.parts > 1;
                 const float inv = part ? 1.0f : sa_inv(l, m, a.sink, head);
                 const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + tok) * a.hq + head;
@@ -645,7 +636,10 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                         for (int k = 0; k < 32; k += 8) {
                             float y[8];
 #pragma unroll
-                            for (int e = 0; e < 8; e++) y[e] = __uint_as_float(o[k + e]) * inv;
+                            for (int e = 0; e < 8; e++) {
+                                odd = odd || !isfinite(__uint_as_float(o[k + e]));
+                                y[e] = __uint_as_float(o[k + e]) * inv;
+                            }
                             if (part) {
                                 float4 *d = reinterpret_cast<float4 *>(a.po + id * D + c + k);
                                 d[0] = make_float4(y[0], y[1], y[2], y[3]);
@@ -658,6 +652,18 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                         }
                     }
                 }
+            }
+            if (odd) s_odd[s] = 1;
+            su_bar<128>(2 + s);
+            if (s_odd[s]) {
+                SaTile ts = t;
+                ts.r0 = t.r0 + row0;
+                ts.rows = rows;
+                ts.blk0 = first;
+                ts.blk1 = end;
+                if (sa_suspect<D, F16, false>(ts, SU_BN, i, 128, is_full, row_of)) s_odd[s] = 2;
+                su_bar<128>(2 + s);
+                if (s_odd[s] == 2) serve_slow_rows<D, F16, false>(a, ts, SU_BN, warp & 3, 4, sees, row_of);
             }
         }
     }
