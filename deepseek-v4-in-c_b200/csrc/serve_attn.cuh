@@ -551,27 +551,27 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
         const bool full = is_full(blk) && s_bad[blk & 1] != blk;
         // ---- partial scores over the warp's dims
 #pragma unroll
-        for (int n = 0; n < BN / 8; n += 2) {
-            float s[2][2][4] = {};
+        for (int n = 0; n < BN / 8; n += 4) {            // eight accumulators at a time cover the product's latency
+            float s[2][4][4] = {};
 #pragma unroll
             for (int kk = 0; kk < KS; kk++) {
-                uint32_t b[4];
-                sa_ldsm4(b, sa_at<D>(kt, 8 * n + brow, d0 + 16 * kk + bcol));
+                uint32_t b[2][4];
+#pragma unroll
+                for (int u = 0; u < 2; u++) sa_ldsm4(b[u], sa_at<D>(kt, 8 * n + 16 * u + brow, d0 + 16 * kk + bcol));
 #pragma unroll
                 for (int x = TERMS - 1; x >= 0; x--)
 #pragma unroll
-                    for (int mt = 0; mt < 2; mt++)
-                        if (mt == 0 || second) {
-                            sa_mma<F16>(s[mt][0], qa[mt][kk][x], b[0], b[1]);
-                            sa_mma<F16>(s[mt][1], qa[mt][kk][x], b[2], b[3]);
-                        }
+                    for (int u = 0; u < 4; u++) {
+                        sa_mma<F16>(s[0][u], qa[0][kk][x], b[u / 2][2 * (u & 1)], b[u / 2][2 * (u & 1) + 1]);
+                        if (second) sa_mma<F16>(s[1][u], qa[1][kk][x], b[u / 2][2 * (u & 1)], b[u / 2][2 * (u & 1) + 1]);
+                    }
             }
             float *dst = part + (warp * BM + g) * SS + 8 * n + 2 * c;
 #pragma unroll
             for (int mt = 0; mt < 2; mt++)
                 if (mt == 0 || second)
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
+                    for (int u = 0; u < 4; u++) {
                         *reinterpret_cast<float2 *>(dst + 16 * mt * SS + 8 * u) = make_float2(s[mt][u][0], s[mt][u][1]);
                         *reinterpret_cast<float2 *>(dst + (16 * mt + 8) * SS + 8 * u) = make_float2(s[mt][u][2], s[mt][u][3]);
                     }
@@ -653,15 +653,17 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
                     sa_ldsm4_t(b[n], sa_at<D>(vt, 16 * kk + arow, d0 + 8 * n0 + 16 * n + acol));
                 }
 #pragma unroll
-                for (int mt = 0; mt < 2; mt++)
-                    if (mt == 0 || second)
+                for (int x = TERMS - 1; x >= 0; x--) {
+                    uint32_t pa[2][4];
 #pragma unroll
-                        for (int x = TERMS - 1; x >= 0; x--) {
-                            uint32_t pa[4];
-                            sa_ldsm4(pa, ps + (x * BM + 16 * mt + arow) * PS + 16 * kk + acol);
+                    for (int mt = 0; mt < 2; mt++)
+                        if (mt == 0 || second) sa_ldsm4(pa[mt], ps + (x * BM + 16 * mt + arow) * PS + 16 * kk + acol);
 #pragma unroll
-                            for (int n = 0; n < OG; n++) sa_mma<F16>(acc[mt][n], pa, b[n / 2][2 * (n & 1)], b[n / 2][2 * (n & 1) + 1]);
-                        }
+                    for (int n = 0; n < OG; n++) {
+                        sa_mma<F16>(acc[0][n], pa[0], b[n / 2][2 * (n & 1)], b[n / 2][2 * (n & 1) + 1]);
+                        if (second) sa_mma<F16>(acc[1][n], pa[1], b[n / 2][2 * (n & 1)], b[n / 2][2 * (n & 1) + 1]);
+                    }
+                }
             }
 #pragma unroll
             for (int mt = 0; mt < 2; mt++)

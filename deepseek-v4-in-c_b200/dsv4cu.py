@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -381,6 +382,15 @@ class TreeAttnArgs(C.Structure):
                [("scale", C.c_float), ("sink", C.c_void_p)]
 
 
+# The same layouts for struct.pack_into: filling a ctypes.Structure of this many
+# fields costs a serving step a few microseconds per call.
+_PLAN = struct.Struct("@5i12Q")
+_PROMPT = struct.Struct("@4Q4q2iQ6ifQ")
+_TREE = struct.Struct("@6Q4q2i4Q11ifQ")
+assert (_PLAN.size, _PROMPT.size, _TREE.size) == tuple(
+    C.sizeof(x) for x in (PagePlanArgs, PromptAttnArgs, TreeAttnArgs))
+
+
 class Device:
     """The native dsv4cu_* entry points on one CUDA device."""
 
@@ -394,6 +404,8 @@ class Device:
         check(self.L.dsv4cu_ctx_create(C.byref(h), device), "ctx_create")
         self.ctx = h
         self._elem = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+        self._args = C.create_string_buffer(256)     # argument structure of the call being made
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
     def close(self):
         if self.ctx:
@@ -401,6 +413,8 @@ class Device:
             self.ctx = None
 
     def stream(self):
+        if self._raw_stream is not None:             # the same handle without building a Stream object
+            return self._raw_stream(self.device)
         return self.torch.cuda.current_stream(self.device).cuda_stream
 
     INJECT_WITHHOLD_STAGE = 1
@@ -730,13 +744,17 @@ class Device:
 
     # ---- paged serving
     def _ints(self, what, n, *tensors):
-        """Every tensor is contiguous int32 on this device with n elements (None passes)."""
-        i32, device = self.torch.int32, self.device
+        """Addresses of contiguous int32 tensors of n elements on this device (None: 0)."""
+        i32, device, out = self.torch.int32, self.device, []
         for t in tensors:
-            if t is not None and (t.dtype is not i32 or t.get_device() != device or t.numel() != n or
-                                  not t.is_contiguous()):
+            if t is None:
+                out.append(0)
+                continue
+            if t.dtype is not i32 or t.get_device() != device or t.numel() != n or not t.is_contiguous():
                 raise DSV4CUError(f"{what}: needs contiguous int32 tensors of {n} elements on cuda:{device}, got "
                                   f"{t.dtype} {tuple(t.shape)} on {t.device}")
+            out.append(t.data_ptr())
+        return out
 
     def _rows(self, what, t, heads, dim, dtype=None):
         """Packed token rows [nt][heads][dim], any stride between tokens: that stride in elements."""
@@ -750,9 +768,12 @@ class Device:
         return step if t.shape[0] > 1 else heads * dim
 
     def _sink(self, what, sink, heads):
-        if sink is not None and (sink.dtype is not self.torch.float32 or sink.numel() != heads or
-                                 sink.get_device() != self.device or not sink.is_contiguous()):
+        if sink is None:
+            return 0
+        if sink.dtype is not self.torch.float32 or sink.numel() != heads or sink.get_device() != self.device or \
+                not sink.is_contiguous():
             raise DSV4CUError(f"{what}: sink needs {heads} contiguous float32 on cuda:{self.device}")
+        return sink.data_ptr()
 
     def _caches(self, what, k_cache, v_cache):
         if k_cache.dim() != 4 or not k_cache.is_contiguous() or k_cache.get_device() != self.device or \
@@ -769,22 +790,22 @@ class Device:
         int64. held_out / ring_pos_out None: held and ring_pos are updated in place."""
         held_out = held if held_out is None else held_out
         ring_pos_out = ring_pos if ring_pos_out is None else ring_pos_out
-        n, cap = seq_len.numel(), slot.numel()
-        self._ints("page_plan", n, seq_len, new_len, held, held_out)
-        self._ints("page_plan", cap, slot, pos, req)
-        self._ints("page_plan", n + 1, cu)
-        self._ints("page_plan", ring.numel(), ring)
+        n, cap, pages = seq_len.numel(), slot.numel(), ring.numel()
         if table.dim() != 2 or table.shape[0] != n:
             raise DSV4CUError(f"page_plan: table needs {n} rows, got {tuple(table.shape)}")
-        self._ints("page_plan", table.numel(), table)
+        seq, new, h, h_out = self._ints("page_plan", n, seq_len, new_len, held, held_out)
+        out = self._ints("page_plan", cap, slot, pos, req)
+        i64, device = self.torch.int64, self.device
         for t in (ring_pos, ring_pos_out):
-            if t.dtype is not self.torch.int64 or t.numel() != 2 or t.get_device() != self.device or \
-                    not t.is_contiguous():
+            if t.dtype is not i64 or t.numel() != 2 or t.get_device() != device or not t.is_contiguous():
                 raise DSV4CUError("page_plan: ring_pos needs two contiguous int64 on this device")
-        p = self.ptr
-        a = PagePlanArgs(n, page_size, ring.numel(), table.shape[1], cap, p(seq_len), p(new_len), p(held), p(held_out),
-                         p(table), p(ring), p(ring_pos), p(ring_pos_out), p(cu), p(slot), p(pos), p(req))
-        check(self.L.dsv4cu_page_plan(self.ctx, C.byref(a), self.stream()), "dsv4cu_page_plan")
+        width = table.shape[1]
+        _PLAN.pack_into(self._args, 0, n, page_size, pages, width, cap, seq, new, h, h_out,
+                        *self._ints("page_plan", n * width, table), *self._ints("page_plan", pages, ring),
+                        ring_pos.data_ptr(), ring_pos_out.data_ptr(), *self._ints("page_plan", n + 1, cu), *out)
+        rc = self.L.dsv4cu_page_plan(self.ctx, self._args, self.stream())
+        if rc:
+            check(rc, "dsv4cu_page_plan")
 
     def paged_write(self, k_cache, v_cache, k, v, slot):
         """k_cache / v_cache [pages][page_size][kv heads][head_dim] at slot[t] = row t of k / v
@@ -798,10 +819,11 @@ class Device:
             ldv = self._rows("paged_write", v, kv, dim, k.dtype)
             if v.shape[0] != nt:
                 raise DSV4CUError(f"paged_write: {nt} key rows and {v.shape[0]} value rows")
-        self._ints("paged_write", nt, slot)
-        check(self.L.dsv4cu_paged_write(self.ctx, self.ptr(k_cache), self.ptr(v_cache), self._elem[k_cache.dtype],
-                                        self.ptr(k), self.ptr(v), self._elem[k.dtype], ldk, ldv, self.ptr(slot), nt,
-                                        pages * page, kv, dim, self.stream()), "dsv4cu_paged_write")
+        rc = self.L.dsv4cu_paged_write(self.ctx, k_cache.data_ptr(), self.ptr(v_cache), self._elem[k_cache.dtype],
+                                       k.data_ptr(), self.ptr(v), self._elem[k.dtype], ldk, ldv,
+                                       self._ints("paged_write", nt, slot)[0], nt, pages * page, kv, dim, self.stream())
+        if rc:
+            check(rc, "dsv4cu_paged_write")
 
     def prompt_attn(self, o, q, k, v, cu, scale: float, window: int = 0, sink=None):
         """Causal attention of packed prompts (dsv4cu_prompt_attn): o / q [nt][heads][dim], k / v [nt][kv heads][dim]
@@ -814,12 +836,13 @@ class Device:
         ldv = 0 if v is None else self._rows(what, v, kv, dim, k.dtype)
         if o.shape[0] != nt or k.shape[0] != nt or (v is not None and v.shape[0] != nt):
             raise DSV4CUError(f"{what}: q, k, v and o must have the same number of tokens")
-        self._ints(what, cu.numel(), cu)
-        self._sink(what, sink, heads)
-        p = self.ptr
-        a = PromptAttnArgs(p(o), p(q), p(k), p(v), ldo, ldq, ldk, ldv, self._elem[q.dtype], self._elem[k.dtype], p(cu),
-                           cu.numel() - 1, nt, heads, kv, dim, window, scale, p(sink))
-        check(self.L.dsv4cu_prompt_attn(self.ctx, C.byref(a), self.stream()), "dsv4cu_prompt_attn")
+        n = cu.numel()
+        _PROMPT.pack_into(self._args, 0, o.data_ptr(), q.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr(), ldo,
+                          ldq, ldk, ldv, self._elem[q.dtype], self._elem[k.dtype], self._ints(what, n, cu)[0], n - 1, nt,
+                          heads, kv, dim, window, scale, self._sink(what, sink, heads))
+        rc = self.L.dsv4cu_prompt_attn(self.ctx, self._args, self.stream())
+        if rc:
+            check(rc, "dsv4cu_prompt_attn")
 
     def _tree_args(self, o, q, k, v, k_cache, v_cache, table, ctx_len, cu, parent, scale, max_nodes, max_ctx, window,
                    sink):
@@ -834,17 +857,16 @@ class Device:
                 (v is not None and v.shape[0] != nt):
             raise DSV4CUError(f"{what}: q, k, v, o and the caches do not fit together")
         n = ctx_len.numel()
-        self._ints(what, n, ctx_len)
-        self._ints(what, n + 1, cu)
-        self._ints(what, nt, parent)
         if table.dim() != 2 or table.shape[0] != n:
             raise DSV4CUError(f"{what}: table needs {n} rows, got {tuple(table.shape)}")
-        self._ints(what, table.numel(), table)
-        self._sink(what, sink, heads)
-        p = self.ptr
-        return TreeAttnArgs(p(o), p(q), p(k), p(v), p(k_cache), p(v_cache), ldo, ldq, ldk, ldv, self._elem[q.dtype],
-                            self._elem[k.dtype], p(table), p(ctx_len), p(cu), p(parent), n, nt, heads, kv, dim, page,
-                            pages, table.shape[1], max_nodes, max_ctx, window, scale, p(sink))
+        width = table.shape[1]
+        _TREE.pack_into(self._args, 0, o.data_ptr(), q.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr(),
+                        k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), ldo, ldq, ldk, ldv,
+                        self._elem[q.dtype], self._elem[k.dtype], *self._ints(what, n * width, table),
+                        *self._ints(what, n, ctx_len), *self._ints(what, n + 1, cu), *self._ints(what, nt, parent), n,
+                        nt, heads, kv, dim, page, pages, width, max_nodes, max_ctx, window, scale,
+                        self._sink(what, sink, heads))
+        return self._args
 
     def tree_attn(self, o, q, k, v, k_cache, v_cache, table, ctx_len, cu, parent, scale: float, max_nodes: int,
                   max_ctx: int, window: int = 0, sink=None):
@@ -853,47 +875,48 @@ class Device:
         [n_req][max_pages], ctx_len [n_req], cu [n_req + 1], parent [nt]: int32."""
         a = self._tree_args(o, q, k, v, k_cache, v_cache, table, ctx_len, cu, parent, scale, max_nodes, max_ctx,
                             window, sink)
-        check(self.L.dsv4cu_tree_attn(self.ctx, C.byref(a), self.stream()), "dsv4cu_tree_attn")
+        rc = self.L.dsv4cu_tree_attn(self.ctx, a, self.stream())
+        if rc:
+            check(rc, "dsv4cu_tree_attn")
 
     def tree_attn_workspace(self, *args, window: int = 0, sink=None) -> int:
         """Workspace bytes of the tree_attn call with these arguments (dsv4cu_tree_attn_workspace)."""
-        return self.L.dsv4cu_tree_attn_workspace(self.ctx, C.byref(self._tree_args(*args, window, sink)))
+        return self.L.dsv4cu_tree_attn_workspace(self.ctx, self._tree_args(*args, window, sink))
 
     def _verify(self, what, accepted, next_token, path, tokens, parent, cu, slot, slot_out):
         n, nt = cu.numel() - 1, tokens.numel()
-        self._ints(what, n, accepted, next_token)
-        self._ints(what, n + 1, cu)
-        self._ints(what, nt, tokens, path, parent, slot, slot_out)
-        return n, nt
+        rows = self._ints(what, nt, path, tokens, parent, slot, slot_out)
+        return n, nt, (*self._ints(what, n, accepted, next_token), *rows[:3], *self._ints(what, n + 1, cu)), rows[3:]
 
     def verify_greedy(self, accepted, next_token, path, tokens, parent, cu, best, slot=None, slot_out=None):
         """Drafted trees against the target's greedy picks best [nt] (dsv4cu_verify_greedy)."""
-        n, nt = self._verify("verify_greedy", accepted, next_token, path, tokens, parent, cu, slot, slot_out)
-        self._ints("verify_greedy", nt, best)
-        p = self.ptr
-        check(self.L.dsv4cu_verify_greedy(self.ctx, p(accepted), p(next_token), p(path), p(tokens), p(parent), p(cu),
-                                          p(best), p(slot), p(slot_out), n, nt, self.stream()), "dsv4cu_verify_greedy")
+        n, nt, lists, slots = self._verify("verify_greedy", accepted, next_token, path, tokens, parent, cu, slot, slot_out)
+        rc = self.L.dsv4cu_verify_greedy(self.ctx, *lists, *self._ints("verify_greedy", nt, best), *slots, n, nt,
+                                         self.stream())
+        if rc:
+            check(rc, "dsv4cu_verify_greedy")
 
     def verify_sample(self, accepted, next_token, path, tokens, parent, cu, probs, u, draft=None, slot=None,
                       slot_out=None):
         """Drafted trees against the target's probabilities probs [nt][vocab] from uniform numbers u [nt], draft
         [nt][vocab] or None for certain drafts (dsv4cu_verify_sample)."""
-        n, nt = self._verify("verify_sample", accepted, next_token, path, tokens, parent, cu, slot, slot_out)
+        n, nt, lists, slots = self._verify("verify_sample", accepted, next_token, path, tokens, parent, cu, slot, slot_out)
         f32, device = self.torch.float32, self.device
-        if probs.dim() != 2 or u.numel() != nt or not u.is_contiguous():
-            raise DSV4CUError("verify_sample: probs [nt][vocab] and contiguous u [nt] are needed")
+        if probs.dim() != 2 or probs.shape[0] != nt or (draft is not None and draft.shape != probs.shape):
+            raise DSV4CUError("verify_sample: probabilities [nt][vocab] are needed")
         for t in (probs, draft):
-            if t is not None and (t.shape != probs.shape or t.shape[0] != nt or t.dtype is not f32 or
-                                  t.get_device() != device or (t.shape[1] > 1 and t.stride(1) != 1)):
+            if t is not None and (t.dtype is not f32 or t.get_device() != device or
+                                  (t.shape[1] > 1 and t.stride(1) != 1)):
                 raise DSV4CUError("verify_sample: probabilities are float32 [nt][vocab] on this device")
-        if u.dtype is not f32 or u.get_device() != device:
-            raise DSV4CUError("verify_sample: u is float32 on this device")
+        if u.dtype is not f32 or u.get_device() != device or u.numel() != nt or not u.is_contiguous():
+            raise DSV4CUError("verify_sample: u is contiguous float32 [nt] on this device")
         vocab = probs.shape[1]
-        step = lambda t: vocab if t is None or nt < 2 else t.stride(0)  # noqa: E731
-        p = self.ptr
-        check(self.L.dsv4cu_verify_sample(self.ctx, p(accepted), p(next_token), p(path), p(tokens), p(parent), p(cu),
-                                          p(probs), step(probs), p(draft), step(draft), p(u), vocab, p(slot),
-                                          p(slot_out), n, nt, self.stream()), "dsv4cu_verify_sample")
+        ldp = vocab if nt < 2 else probs.stride(0)
+        ldd = 0 if draft is None else vocab if nt < 2 else draft.stride(0)
+        rc = self.L.dsv4cu_verify_sample(self.ctx, *lists, probs.data_ptr(), ldp, self.ptr(draft), ldd, u.data_ptr(),
+                                         vocab, *slots, n, nt, self.stream())
+        if rc:
+            check(rc, "dsv4cu_verify_sample")
 
     def quantize_fp8(self, w, s, src, rows, cols):
         check(self.L.dsv4cu_quantize_fp8(self.ptr(w), self.ptr(s), self.ptr(src), rows, cols,
