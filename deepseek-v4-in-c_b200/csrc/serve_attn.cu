@@ -146,6 +146,7 @@ static TreeShape tree_shape(const dsv4cu_ctx *ctx, const dsv4cu_tree_attn_args *
     if (chunk < (blocks + 63) / 64) chunk = (blocks + 63) / 64;
     s.chunk = (int)chunk;
     s.splits = (int)((blocks + chunk - 1) / chunk);
+    if (ctas > DSV4CU_MAX_COUNTERS) s.splits = 1;         // a counter per tile joins its splits
     return s;
 }
 
@@ -204,6 +205,7 @@ extern "C" int dsv4cu_tree_attn(dsv4cu_ctx *ctx, const dsv4cu_tree_attn_args *a,
     s.max_pages = a->max_pages;
     s.max_nodes = a->max_nodes;
     s.status = ctx->status;
+    s.counters = ctx->counters;
     const TreeShape shape = tree_shape(ctx, a, c);
     s.two = shape.two;
     s.row_tiles = shape.row_tiles;

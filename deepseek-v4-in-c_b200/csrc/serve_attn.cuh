@@ -62,6 +62,7 @@ struct SaArgs {
     int max_nodes, row_tiles, splits;
     int chunk;                        // key blocks of a split, at least
     float *pm, *pl, *po;              // partials [splits][nt * hq](, D), splits > 1
+    int *counters;                    // [n_req][hkv][row_tiles], zero between calls: splits done
     int *status;
     int nst;                          // key stages in shared memory
     int two, box_log2;                // tcgen05 kernel: two row tiles per CTA; rows of a cached copy's box
@@ -340,6 +341,59 @@ __device__ __noinline__ void serve_slow_rows(const SaArgs &a, const SaTile &t, i
 #pragma unroll
             for (int e = 0; e < E; e++) sa_store_o<F16, QF32>(a, at + lane + 32 * e, o[e] * inv);
         }
+    }
+}
+
+// Joins the splits of a tile's rows, a warp per row: the partial outputs
+// rescaled to the row's largest maximum and divided by the joint exp-sum (with
+// the sink), in split order whichever split came last.
+template <int D, bool F16, bool QF32>
+DSV4CU_DEV void sa_join(const SaArgs &a, const SaTile &t, int warp, int warps)
+{
+    const int lane = threadIdx.x & 31;
+    constexpr int E = D / 32, B = D >= 256 ? 4 : 8;      // columns of a lane; splits read at once
+    const size_t step = (size_t)a.nt * a.hq;
+    for (int r = warp; r < t.rows; r += warps) {
+        const int pr = t.r0 + r, tok = pr / a.G, head = t.kvh * a.G + pr - tok * a.G;
+        const size_t id = (size_t)(t.begin + tok) * a.hq + head;
+        float m = -INFINITY;
+        for (int s = lane; s < t.parts; s += 32) m = fmaxf(m, __ldcg(a.pm + id + s * step));
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
+        float l = 0.0f, o[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = 0.0f;
+        const float use = m == -INFINITY ? 0.0f : m;
+        for (int s0 = 0; s0 < t.parts; s0 += 32) {
+            // a split's factor and sum by a lane each; one without a visible key has factor 0
+            const int n = min(32, t.parts - s0);
+            float f = 0.0f, ls = 0.0f;
+            if (lane < n) {
+                f = sa_exp2(__ldcg(a.pm + id + (s0 + lane) * step) - use);
+                ls = f != 0.0f ? __ldcg(a.pl + id + (s0 + lane) * step) : 0.0f;
+            }
+            for (int s = 0; s < n; s += B) {
+                float x[B][E], fs[B];
+#pragma unroll
+                for (int u = 0; u < B; u++) {
+                    fs[u] = __shfl_sync(0xFFFFFFFFu, f, min(s + u, 31));
+                    const float *src = a.po + (id + (s0 + s + u) * step) * D + lane;
+#pragma unroll
+                    for (int e = 0; e < E; e++) x[u][e] = s + u < n && fs[u] != 0.0f ? __ldcg(src + 32 * e) : 0.0f;
+                }
+#pragma unroll
+                for (int u = 0; u < B; u++) {
+                    if (s + u >= n) break;
+                    l = fmaf(__shfl_sync(0xFFFFFFFFu, ls, min(s + u, 31)), fs[u], l);
+#pragma unroll
+                    for (int e = 0; e < E; e++) o[e] = fmaf(x[u][e], fs[u], o[e]);
+                }
+            }
+        }
+        const float inv = sa_inv(l, m, a.sink, head);
+        const size_t at = (size_t)(t.begin + tok) * a.ldo + (size_t)head * D;
+#pragma unroll
+        for (int e = 0; e < E; e++) sa_store_o<F16, QF32>(a, at + lane + 32 * e, o[e] * inv);
     }
 }
 
@@ -676,6 +730,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
         __syncthreads();                                 // this stage, the weights and s_alpha are free
         if (a.nst == 1 && blk + 1 < t.blk1) issue(blk + 1);
     }
+    bool done = false;
     {
         bool odd = false;
 #pragma unroll
@@ -687,7 +742,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
         if (__syncthreads_or(odd) &&
             __syncthreads_or(sa_suspect<D, F16, (TERMS > 1)>(t, BN, tid, THREADS, is_full, row))) {
             serve_slow_rows<D, F16, QF32>(a, t, BN, warp, NW, vis, row);
-            return;
+            done = true;
         }
     }
 #pragma unroll
@@ -695,7 +750,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const int r = 16 * mt + g + 8 * h;
-            if (r >= t.rows) continue;
+            if (done || r >= t.rows) continue;
             const int pr = t.r0 + r, tok = pr / a.G, head = t.kvh * a.G + pr % a.G, col = d0 + 2 * c;
             if (t.parts > 1) {
                 const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + tok) * a.hq + head;
@@ -717,68 +772,22 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
                 }
             }
         }
-}
-
-// Joins the splits of a tree's rows, a warp per row: the partial outputs
-// rescaled to the row's largest maximum and divided by the joint exp-sum (with
-// the sink), in split order.
-template <int D, bool F16, bool QF32>
-__global__ void __launch_bounds__(256) serve_join_kernel(const SaArgs a, int BN)
-{
-    pdl_wait();
-    const SaSpan sp = sa_span(a, blockIdx.y, BN);
-    const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (sp.len > a.max_nodes || r >= sp.len * a.hq || sp.used <= 1) return;   // one split writes its rows itself
-    const int head = r % a.hq;
-    const size_t id = (size_t)(sp.begin + r / a.hq) * a.hq + head, step = (size_t)a.nt * a.hq;
-    float m = -INFINITY;
-    for (int s = lane; s < sp.used; s += 32) m = fmaxf(m, a.pm[id + s * step]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
-    constexpr int E = D / 32, B = D >= 256 ? 4 : 8;      // columns of a lane; splits read at once
-    float l = 0.0f, o[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) o[e] = 0.0f;
-    const float use = m == -INFINITY ? 0.0f : m;
-    for (int s0 = 0; s0 < sp.used; s0 += 32) {
-        // a split's factor and sum by a lane each; one without a visible key has factor 0
-        const int n = min(32, sp.used - s0);
-        float f = 0.0f, ls = 0.0f;
-        if (lane < n) {
-            f = sa_exp2(a.pm[id + (s0 + lane) * step] - use);
-            ls = f > 0.0f ? a.pl[id + (s0 + lane) * step] : 0.0f;
+    if (TREE && t.parts > 1) {
+        // the tile's last split to finish joins them all
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+            int *count = a.counters + ((size_t)blockIdx.z * a.hkv + t.kvh) * a.row_tiles + blockIdx.x % a.row_tiles;
+            const bool last = atomicAdd(count, 1) == t.parts - 1;
+            if (last) *count = 0;
+            s_bad[0] = last;
         }
-        for (int s = 0; s < n; s += B) {
-            float x[B][E], fs[B];
-#pragma unroll
-            for (int u = 0; u < B; u++) {
-                fs[u] = __shfl_sync(0xFFFFFFFFu, f, min(s + u, 31));
-                const float *src = a.po + (id + (s0 + s + u) * step) * D + lane;
-#pragma unroll
-                for (int e = 0; e < E; e++) x[u][e] = s + u < n && fs[u] != 0.0f ? __ldg(src + 32 * e) : 0.0f;
-            }
-#pragma unroll
-            for (int u = 0; u < B; u++) {
-                if (s + u >= n) break;
-                l = fmaf(__shfl_sync(0xFFFFFFFFu, ls, min(s + u, 31)), fs[u], l);
-#pragma unroll
-                for (int e = 0; e < E; e++) o[e] = fmaf(x[u][e], fs[u], o[e]);
-            }
+        __syncthreads();
+        if (s_bad[0]) {
+            __threadfence();
+            sa_join<D, F16, QF32>(a, t, warp, NW);
         }
     }
-    const float inv = sa_inv(l, m, a.sink, head);
-    const size_t at = (size_t)(sp.begin + r / a.hq) * a.ldo + (size_t)head * D;
-#pragma unroll
-    for (int e = 0; e < E; e++) sa_store_o<F16, QF32>(a, at + lane + 32 * e, o[e] * inv);
-}
-
-// Launches the join behind a split tree pass of key blocks of BN.
-template <int D, bool F16, bool QF32>
-int serve_join_launch(const SaArgs &a, int BN, cudaStream_t st)
-{
-    const dim3 grid((unsigned)(((int64_t)a.max_nodes * a.hq + 7) / 8), a.n_req, 1);
-    DSV4CU_CUDA_TRY(launch_pdl(serve_join_kernel<D, F16, QF32>, grid, dim3(256), 0, st, a, BN));
-    return DSV4CU_OK;
 }
 
 constexpr int SA_SMEM_MAX = 220 * 1024;      // of 227 KB: the static arrays come on top
@@ -807,7 +816,6 @@ int serve_attn_launch(SaArgs a, cudaStream_t st)
     }
     kern<<<grid, 32 * NW, smem, st>>>(a);
     DSV4CU_LAUNCH_CHECK();
-    if (TREE && a.splits > 1) return serve_join_launch<D, F16, (TERMS > 1)>(a, BN, st);
     return DSV4CU_OK;
 }
 

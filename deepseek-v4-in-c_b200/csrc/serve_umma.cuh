@@ -30,6 +30,7 @@
 #pragma once
 
 #include <cuda.h>
+#include <type_traits>
 
 #include "serve_attn.cuh"
 #include "tma_gemv.cuh"
@@ -42,7 +43,8 @@ constexpr int SU_BN = 128;                // keys per block
 constexpr int SU_THREADS = 384;
 constexpr int SU_SUB = 128 * 128;         // bytes of a 128-row x 64-column operand tile
 constexpr int SU_MAX_STAGES = 4;
-constexpr int SU_REGS_FEW = 72, SU_REGS_MANY = 216;   // per thread: copy and product warps, softmax warps
+constexpr int SU_REGS_FEW = 104, SU_REGS_MANY = 200;   // per thread: copy and product warps, softmax warps
+constexpr int SU_MIX = 2;                 // of four pairs of exponentials, those on the FMA pipe
 constexpr float SU_LAZY = 8.0f;           // log2 units the running maximum may fall behind
 enum { SUE_KEMPTY = 81, SUE_VEMPTY, SUE_KFULL, SUE_VFULL, SUE_S, SUE_P, SUE_O, SUE_Q, SUE_DRAIN };
 
@@ -88,6 +90,10 @@ DSV4CU_DEV void su_st32(uint32_t taddr, const uint32_t *r)
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
 }
+DSV4CU_DEV void su_st16(uint32_t taddr, const uint32_t *r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr) : "memory");
+}
 DSV4CU_DEV void su_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 DSV4CU_DEV void su_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 DSV4CU_DEV void su_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -98,6 +104,77 @@ DSV4CU_DEV void su_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0
 template <int R>
 DSV4CU_DEV void su_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R)); }
 
+// True in one lane of the (converged) warp.
+DSV4CU_DEV bool su_elect()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// Pairs of floats for the packed fp32 instructions.
+DSV4CU_DEV uint64_t su_f2(float x, float y)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+DSV4CU_DEV uint64_t su_u2(uint32_t x, uint32_t y)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(x), "r"(y));
+    return r;
+}
+DSV4CU_DEV void su_unf2(uint64_t v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+DSV4CU_DEV uint64_t su_fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+DSV4CU_DEV uint64_t su_add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// Largest of three, NaN if any is.
+DSV4CU_DEV float su_max3(float a, float b, float c)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of two finite numbers below 128 on the FMA pipe: x = n + f with n the
+// nearest integer (adding 1.5 * 2^23 leaves it in the low bits), a polynomial
+// for 2^f on [-1/2, 1/2] with equioscillating relative error - degree 3: 7.5e-5
+// for bf16 weights, whose rounding is 2^-9, degree 4: 2.6e-6 for f16 weights -
+// and n added to the exponent. Below 2^-126 the result stays at 2^-126.
+template <bool F16>
+DSV4CU_DEV uint64_t su_exp2_poly(uint64_t v)
+{
+    float x, y;
+    su_unf2(v, x, y);
+    v = su_f2(fmaxf(x, -126.0f), fmaxf(y, -126.0f));
+    constexpr float MAGIC = 12582912.0f;
+    const uint64_t n = su_add2(v, su_f2(MAGIC, MAGIC));
+    const uint64_t f = su_fma2(su_add2(n, su_f2(-MAGIC, -MAGIC)), su_f2(-1.0f, -1.0f), v);
+    uint64_t p;
+    if constexpr (F16) {
+        p = su_fma2(f, su_f2(0.0095701021f, 0.0095701021f), su_f2(0.055917859f, 0.055917859f));
+        p = su_fma2(p, f, su_f2(0.24024744f, 0.24024744f));
+        p = su_fma2(p, f, su_f2(0.69312179f, 0.69312179f));
+        p = su_fma2(p, f, su_f2(0.99999928f, 0.99999928f));
+    } else {
+        p = su_fma2(f, su_f2(0.055171669f, 0.055171669f), su_f2(0.24261113f, 0.24261113f));
+        p = su_fma2(p, f, su_f2(0.69326097f, 0.69326097f));
+        p = su_fma2(p, f, su_f2(0.99992806f, 0.99992806f));
+    }
+    float px, py, nx, ny;
+    su_unf2(p, px, py);
+    su_unf2(n, nx, ny);
+    return su_u2(__float_as_uint(px) + (__float_as_uint(nx) << 23), __float_as_uint(py) + (__float_as_uint(ny) << 23));
+}
+
 // Box of a [row][head][column] map; x = column (a multiple of 64).
 DSV4CU_DEV void su_tma(void *dst, const CUtensorMap *map, int x, int head, int row, uint64_t *bar)
 {
@@ -105,21 +182,23 @@ DSV4CU_DEV void su_tma(void *dst, const CUtensorMap *map, int x, int head, int r
                  " [%0], [%1, {%2, %3, %4}], [%5];"
                  ::"r"(umma::saddr(dst)), "l"(map), "r"(x), "r"(head), "r"(row), "r"(umma::saddr(bar)) : "memory");
 }
-// Bounded poll for the single-thread roles.
-DSV4CU_DEV bool su_spin(uint64_t *bar, uint32_t parity, int *err, int code)
+// Bounded wait that polls: no suspend hint and no look at the clock on the
+// way to a phase that completes in time (a strip's products and softmax wait
+// for each other every block).
+DSV4CU_DEV bool su_wait(uint64_t *bar, uint32_t parity, int *err, int code)
 {
     const uint32_t a = umma::saddr(bar);
     uint64_t t0 = 0;
-    for (uint32_t i = 0;; i++) {
+    for (uint32_t i = 1;; i++) {
         uint32_t ok;
         asm volatile("{\n\t.reg .pred p;\n\t"
                      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
                      "selp.u32 %0, 1, 0, p;\n\t}"
                      : "=r"(ok) : "r"(a), "r"(parity) : "memory");
         if (ok) return true;
-        if ((i & 255u) == 0u) {
+        if ((i & 1023u) == 0u) {
             const uint64_t now = globaltimer_ns();
-            if (i == 0) t0 = now;
+            if (t0 == 0) t0 = now;
             else if (now - t0 > MBAR_TIMEOUT_NS) break;
         }
     }
@@ -150,7 +229,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
     __shared__ uint32_t s_anc[TREE ? SA_MAX_NODES : 1][4];
     __shared__ int s_odd[2];
     uint8_t *smem = (uint8_t *)(((uintptr_t)su_raw + 1023) & ~(uintptr_t)1023);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
     const int rows_cta = a.two ? 256 : 128;
 
     // ---- which rows and keys
@@ -294,7 +373,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
 #pragma unroll
                 for (int kv = 0; kv < 2; kv++) {
                     uint64_t *full = kv ? &vfull[st] : &kfull[st], *empty = kv ? &vempty[st] : &kempty[st];
-                    if (lane == 0 && u > 0) ok = su_spin(empty, (u - 1) & 1, a.status, kv ? SUE_VEMPTY : SUE_KEMPTY);
+                    if (lane == 0 && u > 0) ok = su_wait(empty, (u - 1) & 1, a.status, kv ? SUE_VEMPTY : SUE_KEMPTY);
                     ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
                     if (!ok) break;
                     if (lane == 0) mbar_arrive_expect_tx(full, bytes);
@@ -312,56 +391,86 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                     mbar_wait(&kfull[j % a.nst], (j / a.nst) & 1, nullptr, 0);
                     mbar_wait(&vfull[j % a.nst], (j / a.nst) & 1, nullptr, 0);
                 }
-        } else if (warp == 1 && lane == 0) {
+        } else if (warp == 1) {
             // ------------------------------------------------ products
+            // The whole warp walks the blocks and one elected lane issues: what
+            // the instructions take comes from warp-uniform values (broadcast
+            // once), so descriptors stay in uniform registers. Issued by a lone
+            // lane, moving them there took longer than the products.
             constexpr uint32_t id_s = su_idesc(F16, SU_BN, false), id_o = su_idesc(F16, D, true);
-            bool ok = su_spin(&qfull, 0, a.status, SUE_Q);
-            umma::fence_after();
+            auto same = [](int x) { return __shfl_sync(0xFFFFFFFFu, x, 0); };
+            const bool one = su_elect();
+            const int u0 = same(c0), u1 = same(c1), g0 = same(f0), g1 = same(f1), h0 = same(e0), h1 = same(e1);
+            const int nst = a.nst;
+            const bool ualt = same(alt) != 0;
+            const int ustep = ualt ? 2 : 1;
+            const uint32_t ts = (uint32_t)same((int)tm_s), to = (uint32_t)same((int)tm_o);
+            // operand descriptors: the address field counts 16 bytes, and shared
+            // memory ends before it overflows
+            const uint64_t dq = umma::desc_sw128(qs), dk = umma::desc_sw128(ks), dv = su_desc_v(vs);
             uint32_t once = 0;                           // blocks that one of their two strips has scored
+            bool ok = su_wait(&qfull, 0, a.status, SUE_Q);
+            umma::fence_after();
+            // scores of strip s against block b: its key stage and phase
             auto scores = [&](int s, int b) {
-                const int n = b - c0, st = n % a.nst;
-                ok = ok && su_spin(&kfull[st], (n / a.nst) & 1, a.status, SUE_KFULL);
+                const int n = b - u0, use = n / nst, st = n - use * nst;
+                ok = ok && su_wait(&kfull[st], use & 1, a.status, SUE_KFULL);
                 if (!ok) return;
                 umma::fence_after();
-                const uint8_t *q = qs + (alt ? 0 : s) * KVB, *k = ks + st * KVB;
-#pragma unroll
-                for (int kk = 0; kk < D / 16; kk++) {
-                    const int at = (kk >> 2) * SU_SUB + 32 * (kk & 3);
-                    su_mma(tm_s + 128 * s, umma::desc_sw128(q + at), umma::desc_sw128(k + at), id_s, kk > 0);
-                }
-                umma::commit(&sfull[s]);
+                const uint64_t q = dq + (uint32_t)((ualt ? 0 : s) * (KVB >> 4)), k = dk + (uint32_t)(st * (KVB >> 4));
                 const uint32_t bit = 1u << (b & 31);
-                if (uses(s ^ 1, b) && !(once & bit)) {
-                    once |= bit;
-                } else {                                 // its last reader
-                    once &= ~bit;
-                    umma::commit(&kempty[st]);
+                const bool both = !ualt && b >= g1 && b < h0;    // two strips read this block
+                const bool last = !both || (once & bit);
+                once = both && !last ? once | bit : once & ~bit;
+                if (one) {
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; kk++) {
+                        const int at = ((kk >> 2) * SU_SUB + 32 * (kk & 3)) >> 4;
+                        su_mma(ts + 128 * s, q + at, k + at, id_s, kk > 0);
+                    }
+                    umma::commit(&sfull[s]);
+                    if (last) umma::commit(&kempty[st]);
                 }
+                __syncwarp();
             };
-            if (f0 < e0) scores(0, f0);
-            if (f1 < e1) scores(1, f1);
+            if (g0 < h0) scores(0, g0);
+            if (g1 < h1) scores(1, g1);
             uint32_t turn[2] = {0, 0};
-            for (int b = c0; b < c1 && ok; b++)
-                for (int s = 0; s < 2 && ok; s++) {
-                    if (!uses(s, b)) continue;
-                    const int n = b - c0, st = n % a.nst;
-                    ok = su_spin(&pfull[s], turn[s] & 1, a.status, SUE_P) &&
-                         su_spin(&vfull[st], (n / a.nst) & 1, a.status, SUE_VFULL);
+            int st = 0, phase = 0;
+            for (int b = u0; b < u1 && ok; b++) {
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    if (ualt ? ((b - u0) & 1) != s : s ? b < g1 : b >= h0) continue;   // strip 0 ends first, strip 1 starts last
+                    ok = ok && su_wait(&pfull[s], turn[s] & 1, a.status, SUE_P) &&
+                         su_wait(&vfull[st], phase, a.status, SUE_VFULL);
+                    ok = __all_sync(0xFFFFFFFFu, ok);
                     if (!ok) break;
                     umma::fence_after();
-                    const uint8_t *v = vs + st * KVB;
+                    const uint64_t v = dv + (uint32_t)(st * (KVB >> 4));
+                    const uint32_t more = turn[s] > 0;
+                    const bool last = s == 1 || ualt || b < g1;  // strip 1 comes second
+                    if (one) {
 #pragma unroll
-                    for (int kk = 0; kk < SU_BN / 16; kk++)
-                        su_mma_ta(tm_o + 128 * s, tm_s + 128 * s + 8 * kk, su_desc_v(v + 2048 * kk), id_o,
-                                  (turn[s] > 0 || kk > 0) ? 1u : 0u);
+                        for (int kk = 0; kk < SU_BN / 16; kk++)
+                            su_mma_ta(to + 128 * s, ts + 128 * s + 8 * kk, v + (2048 >> 4) * kk, id_o, kk > 0 ? 1u : more);
+                        if (last) umma::commit(&vempty[st]);
+                    }
+                    __syncwarp();
                     turn[s]++;
-                    if (s || !uses(1, b)) umma::commit(&vempty[st]);   // strip 1 comes second
-                    if (b + step < (s ? e1 : e0)) scores(s, b + step);
-                    else umma::commit(&ofull[s]);
+                    if (b + ustep < (s ? h1 : h0)) scores(s, b + ustep);
+                    else if (one) umma::commit(&ofull[s]);
                 }
+                if (++st == nst) {
+                    st = 0;
+                    phase ^= 1;
+                }
+            }
             // the products in flight complete before TMEM is released
-            umma::commit(&drain);
-            mbar_wait(&drain, 0, a.status, SUE_DRAIN);
+            if (one) {
+                umma::commit(&drain);
+                mbar_wait(&drain, 0, a.status, SUE_DRAIN);
+            }
+            __syncwarp();
         }
     } else {
         su_regs_inc<SU_REGS_MANY>();
@@ -418,7 +527,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
             // cache, or on a missing page
             const bool gaps = cached ? lost || base + SU_BN > t.kend : base + SU_BN > t.len;
             uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&sfull[s], turn & 1, a.status, SUE_S));
+            ok = __all_sync(0xFFFFFFFFu, su_wait(&sfull[s], turn & 1, a.status, SUE_S));
             if (!ok) break;
             if (gaps) {
                 // values of absent keys become zeros (what the copies left, or
@@ -427,7 +536,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                 // it, so the stage's last use is over and its barrier is at
                 // most one phase away: the parity below means this block.
                 const int n = b - c0, st = n % a.nst;
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(&vfull[st], (n / a.nst) & 1, a.status, SUE_VFULL));
+                ok = __all_sync(0xFFFFFFFFu, su_wait(&vfull[st], (n / a.nst) & 1, a.status, SUE_VFULL));
                 if (!ok) break;
                 if (!(cached ? in_pool(base + i) : base + i < t.len)) {
                     uint8_t *v = vs + st * KVB + i * 128;
@@ -471,9 +580,13 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < 128; k++) top[k & 3] = fmaxf(top[k & 3], __uint_as_float(x[k]));
-                const float mrow = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale2;
-                const bool move = mrow > m + SU_LAZY || (m == -INFINITY && mrow > m);
+                for (int k = 0; k < 128; k += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        top[e] = su_max3(top[e], __uint_as_float(x[k + 2 * e]), __uint_as_float(x[k + 2 * e + 1]));
+                float mrow = su_max3(su_max3(top[0], top[1], top[2]), top[3], top[3]) * a.scale2;
+                if (mrow == INFINITY) mrow = __uint_as_float(0x7FC00000u);   // inf - inf: the row is NaN, as NaN scores make it
+                const bool move = !(mrow <= m + SU_LAZY);
                 if (__any_sync(0xFFFFFFFFu, move)) {
                     const float to = move ? mrow : m, alpha = move ? sa_exp2(m - to) : 1.0f;
                     m = to;
@@ -491,17 +604,34 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                     }
                 }
                 const float use = m == -INFINITY ? 0.0f : m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint64_t scale2 = su_f2(a.scale2, a.scale2), shift2 = su_f2(-use, -use);
+                uint64_t sum[2] = {su_f2(l, 0.0f), su_f2(0.0f, 0.0f)};
+                auto weights = [&](auto mixed) {
 #pragma unroll
-                for (int k = 0; k < 128; k += 2) {
-                    const float p0 = sa_exp2(fmaf(__uint_as_float(x[k]), a.scale2, -use));
-                    const float p1 = sa_exp2(fmaf(__uint_as_float(x[k + 1]), a.scale2, -use));
-                    sum[(k >> 1) & 3] += p0 + p1;
-                    x[k >> 1] = sa_pack<F16>(p0, p1);
-                }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                su_st32(sp_s, x);
-                su_st32(sp_s + 32, x + 32);
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int k = 0; k < 16; k++) {
+                            uint64_t y = su_fma2(su_u2(x[32 * c + 2 * k], x[32 * c + 2 * k + 1]), scale2, shift2);
+                            if (decltype(mixed)::value && (k & 3) < SU_MIX) y = su_exp2_poly<F16>(y);
+                            else {
+                                float p, q;
+                                su_unf2(y, p, q);
+                                y = su_f2(sa_exp2(p), sa_exp2(q));
+                            }
+                            sum[k & 1] = su_add2(sum[k & 1], y);
+                            float p, q;
+                            su_unf2(y, p, q);
+                            w[k] = sa_pack<F16>(p, q);
+                        }
+                        su_st16(sp_s + 16 * c, w);
+                    }
+                };
+                if (masked) weights(std::false_type());  // masked entries are exactly 0
+                else weights(std::true_type());
+                float s0, s1;
+                su_unf2(su_add2(sum[0], sum[1]), s0, s1);
+                l = s0 + s1;
                 su_wait_st();
                 umma::fence_before();
             }
@@ -510,7 +640,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
         }
         // ---- outputs
         const bool any = first < end;
-        if (any) ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(&ofull[s], 0, a.status, SUE_O));
+        if (any) ok = ok && __all_sync(0xFFFFFFFFu, su_wait(&ofull[s], 0, a.status, SUE_O));
         umma::fence_after();
         const SaArgs &a0 = a;
         auto row_of = [t, ap = &a0](int blk, int j, bool values) -> const uint16_t * {
@@ -545,7 +675,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
             constexpr int OS = D + 4;
             float *xo = reinterpret_cast<float *>(ks), *xm = xo + 128 * OS, *xl = xm + 128;
             const bool two = f1 < e1;
-            if (s && two) ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait(&ofull[0], 0, a.status, SUE_O));
+            if (s && two) ok = ok && __all_sync(0xFFFFFFFFu, su_wait(&ofull[0], 0, a.status, SUE_O));
             if (s && two && live) {
 #pragma unroll
                 for (int c = 0; c < D; c += 32) {
@@ -666,6 +796,22 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                 if (s_odd[s] == 2) serve_slow_rows<D, F16, false>(a, ts, SU_BN, warp & 3, 4, sees, row_of);
             }
         }
+        if (TREE && t.parts > 1) {
+            // the tile's last split to finish joins them all
+            __threadfence();
+            su_bar<256>(1);
+            if (threadIdx.x == 128) {
+                int *count = a.counters + ((size_t)blockIdx.z * a.hkv + t.kvh) * a.row_tiles + blockIdx.x % a.row_tiles;
+                const bool last = atomicAdd(count, 1) == t.parts - 1;
+                if (last) *count = 0;
+                s_odd[0] = last;
+            }
+            su_bar<256>(1);
+            if (s_odd[0]) {
+                __threadfence();
+                sa_join<D, F16, false>(a, t, warp - 4, 8);
+            }
+        }
     }
     umma::fence_before();
     __syncthreads();
@@ -725,7 +871,7 @@ int serve_umma_launch(SaArgs a, bool tree, cudaStream_t st)
         return dsv4cu_set_error(DSV4CU_ERR_UNSUPPORTED, "serving attention: launched with %d registers a thread", regs[tree]);
     kern<<<grid, SU_THREADS, smem, st>>>(mk, mv, mkc, mvc, a);
     DSV4CU_LAUNCH_CHECK();
-    return tree && a.splits > 1 ? serve_join_launch<D, F16, false>(a, SU_BN, st) : DSV4CU_OK;
+    return DSV4CU_OK;
 }
 
 int serve_umma_bf16(const SaArgs &a, int D, bool tree, cudaStream_t st);
