@@ -143,7 +143,9 @@ static TreeShape tree_shape(const dsv4cu_ctx *ctx, const dsv4cu_tree_attn_args *
     if (least < 2) least = 2;
     int64_t chunk = (blocks * ctas + 8 * ctx->sm_count - 1) / (8 * ctx->sm_count);
     if (chunk < least) chunk = least;
-    if (chunk < (blocks + 63) / 64) chunk = (blocks + 63) / 64;
+    // the join keeps two numbers per split and row in 64 KB of shared memory
+    const int64_t most = s.two ? 32 : 64;
+    if (chunk < (blocks + most - 1) / most) chunk = (blocks + most - 1) / most;
     s.chunk = (int)chunk;
     s.splits = (int)((blocks + chunk - 1) / chunk);
     if (ctas > DSV4CU_MAX_COUNTERS) s.splits = 1;         // a counter per tile joins its splits

@@ -344,56 +344,87 @@ __device__ __noinline__ void serve_slow_rows(const SaArgs &a, const SaTile &t, i
     }
 }
 
-// Joins the splits of a tile's rows, a warp per row: the partial outputs
-// rescaled to the row's largest maximum and divided by the joint exp-sum (with
-// the sink), in split order whichever split came last.
-template <int D, bool F16, bool QF32>
-DSV4CU_DEV void sa_join(const SaArgs &a, const SaTile &t, int warp, int warps)
+// Joins the splits of a tile's rows: the partial outputs rescaled to the row's
+// largest maximum and divided by the joint exp-sum (with the sink), in split
+// order whichever split came last. First the maxima and sums into sm (2 parts
+// + 1 numbers a row), a row's factors by a thread; then the outputs, four
+// columns per thread.
+template <int D, bool F16, bool QF32, class Sync>
+DSV4CU_DEV void sa_join(const SaArgs &a, const SaTile &t, float *sm, int tid, int threads, Sync sync)
 {
-    const int lane = threadIdx.x & 31;
-    constexpr int E = D / 32, B = D >= 256 ? 4 : 8;      // columns of a lane; splits read at once
     const size_t step = (size_t)a.nt * a.hq;
-    for (int r = warp; r < t.rows; r += warps) {
-        const int pr = t.r0 + r, tok = pr / a.G, head = t.kvh * a.G + pr - tok * a.G;
-        const size_t id = (size_t)(t.begin + tok) * a.hq + head;
-        float m = -INFINITY;
-        for (int s = lane; s < t.parts; s += 32) m = fmaxf(m, __ldcg(a.pm + id + s * step));
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
-        float l = 0.0f, o[E];
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] = 0.0f;
-        const float use = m == -INFINITY ? 0.0f : m;
-        for (int s0 = 0; s0 < t.parts; s0 += 32) {
-            // a split's factor and sum by a lane each; one without a visible key has factor 0
-            const int n = min(32, t.parts - s0);
-            float f = 0.0f, ls = 0.0f;
-            if (lane < n) {
-                f = sa_exp2(__ldcg(a.pm + id + (s0 + lane) * step) - use);
-                ls = f != 0.0f ? __ldcg(a.pl + id + (s0 + lane) * step) : 0.0f;
-            }
-            for (int s = 0; s < n; s += B) {
-                float x[B][E], fs[B];
-#pragma unroll
-                for (int u = 0; u < B; u++) {
-                    fs[u] = __shfl_sync(0xFFFFFFFFu, f, min(s + u, 31));
-                    const float *src = a.po + (id + (s0 + s + u) * step) * D + lane;
-#pragma unroll
-                    for (int e = 0; e < E; e++) x[u][e] = s + u < n && fs[u] != 0.0f ? __ldcg(src + 32 * e) : 0.0f;
-                }
-#pragma unroll
-                for (int u = 0; u < B; u++) {
-                    if (s + u >= n) break;
-                    l = fmaf(__shfl_sync(0xFFFFFFFFu, ls, min(s + u, 31)), fs[u], l);
-#pragma unroll
-                    for (int e = 0; e < E; e++) o[e] = fmaf(x[u][e], fs[u], o[e]);
-                }
-            }
+    const int rows = t.rows, parts = t.parts;
+    float *inv = sm + parts * rows;
+    float *ls = inv + rows;                              // [parts][rows]
+    for (int x = tid; x < parts * rows; x += threads) {
+        const int p = x / rows, r = x - p * rows, pr = t.r0 + r, tok = pr / a.G, head = t.kvh * a.G + pr - tok * a.G;
+        const size_t id = (size_t)(t.begin + tok) * a.hq + head + p * step;
+        sm[x] = __ldcg(a.pm + id);
+        ls[x] = __ldcg(a.pl + id);
+    }
+    sync();
+    for (int r = tid; r < rows; r += threads) {
+        float m = -INFINITY, l = 0.0f;
+        for (int s = 0; s < parts; s++) {
+            const float x = sm[s * rows + r];
+            m = x > m || x != x ? x : m;                 // a NaN row stays one
         }
-        const float inv = sa_inv(l, m, a.sink, head);
-        const size_t at = (size_t)(t.begin + tok) * a.ldo + (size_t)head * D;
+        const float use = m == -INFINITY ? 0.0f : m;
+        for (int s = 0; s < parts; s++) {
+            const float f = sa_exp2(sm[s * rows + r] - use);
+            sm[s * rows + r] = f;
+            if (f != 0.0f) l = fmaf(ls[s * rows + r], f, l);   // factor 0: a split without a visible key
+        }
+        inv[r] = sa_inv(l, m, a.sink, t.kvh * a.G + (t.r0 + r) % a.G);
+    }
+    sync();
+    constexpr int B = 8;                                 // splits read at once, of two pieces each
+    for (int x0 = tid; x0 < rows * (D / 4); x0 += 2 * threads) {
+        float4 o[2];
+        const float *src[2];
+        int row[2];
+        size_t at[2];
 #pragma unroll
-        for (int e = 0; e < E; e++) sa_store_o<F16, QF32>(a, at + lane + 32 * e, o[e] * inv);
+        for (int u = 0; u < 2; u++) {
+            const int x = min(x0 + u * threads, rows * (D / 4) - 1);   // the last piece twice where there is no second
+            const int r = x / (D / 4), c = (x - r * (D / 4)) * 4, pr = t.r0 + r, tok = pr / a.G,
+                      head = t.kvh * a.G + pr - tok * a.G;
+            o[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            row[u] = r;
+            src[u] = a.po + ((size_t)(t.begin + tok) * a.hq + head) * D + c;
+            at[u] = (size_t)(t.begin + tok) * a.ldo + (size_t)head * D + c;
+        }
+        for (int s0 = 0; s0 < parts; s0 += B) {
+            float4 y[2][B];
+#pragma unroll
+            for (int s = 0; s < B; s++)
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+                    y[u][s] = s0 + s < parts ? __ldcg(reinterpret_cast<const float4 *>(src[u] + (s0 + s) * step * D))
+                                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int s = 0; s < B; s++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const float f = s0 + s < parts ? sm[(s0 + s) * rows + row[u]] : 0.0f;
+                    if (f != 0.0f) {
+                        o[u].x = fmaf(y[u][s].x, f, o[u].x);
+                        o[u].y = fmaf(y[u][s].y, f, o[u].y);
+                        o[u].z = fmaf(y[u][s].z, f, o[u].z);
+                        o[u].w = fmaf(y[u][s].w, f, o[u].w);
+                    }
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const float i = inv[row[u]];
+            if constexpr (QF32)
+                *reinterpret_cast<float4 *>(reinterpret_cast<float *>(a.o) + at[u]) =
+                    make_float4(o[u].x * i, o[u].y * i, o[u].z * i, o[u].w * i);
+            else
+                *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.o) + at[u]) =
+                    make_uint2(sa_pack<F16>(o[u].x * i, o[u].y * i), sa_pack<F16>(o[u].z * i, o[u].w * i));
+        }
     }
 }
 
@@ -785,7 +816,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
         __syncthreads();
         if (s_bad[0]) {
             __threadfence();
-            sa_join<D, F16, QF32>(a, t, warp, NW);
+            sa_join<D, F16, QF32>(a, t, part, tid, THREADS, [] { __syncthreads(); });
         }
     }
 }

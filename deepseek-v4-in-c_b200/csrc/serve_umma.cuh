@@ -30,7 +30,6 @@
 #pragma once
 
 #include <cuda.h>
-#include <type_traits>
 
 #include "serve_attn.cuh"
 #include "tma_gemv.cuh"
@@ -43,8 +42,7 @@ constexpr int SU_BN = 128;                // keys per block
 constexpr int SU_THREADS = 384;
 constexpr int SU_SUB = 128 * 128;         // bytes of a 128-row x 64-column operand tile
 constexpr int SU_MAX_STAGES = 4;
-constexpr int SU_REGS_FEW = 104, SU_REGS_MANY = 200;   // per thread: copy and product warps, softmax warps
-constexpr int SU_MIX = 2;                 // of four pairs of exponentials, those on the FMA pipe
+constexpr int SU_REGS_FEW = 72, SU_REGS_MANY = 216;   // per thread: copy and product warps, softmax warps
 constexpr float SU_LAZY = 8.0f;           // log2 units the running maximum may fall behind
 enum { SUE_KEMPTY = 81, SUE_VEMPTY, SUE_KFULL, SUE_VFULL, SUE_S, SUE_P, SUE_O, SUE_Q, SUE_DRAIN };
 
@@ -90,11 +88,24 @@ DSV4CU_DEV void su_st32(uint32_t taddr, const uint32_t *r)
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
 }
+// 16 columns, arrived.
+DSV4CU_DEV void su_ld16(uint32_t taddr, uint32_t *r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
+}
 DSV4CU_DEV void su_st16(uint32_t taddr, const uint32_t *r)
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr) : "memory");
 }
 DSV4CU_DEV void su_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Behind su_wait_ld: values of a load that arithmetic may only use from here
+// on (nothing else ties the use of a loaded register to the wait).
+DSV4CU_DEV void su_loaded32(uint32_t *r)
+{
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
 DSV4CU_DEV void su_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 DSV4CU_DEV void su_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 template <int N>
@@ -144,37 +155,6 @@ DSV4CU_DEV float su_max3(float a, float b, float c)
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 2^x of two finite numbers below 128 on the FMA pipe: x = n + f with n the
-// nearest integer (adding 1.5 * 2^23 leaves it in the low bits), a polynomial
-// for 2^f on [-1/2, 1/2] with equioscillating relative error - degree 3: 7.5e-5
-// for bf16 weights, whose rounding is 2^-9, degree 4: 2.6e-6 for f16 weights -
-// and n added to the exponent. Below 2^-126 the result stays at 2^-126.
-template <bool F16>
-DSV4CU_DEV uint64_t su_exp2_poly(uint64_t v)
-{
-    float x, y;
-    su_unf2(v, x, y);
-    v = su_f2(fmaxf(x, -126.0f), fmaxf(y, -126.0f));
-    constexpr float MAGIC = 12582912.0f;
-    const uint64_t n = su_add2(v, su_f2(MAGIC, MAGIC));
-    const uint64_t f = su_fma2(su_add2(n, su_f2(-MAGIC, -MAGIC)), su_f2(-1.0f, -1.0f), v);
-    uint64_t p;
-    if constexpr (F16) {
-        p = su_fma2(f, su_f2(0.0095701021f, 0.0095701021f), su_f2(0.055917859f, 0.055917859f));
-        p = su_fma2(p, f, su_f2(0.24024744f, 0.24024744f));
-        p = su_fma2(p, f, su_f2(0.69312179f, 0.69312179f));
-        p = su_fma2(p, f, su_f2(0.99999928f, 0.99999928f));
-    } else {
-        p = su_fma2(f, su_f2(0.055171669f, 0.055171669f), su_f2(0.24261113f, 0.24261113f));
-        p = su_fma2(p, f, su_f2(0.69326097f, 0.69326097f));
-        p = su_fma2(p, f, su_f2(0.99992806f, 0.99992806f));
-    }
-    float px, py, nx, ny;
-    su_unf2(p, px, py);
-    su_unf2(n, nx, ny);
-    return su_u2(__float_as_uint(px) + (__float_as_uint(nx) << 23), __float_as_uint(py) + (__float_as_uint(ny) << 23));
-}
-
 // Box of a [row][head][column] map; x = column (a multiple of 64).
 DSV4CU_DEV void su_tma(void *dst, const CUtensorMap *map, int x, int head, int row, uint64_t *bar)
 {
@@ -228,6 +208,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
     __shared__ int s_par[TREE ? SA_MAX_NODES : 1], s_depth[TREE ? SA_MAX_NODES : 1];
     __shared__ uint32_t s_anc[TREE ? SA_MAX_NODES : 1][4];
     __shared__ int s_odd[2];
+    __shared__ SaTile s_t;                               // for what is seldom looked at
     uint8_t *smem = (uint8_t *)(((uintptr_t)su_raw + 1023) & ~(uintptr_t)1023);
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
     const int rows_cta = a.two ? 256 : 128;
@@ -288,8 +269,27 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
         return s ? b >= f1 && b < e1 && (!alt || ((b - f1) & 1) == 0) : b >= f0 && b < e0 && (!alt || ((b - f0) & 1) == 0);
     };
 
+    // The softmax warps' queries are on their way while the rest is set up:
+    // strip s by its own warps, a single strip by all.
+    constexpr int QN = D / 8;                            // 16-byte pieces of a thread
+    uint4 qw[QN];
+    const int q_s = alt ? 0 : (warp - 4) >> 2, q_n = alt ? 256 : 128, q_i = (threadIdx.x - 128) & (q_n - 1);
+    if (warp >= 4) {
+        const int n = min(128, t.rows - 128 * q_s);
+#pragma unroll
+        for (int e = 0; e < QN; e++) {
+            const int x = q_i + e * q_n, r = x / (D / 8), ch = x - r * (D / 8);
+            qw[e] = make_uint4(0, 0, 0, 0);
+            if (r < n) {
+                const int pr = t.r0 + 128 * q_s + r, tok = pr / a.G, head = t.kvh * a.G + pr - tok * a.G;
+                qw[e] = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) +
+                                                              (size_t)(t.begin + tok) * a.ldq + (size_t)head * D + 8 * ch));
+            }
+        }
+    }
     uint8_t *qs = smem, *ks = qs + (a.two ? 2 : 1) * KVB, *vs = ks + a.nst * KVB;
     if (threadIdx.x == 0) {
+        s_t = t;
         for (int s = 0; s < SU_MAX_STAGES; s++) {
             mbar_init(&kfull[s], 1);
             mbar_init(&kempty[s], 1);
@@ -478,18 +478,11 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
         const int s = (warp - 4) >> 2, i = (threadIdx.x - 128) & 127;    // strip; row, and key in prepared values
         const int row0 = alt ? 0 : 128 * s, rows = min(128, t.rows - row0);
         {
-            // queries: strip s by its own warps, a single strip by all
-            const int r_n = alt ? 256 : 128, r_i = alt ? threadIdx.x - 128 : i;
-            for (int x = r_i; x < 128 * (D / 8); x += r_n) {
-                const int r = x / (D / 8), ch = x - r * (D / 8);
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (r < rows) {
-                    const int pr = t.r0 + row0 + r, tok = pr / a.G, head = t.kvh * a.G + pr - tok * a.G;
-                    w = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) +
-                                                              (size_t)(t.begin + tok) * a.ldq + (size_t)head * D + 8 * ch));
-                }
-                *reinterpret_cast<uint4 *>(qs + (alt ? 0 : s) * KVB + (ch >> 3) * SU_SUB + r * 128 +
-                                           (((ch & 7) ^ (r & 7)) << 4)) = w;
+            uint8_t *q = qs + (alt ? 0 : s) * KVB;
+#pragma unroll
+            for (int e = 0; e < QN; e++) {
+                const int x = q_i + e * q_n, r = x / (D / 8), ch = x - r * (D / 8);
+                if (r < 128) *reinterpret_cast<uint4 *>(q + (ch >> 3) * SU_SUB + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = qw[e];
             }
             su_fence_async();
             __syncwarp();
@@ -505,31 +498,35 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
         float m = -INFINITY, l = 0.0f;
         uint32_t turn = 0;
         bool ok = true;
-        auto is_full = [t, tok_lo, tok_hi, w = a.window](int b) {   // no mask crosses the block (missing pages aside)
-            if constexpr (TREE) {
-                const int base = t.key0 + b * SU_BN;
-                return b < t.nblk_c && base + SU_BN <= t.kend && t.ctx + t.len - base <= w;
-            } else {
-                return b * SU_BN + SU_BN - 1 <= tok_lo && tok_hi - b * SU_BN < w;
-            }
-        };
+        // blocks full_lo .. full_hi - 1 are crossed by no mask (missing pages aside)
+        int full_lo, full_hi;
+        if constexpr (TREE) {
+            const int back = t.ctx + t.len - a.window;   // no key below this is in every row's window
+            full_lo = back <= t.key0 ? 0 : (back - t.key0 + SU_BN - 1) / SU_BN;
+            full_hi = (t.kend - t.key0) / SU_BN;         // at least 0 where there are cached blocks
+        } else {
+            const int back = tok_hi - a.window + 1;
+            full_lo = back <= 0 ? 0 : (back + SU_BN - 1) / SU_BN;
+            full_hi = (tok_lo + 1) / SU_BN;
+        }
+        auto is_full = [full_lo, full_hi](int b) { return b >= full_lo && b < full_hi; };
+        const SaTile *tp = &s_t;
         auto in_pool = [&](int key) {
-            if (key >= t.kend) return false;
-            const int id = __ldg(t.table + (key >> a.page_log2));
+            if (key >= tp->kend) return false;
+            const int id = __ldg(tp->table + (key >> a.page_log2));
             return id >= 0 && id < a.n_pages;
         };
         for (int b = first; b < end; b += step, turn++) {
             // ---- the mask
-            const bool cached = TREE && b < t.nblk_c;
-            const int base = (TREE ? (cached ? t.key0 + b * SU_BN : (b - t.nblk_c) * SU_BN) : b * SU_BN);
-            const bool masked = !is_full(b) || (cached && lost);
-            // keys that are not there: behind the sequence, the nodes or the
-            // cache, or on a missing page
-            const bool gaps = cached ? lost || base + SU_BN > t.kend : base + SU_BN > t.len;
+            const bool masked = !is_full(b) || (TREE && lost);
             uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
             ok = __all_sync(0xFFFFFFFFu, su_wait(&sfull[s], turn & 1, a.status, SUE_S));
             if (!ok) break;
-            if (gaps) {
+            const bool cached = TREE && b < tp->nblk_c;
+            const int base = (TREE ? (cached ? tp->key0 + b * SU_BN : (b - tp->nblk_c) * SU_BN) : b * SU_BN);
+            // keys that are not there: behind the sequence, the nodes or the
+            // cache, or on a missing page
+            if (masked && (cached ? lost || base + SU_BN > tp->kend : base + SU_BN > tp->len)) {
                 // values of absent keys become zeros (what the copies left, or
                 // brought from the next sequence, may be no number). Behind
                 // this block's scores lie the products of every block before
@@ -538,7 +535,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                 const int n = b - c0, st = n % a.nst;
                 ok = __all_sync(0xFFFFFFFFu, su_wait(&vfull[st], (n / a.nst) & 1, a.status, SUE_VFULL));
                 if (!ok) break;
-                if (!(cached ? in_pool(base + i) : base + i < t.len)) {
+                if (!(cached ? in_pool(base + i) : base + i < tp->len)) {
                     uint8_t *v = vs + st * KVB + i * 128;
 #pragma unroll
                     for (int c = 0; c < DC; c++)
@@ -549,17 +546,17 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
             }
             if (masked) {
                 if (cached) {
-                    const int pos = t.ctx + depth, lo = a.window > pos ? 0 : pos - a.window + 1 - base;
+                    const int pos = tp->ctx + depth, lo = a.window > pos ? 0 : pos - a.window + 1 - base;
 #pragma unroll
                     for (int w = 0; w < 4; w++) {
-                        vis[w] = su_range(lo, t.kend - 1 - base, w);
+                        vis[w] = su_range(lo, tp->kend - 1 - base, w);
                         if (lost) vis[w] &= __ballot_sync(0xFFFFFFFFu, in_pool(base + 32 * w + lane));
                     }
                 } else if (TREE) {
 #pragma unroll
                     for (int w = 0; w < 4; w++) vis[w] = s_anc[tok][w];
                     if (depth >= a.window)
-                        for (int x = 0; x < t.len; x++)
+                        for (int x = 0; x < tp->len; x++)
                             if (depth - s_depth[x] >= a.window) vis[x >> 5] &= ~(1u << (x & 31));
                 } else {
                     const int lo = a.window > tok ? 0 : tok - a.window + 1 - base;
@@ -573,6 +570,8 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
 #pragma unroll
                 for (int c = 0; c < 4; c++) su_ld32(sp_s + 32 * c, x + 32 * c);
                 su_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 4; c++) su_loaded32(x + 32 * c);
                 if (masked) {
 #pragma unroll
                     for (int k = 0; k < 128; k++)
@@ -592,43 +591,33 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                     m = to;
                     l *= alpha;
                     if (turn > 0) {                      // the products so far are complete: S came behind them
+#pragma unroll 2
+                        for (int c = 0; c < D; c += 16) {    // few columns at a time: the scores stay in registers
+                            uint32_t o[16];
+                            su_ld16(sp_o + c, o);
 #pragma unroll
-                        for (int c = 0; c < D; c += 32) {
-                            uint32_t o[32];
-                            su_ld32(sp_o + c, o);
-                            su_wait_ld();
-#pragma unroll
-                            for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-                            su_st32(sp_o + c, o);
+                            for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                            su_st16(sp_o + c, o);
                         }
                     }
                 }
                 const float use = m == -INFINITY ? 0.0f : m;
                 const uint64_t scale2 = su_f2(a.scale2, a.scale2), shift2 = su_f2(-use, -use);
                 uint64_t sum[2] = {su_f2(l, 0.0f), su_f2(0.0f, 0.0f)};
-                auto weights = [&](auto mixed) {
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        uint32_t w[16];
+                for (int c = 0; c < 4; c++) {
+                    uint32_t w[16];
 #pragma unroll
-                        for (int k = 0; k < 16; k++) {
-                            uint64_t y = su_fma2(su_u2(x[32 * c + 2 * k], x[32 * c + 2 * k + 1]), scale2, shift2);
-                            if (decltype(mixed)::value && (k & 3) < SU_MIX) y = su_exp2_poly<F16>(y);
-                            else {
-                                float p, q;
-                                su_unf2(y, p, q);
-                                y = su_f2(sa_exp2(p), sa_exp2(q));
-                            }
-                            sum[k & 1] = su_add2(sum[k & 1], y);
-                            float p, q;
-                            su_unf2(y, p, q);
-                            w[k] = sa_pack<F16>(p, q);
-                        }
-                        su_st16(sp_s + 16 * c, w);
+                    for (int k = 0; k < 16; k++) {
+                        float p, q;
+                        su_unf2(su_fma2(su_u2(x[32 * c + 2 * k], x[32 * c + 2 * k + 1]), scale2, shift2), p, q);
+                        p = sa_exp2(p);
+                        q = sa_exp2(q);
+                        sum[k & 1] = su_add2(sum[k & 1], su_f2(p, q));
+                        w[k] = sa_pack<F16>(p, q);
                     }
-                };
-                if (masked) weights(std::false_type());  // masked entries are exactly 0
-                else weights(std::true_type());
+                    su_st16(sp_s + 16 * c, w);
+                }
                 float s0, s1;
                 su_unf2(su_add2(sum[0], sum[1]), s0, s1);
                 l = s0 + s1;
@@ -643,8 +632,9 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
         if (any) ok = ok && __all_sync(0xFFFFFFFFu, su_wait(&ofull[s], 0, a.status, SUE_O));
         umma::fence_after();
         const SaArgs &a0 = a;
-        auto row_of = [t, ap = &a0](int blk, int j, bool values) -> const uint16_t * {
+        auto row_of = [tp, ap = &a0](int blk, int j, bool values) -> const uint16_t * {
             const SaArgs &a = *ap;
+            const SaTile &t = *tp;
             const bool vv = values && a.v != nullptr;
             if (TREE && blk < t.nblk_c) {
                 const int key = t.key0 + blk * SU_BN + j;
@@ -655,8 +645,9 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
             return reinterpret_cast<const uint16_t *>(vv ? a.v : a.k) + (size_t)(t.begin + key) * (vv ? a.ldv : a.ldk) +
                    (size_t)t.kvh * D;
         };
-        auto sees = [t, row_of, ap = &a0, dp = &s_depth[0], an = &s_anc[0]](int tok, int blk, int j) -> bool {
+        auto sees = [tp, row_of, ap = &a0, dp = &s_depth[0], an = &s_anc[0]](int tok, int blk, int j) -> bool {
             const SaArgs &a = *ap;
+            const SaTile &t = *tp;
             if constexpr (TREE) {
                 if (blk < t.nblk_c) {
                     const int key = t.key0 + blk * SU_BN + j;
@@ -669,132 +660,128 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                 return key <= tok && tok - key < a.window;
             }
         };
+        // A warp's rows go out through its own part of the shared memory that
+        // the products are done with, so that stores cover whole rows. With two
+        // strips that is the strip's queries; a single strip first adds its
+        // even and odd blocks: each half of the columns is finished by one
+        // strip's warps, which get the other strip's share of it through xch.
+        constexpr int PN = D == 128 ? 16 : 8;            // 16-byte pieces of a row per pass
+        constexpr int XN = D / 8;                        // 16-byte pieces of half a row of floats
+        uint8_t *out = alt ? ks + 65536 + (warp - 4) * (PN * 512) : qs + s * KVB + (warp & 3) * (PN * 512);
+        float f_own = 1.0f;
+        const int col0 = alt ? s * (D / 2) : 0, ncol = alt ? D / 2 : D;
         if (alt) {
-            // the odd blocks' rows go through shared memory (every product has
-            // read its operands) to the even blocks' threads
-            constexpr int OS = D + 4;
-            float *xo = reinterpret_cast<float *>(ks), *xm = xo + 128 * OS, *xl = xm + 128;
-            const bool two = f1 < e1;
-            if (s && two) ok = ok && __all_sync(0xFFFFFFFFu, su_wait(&ofull[0], 0, a.status, SUE_O));
-            if (s && two && live) {
-#pragma unroll
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    su_ld32(sp_o + c, o);
-                    su_wait_ld();
-#pragma unroll
-                    for (int k = 0; k < 32; k += 4)
-                        *reinterpret_cast<uint4 *>(xo + i * OS + c + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-                }
-                xm[i] = m;
-                xl[i] = l;
-            }
+            float2 *ml = reinterpret_cast<float2 *>(ks + 65536);
+            su_bar<256>(1);                              // both strips' products are complete: the stages are free
+            ml[128 * s + i] = make_float2(m, l);
             su_bar<256>(1);
-            bool odd = false;
-            if (s == 0 && live) {
-                float f_a = 1.0f, f_b = 0.0f;
-                if (two) {
-                    const float mb = xm[i], top = fmaxf(m, mb), use = top == -INFINITY ? 0.0f : top;
-                    f_a = sa_exp2(m - use);
-                    f_b = sa_exp2(mb - use);
-                    l = l * f_a + xl[i] * f_b;
-                    m = top;
-                }
-                const bool part = t.parts > 1;
-                const float inv = part ? 1.0f : sa_inv(l, m, a.sink, head);
-                const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + tok) * a.hq + head;
-                const size_t at = (size_t)(t.begin + tok) * a.ldo + (size_t)head * D;
-                if (part && i < rows) {
-                    a.pm[id] = m;
-                    a.pl[id] = l;
-                }
-#pragma unroll
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    su_ld32(sp_o + c, o);
-                    su_wait_ld();
-                    float y[32];
-#pragma unroll
-                    for (int k = 0; k < 32; k++) {
-                        y[k] = __uint_as_float(o[k]) * f_a;
-                        if (two) y[k] = fmaf(xo[i * OS + c + k], f_b, y[k]);
-                        odd = odd || (i < rows && !isfinite(y[k]));
-                        y[k] *= inv;
-                    }
-                    if (i < rows) {
-#pragma unroll
-                        for (int k = 0; k < 32; k += 8) {
-                            if (part) {
-                                float4 *d = reinterpret_cast<float4 *>(a.po + id * D + c + k);
-                                d[0] = make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]);
-                                d[1] = make_float4(y[k + 4], y[k + 5], y[k + 6], y[k + 7]);
-                            } else {
-                                *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.o) + at + c + k) =
-                                    make_uint4(sa_pack<F16>(y[k], y[k + 1]), sa_pack<F16>(y[k + 2], y[k + 3]),
-                                               sa_pack<F16>(y[k + 4], y[k + 5]), sa_pack<F16>(y[k + 6], y[k + 7]));
-                            }
-                        }
-                    }
-                }
-            }
-            // a row that is not finite: was it a value behind the mask?
-            if (odd) s_odd[0] = 1;
-            su_bar<256>(1);
-            if (s_odd[0]) {
-                if (sa_suspect<D, F16, false>(t, SU_BN, threadIdx.x - 128, 256, is_full, row_of)) s_odd[1] = 1;
-                su_bar<256>(1);
-                if (s_odd[1]) serve_slow_rows<D, F16, false>(a, t, SU_BN, warp - 4, 8, sees, row_of);
-            }
-        } else {
-            bool odd = false;
+            const float2 other = ml[128 * (s ^ 1) + i];
+            const float top = m != m || other.x != other.x ? m + other.x : fmaxf(m, other.x);
+            const float use = top == -INFINITY ? 0.0f : top;
+            f_own = sa_exp2(m - use);
+            l = l * f_own + other.y * sa_exp2(other.x - use);
+            m = top;
             if (live) {
-                const bool part = t.parts > 1;
-                const float inv = part ? 1.0f : sa_inv(l, m, a.sink, head);
-                const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + tok) * a.hq + head;
-                const size_t at = (size_t)(t.begin + tok) * a.ldo + (size_t)head * D;
-                if (part && i < rows) {
-                    a.pm[id] = m;
-                    a.pl[id] = l;
-                }
+                uint8_t *x = ks + (s ^ 1) * 32768 + i * (XN * 16);
+                for (int c = 0; c < D / 2; c += 16) {
+                    uint32_t o[16];
+                    if (any) su_ld16(sp_o + (s ^ 1) * (D / 2) + c, o);
 #pragma unroll
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    su_ld32(sp_o + c, o);
-                    su_wait_ld();
-                    if (i < rows) {
+                    for (int k = 0; k < 16; k += 4) {
+                        float y[4];
 #pragma unroll
-                        for (int k = 0; k < 32; k += 8) {
-                            float y[8];
-#pragma unroll
-                            for (int e = 0; e < 8; e++) {
-                                odd = odd || !isfinite(__uint_as_float(o[k + e]));
-                                y[e] = __uint_as_float(o[k + e]) * inv;
-                            }
-                            if (part) {
-                                float4 *d = reinterpret_cast<float4 *>(a.po + id * D + c + k);
-                                d[0] = make_float4(y[0], y[1], y[2], y[3]);
-                                d[1] = make_float4(y[4], y[5], y[6], y[7]);
-                            } else {
-                                *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.o) + at + c + k) =
-                                    make_uint4(sa_pack<F16>(y[0], y[1]), sa_pack<F16>(y[2], y[3]),
-                                               sa_pack<F16>(y[4], y[5]), sa_pack<F16>(y[6], y[7]));
-                            }
-                        }
+                        for (int e = 0; e < 4; e++) y[e] = any ? __uint_as_float(o[k + e]) * f_own : 0.0f;
+                        *reinterpret_cast<float4 *>(x + ((((c + k) >> 2) ^ (i & 7)) << 4)) = make_float4(y[0], y[1], y[2], y[3]);
                     }
                 }
             }
-            if (odd) s_odd[s] = 1;
-            su_bar<128>(2 + s);
-            if (s_odd[s]) {
-                SaTile ts = t;
-                ts.r0 = t.r0 + row0;
-                ts.rows = rows;
+            su_bar<256>(1);
+        }
+        bool odd = false;
+        if (live) {
+            const bool part = t.parts > 1;
+            const float inv = part ? 1.0f : sa_inv(l, m, a.sink, head);
+            const size_t row_id = (size_t)(t.begin + tok) * a.hq + head;
+            const size_t id = (size_t)t.split * a.nt * a.hq + row_id;
+            if (part && i < rows && (!alt || s == 0)) {
+                a.pm[id] = m;
+                a.pl[id] = l;
+            }
+            char *dst = part ? reinterpret_cast<char *>(a.po + id * D + col0)
+                             : reinterpret_cast<char *>(reinterpret_cast<uint16_t *>(a.o) + (size_t)(t.begin + tok) * a.ldo +
+                                                        (size_t)head * D + col0);
+            const uint8_t *x = ks + s * 32768 + i * (XN * 16);
+            const int mine = min(32, rows - 32 * (warp & 3));    // rows of this warp
+            int piece = 0;                               // of the pass
+            for (int c = 0; c < ncol; c += 16) {         // a loop: its code is cold at every launch
+                uint32_t o[16];
+                if (any) su_ld16(sp_o + col0 + c, o);
+                float y[16];
+#pragma unroll
+                for (int k = 0; k < 16; k++) y[k] = any ? __uint_as_float(o[k]) * f_own : 0.0f;
+                if (alt)
+#pragma unroll
+                    for (int k = 0; k < 16; k += 4) {
+                        const float4 z = *reinterpret_cast<const float4 *>(x + ((((c + k) >> 2) ^ (i & 7)) << 4));
+                        y[k] += z.x;
+                        y[k + 1] += z.y;
+                        y[k + 2] += z.z;
+                        y[k + 3] += z.w;
+                    }
+#pragma unroll
+                for (int k = 0; k < 16; k++) {
+                    odd = odd || !isfinite(y[k]);
+                    y[k] *= inv;
+                }
+                uint8_t *w = out + lane * (PN * 16);
+                if (part) {
+#pragma unroll
+                    for (int k = 0; k < 16; k += 4)
+                        *reinterpret_cast<float4 *>(w + (((piece + k / 4) ^ (lane & 7)) << 4)) =
+                            make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]);
+                    piece += 4;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 16; k += 8)
+                        *reinterpret_cast<uint4 *>(w + (((piece + k / 8) ^ (lane & 7)) << 4)) =
+                            make_uint4(sa_pack<F16>(y[k], y[k + 1]), sa_pack<F16>(y[k + 2], y[k + 3]),
+                                       sa_pack<F16>(y[k + 4], y[k + 5]), sa_pack<F16>(y[k + 6], y[k + 7]));
+                    piece += 2;
+                }
+                if (piece == PN || c + 16 >= ncol) {     // the pass is full: 2^b pieces per row
+                    const int b = 31 - __clz(piece);
+                    __syncwarp();
+#pragma unroll 4
+                    for (int e = 0; e < (mine << b); e += 32) {
+                        const int r = (e + lane) >> b, pc = (e + lane) & (piece - 1);
+                        char *d = reinterpret_cast<char *>(__shfl_sync(0xFFFFFFFFu, (unsigned long long)dst, r & 31));
+                        if (r < mine)
+                            *reinterpret_cast<uint4 *>(d + 16 * pc) =
+                                *reinterpret_cast<const uint4 *>(out + r * (PN * 16) + ((pc ^ (r & 7)) << 4));
+                    }
+                    __syncwarp();
+                    dst += 16 * piece;
+                    piece = 0;
+                }
+            }
+            odd = odd && i < rows;
+        }
+        // a row that is not finite: was it a value behind the mask?
+        const int who = alt ? 0 : s;
+        if (odd) s_odd[who] = 1;
+        alt ? su_bar<256>(1) : su_bar<128>(2 + s);
+        if (s_odd[who]) {
+            SaTile ts = t;
+            ts.r0 = t.r0 + row0;
+            ts.rows = rows;
+            if (!alt) {
                 ts.blk0 = first;
                 ts.blk1 = end;
-                if (sa_suspect<D, F16, false>(ts, SU_BN, i, 128, is_full, row_of)) s_odd[s] = 2;
-                su_bar<128>(2 + s);
-                if (s_odd[s] == 2) serve_slow_rows<D, F16, false>(a, ts, SU_BN, warp & 3, 4, sees, row_of);
             }
+            const int threads = alt ? 256 : 128, thread = alt ? threadIdx.x - 128 : i;
+            if (sa_suspect<D, F16, false>(ts, SU_BN, thread, threads, is_full, row_of)) s_odd[who] = 2;
+            alt ? su_bar<256>(1) : su_bar<128>(2 + s);
+            if (s_odd[who] == 2) serve_slow_rows<D, F16, false>(a, ts, SU_BN, thread >> 5, threads >> 5, sees, row_of);
         }
         if (TREE && t.parts > 1) {
             // the tile's last split to finish joins them all
@@ -809,7 +796,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
             su_bar<256>(1);
             if (s_odd[0]) {
                 __threadfence();
-                sa_join<D, F16, false>(a, t, warp - 4, 8);
+                sa_join<D, F16, false>(a, t, reinterpret_cast<float *>(ks), threadIdx.x - 128, 256, [] { su_bar<256>(1); });
             }
         }
     }
