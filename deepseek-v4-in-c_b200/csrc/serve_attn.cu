@@ -132,19 +132,21 @@ static TreeShape tree_shape(const dsv4cu_ctx *ctx, const dsv4cu_tree_attn_args *
     s.umma = use_umma(a, c);
     const int64_t rows = (int64_t)a->max_nodes * (a->n_heads / a->n_kv);
     s.two = s.umma && rows > 128;
-    const int BM = s.umma ? (s.two ? 256 : 128) : SA_BM, BN = s.umma ? 128 : sa_block(a->head_dim, a->v == nullptr);
+    const int BM = s.umma ? (s.two ? 256 : 128) : SA_BM, BN = s.umma ? a->head_dim : sa_block(a->head_dim, a->v == nullptr);
     s.row_tiles = (int)((rows + BM - 1) / BM);
     const int64_t ctas = (int64_t)s.row_tiles * a->n_kv * a->n_req;
     const int seen = a->window && a->window < a->max_ctx ? a->window : a->max_ctx;
     const int64_t blocks = (int64_t)seen / BN + 2;        // the cached ones and the nodes' own
-    // about 8 CTAs per SM in all; a split of few blocks costs more for its
-    // partial rows (4 (D + 2) bytes each, written and read) than it saves
-    int64_t least = min(rows, (int64_t)BM) / 8;
-    if (least < 2) least = 2;
-    int64_t chunk = (blocks * ctas + 8 * ctx->sm_count - 1) / (8 * ctx->sm_count);
+    // about 4 CTAs per SM in all (8 where two run at a time): fewer leave SMs
+    // idle at the end, more pay for set-up and partial rows - 4 (D + 2) bytes
+    // each, written and read, which also sets the least blocks of a split
+    const int64_t goal = (int64_t)ctx->sm_count * (s.umma && BN == 64 ? 8 : 4);
+    int64_t least = min(rows, (int64_t)BM) * 16 / BN;
+    if (least < 256 / BN) least = 256 / BN;
+    int64_t chunk = (blocks * ctas + goal - 1) / goal;
     if (chunk < least) chunk = least;
     // the join keeps two numbers per split and row in 64 KB of shared memory
-    const int64_t most = s.two ? 32 : 64;
+    const int64_t most = s.two ? 30 : 60;
     if (chunk < (blocks + most - 1) / most) chunk = (blocks + most - 1) / most;
     s.chunk = (int)chunk;
     s.splits = (int)((blocks + chunk - 1) / chunk);

@@ -3,8 +3,8 @@
 // cache whose pages TMA can copy. The mathematics, the packing of grouped
 // heads into rows and the masks are those of serve_attn.cuh.
 //
-// A CTA works on two strips of 128 rows with their scores S (128 fp32 columns)
-// and outputs O (D columns) in TMEM; keys come in blocks of 128.
+// A CTA works on two strips of 128 rows with their scores S (BN fp32 columns)
+// and outputs O (D columns) in TMEM; keys come in blocks of BN.
 //   warp 0       TMA of key and value blocks, two rings of stages
 //   warp 1       TMEM and the single MMA thread: S = Q K^T, then O += P V with
 //                P read from TMEM and V as it lies (its rows are the
@@ -38,13 +38,20 @@
 
 namespace dsv4cu {
 
-constexpr int SU_BN = 128;                // keys per block
 constexpr int SU_THREADS = 384;
-constexpr int SU_SUB = 128 * 128;         // bytes of a 128-row x 64-column operand tile
+// Keys per block, CTAs per SM and registers a thread (copy and product warps,
+// softmax warps). Head dim 128 takes the SM's whole TMEM and its registers for
+// 128-key blocks. Head dim 64 has half the products per score, so its softmax
+// and the fixed parts of a CTA weigh more: 64-key blocks fit twice, and one
+// CTA's set-up and output run beside the other's blocks.
+template <int D>
+struct SuShape {
+    static constexpr int BN = D, CTAS = D == 64 ? 2 : 1, FEW = D == 64 ? 48 : 72, MANY = D == 64 ? 96 : 216;
+};
+constexpr int SU_SUB = 128 * 128;         // bytes of 128 rows x 64 columns of the queries
 constexpr int SU_MAX_STAGES = 4;
-constexpr int SU_REGS_FEW = 72, SU_REGS_MANY = 216;   // per thread: copy and product warps, softmax warps
 constexpr float SU_LAZY = 8.0f;           // log2 units the running maximum may fall behind
-enum { SUE_KEMPTY = 81, SUE_VEMPTY, SUE_KFULL, SUE_VFULL, SUE_S, SUE_P, SUE_O, SUE_Q, SUE_DRAIN };
+enum { SUE_KEMPTY = 81, SUE_VEMPTY, SUE_KFULL, SUE_VFULL, SUE_S, SUE_P, SUE_O, SUE_Q, SUE_DRAIN, SUE_ALIGN };
 
 // Instruction descriptor of kind::f16: fp32 accumulator, both operands of one
 // 16-bit type (0 f16, 1 bf16), N >> 3 in bits 17-22, M >> 4 in bits 24-28; bit
@@ -54,13 +61,13 @@ __host__ __device__ constexpr uint32_t su_idesc(bool f16, int N, bool bt)
     return (1u << 4) | ((f16 ? 0u : 1u) << 7) | ((f16 ? 0u : 1u) << 10) | ((bt ? 1u : 0u) << 16) |
            ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-// The value tile [128 keys][64 columns] x D / 64 read with keys as the
-// contraction: 8-key groups 1024 bytes apart (stride byte offset), 64-column
-// groups one operand tile apart (leading byte offset).
-DSV4CU_DEV uint64_t su_desc_v(const void *p)
+// The value tile [keys][64 columns] x D / 64 read with keys as the contraction:
+// 8-key groups 1024 bytes apart (stride byte offset), 64-column groups `sub`
+// bytes apart (leading byte offset).
+DSV4CU_DEV uint64_t su_desc_v(const void *p, uint32_t sub)
 {
     const uint64_t a = umma::saddr(p);
-    return ((a >> 4) & 0x3FFFull) | ((uint64_t)(SU_SUB >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+    return ((a >> 4) & 0x3FFFull) | ((uint64_t)(sub >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
            (2ull << 61);
 }
 DSV4CU_DEV void su_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
@@ -193,23 +200,42 @@ DSV4CU_DEV uint32_t su_range(int lo, int hi, int word)
     return l > h ? 0u : (0xFFFFFFFFu << l) & (0xFFFFFFFFu >> (31 - h));
 }
 
+// What a CTA shares besides the operand tiles; it lies behind them, so that
+// three stages of 128-key blocks and a strip's queries fit.
+struct SuShared {
+    uint64_t kfull[SU_MAX_STAGES], kempty[SU_MAX_STAGES], vfull[SU_MAX_STAGES], vempty[SU_MAX_STAGES];
+    uint64_t sfull[2], pfull[2], ofull[2], qfull, drain;
+    SaTile t;                                            // for what is seldom looked at
+    uint32_t anc[SA_MAX_NODES][4];                       // tree: ancestors-or-self
+    uint32_t tmem;
+    int odd[2];
+    int16_t par[SA_MAX_NODES];
+    uint8_t depth[SA_MAX_NODES];
+};
+
 template <int D, bool F16, bool TREE>
-__global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_constant__ CUtensorMap mk,
+__global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kernel(const __grid_constant__ CUtensorMap mk,
                                                                    const __grid_constant__ CUtensorMap mv,
                                                                    const __grid_constant__ CUtensorMap mkc,
                                                                    const __grid_constant__ CUtensorMap mvc,
                                                                    const __grid_constant__ SaArgs a)
 {
-    constexpr int DC = D / 64, KVB = DC * SU_SUB;        // operand tiles and bytes of a block
-    extern __shared__ uint8_t su_raw[];
-    __shared__ __align__(8) uint64_t kfull[SU_MAX_STAGES], kempty[SU_MAX_STAGES], vfull[SU_MAX_STAGES],
-        vempty[SU_MAX_STAGES], sfull[2], pfull[2], ofull[2], qfull, drain;
-    __shared__ uint32_t tmem_holder;
-    __shared__ int s_par[TREE ? SA_MAX_NODES : 1], s_depth[TREE ? SA_MAX_NODES : 1];
-    __shared__ uint32_t s_anc[TREE ? SA_MAX_NODES : 1][4];
-    __shared__ int s_odd[2];
-    __shared__ SaTile s_t;                               // for what is seldom looked at
-    uint8_t *smem = (uint8_t *)(((uintptr_t)su_raw + 1023) & ~(uintptr_t)1023);
+    constexpr int BN = SuShape<D>::BN, DC = D / 64;      // keys of a block, 64-column tiles of a row
+    constexpr int KSUB = BN * 128, QB = DC * SU_SUB, KVB = DC * KSUB;   // bytes: block's tile, strip's queries, block
+    constexpr int TM_COLS = 2 * BN + 2 * D;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t *qs = smem, *ks = qs + (a.two ? 2 : 1) * QB, *vs = ks + a.nst * KVB;
+    SuShared &sh = *reinterpret_cast<SuShared *>(vs + a.nst * KVB);
+    uint64_t *kfull = sh.kfull, *kempty = sh.kempty, *vfull = sh.vfull, *vempty = sh.vempty, *sfull = sh.sfull,
+             *pfull = sh.pfull, *ofull = sh.ofull;
+    uint64_t &qfull = sh.qfull, &drain = sh.drain;
+    uint8_t *s_depth = sh.depth;
+    uint32_t (*s_anc)[4] = sh.anc;
+    int *s_odd = sh.odd;
+    if (umma::saddr(smem) & 1023u) {                     // the swizzle's period; never so without static shared memory
+        if (threadIdx.x == 0) atomicCAS(a.status, 0, SUE_ALIGN);
+        return;
+    }
     const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
     const int rows_cta = a.two ? 256 : 128;
 
@@ -221,7 +247,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
     t.kvh = blockIdx.y;
     if constexpr (TREE) {
         const int b = blockIdx.z;
-        const SaSpan sp = sa_span(a, b, SU_BN);
+        const SaSpan sp = sa_span(a, b, BN);
         t.split = blockIdx.x / a.row_tiles;
         t.begin = sp.begin;
         t.len = sp.len;
@@ -253,11 +279,11 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
     auto strip_first = [&](int s) {
         if constexpr (TREE) return t.blk0 + (alt ? s : 0);
         const int tok = (t.r0 + (alt ? 0 : 128 * s)) / a.G, lo = a.window > tok ? 0 : tok - a.window + 1;
-        return lo / SU_BN + (alt ? s : 0);
+        return lo / BN + (alt ? s : 0);
     };
     auto strip_end = [&](int s) {
         if constexpr (TREE) return t.blk1;
-        return (alt || s ? tok_end : (t.r0 + 127) / a.G) / SU_BN + 1;
+        return (alt || s ? tok_end : (t.r0 + 127) / a.G) / BN + 1;
     };
     const int f0 = strip_first(0), f1 = strip_first(1), e0 = strip_end(0), e1 = strip_end(1), step = alt ? 2 : 1;
     if constexpr (!TREE) {
@@ -287,9 +313,8 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
             }
         }
     }
-    uint8_t *qs = smem, *ks = qs + (a.two ? 2 : 1) * KVB, *vs = ks + a.nst * KVB;
     if (threadIdx.x == 0) {
-        s_t = t;
+        sh.t = t;
         for (int s = 0; s < SU_MAX_STAGES; s++) {
             mbar_init(&kfull[s], 1);
             mbar_init(&kempty[s], 1);
@@ -307,18 +332,18 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
         fence_mbar_init();
     }
     if (warp == 1) {
-        umma::tmem_alloc(&tmem_holder, 512);
+        umma::tmem_alloc(&sh.tmem, TM_COLS);
         umma::tmem_relinquish();
     }
     int lost = 0;                                        // a page of these blocks is not in the pool
     if constexpr (TREE) {
-        const int k_lo = t.key0 + t.blk0 * SU_BN, k_hi = min(t.kend, t.key0 + min(t.blk1, t.nblk_c) * SU_BN);
+        const int k_lo = t.key0 + t.blk0 * BN, k_hi = min(t.kend, t.key0 + min(t.blk1, t.nblk_c) * BN);
         if (k_lo < k_hi)
             for (int pg = k_lo / a.page_size + threadIdx.x; pg <= (k_hi - 1) / a.page_size; pg += SU_THREADS) {
                 const int id = __ldg(t.table + pg);
                 lost |= id < 0 || id >= a.n_pages;
             }
-        for (int i = threadIdx.x; i < t.len; i += SU_THREADS) s_par[i] = __ldg(a.parent + t.begin + i);
+        for (int i = threadIdx.x; i < t.len; i += SU_THREADS) sh.par[i] = (int16_t)max(-1, min(__ldg(a.parent + t.begin + i), SA_MAX_NODES));
     }
     umma::fence_before();
     lost = __syncthreads_or(lost);
@@ -331,24 +356,24 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
 #pragma unroll
                 for (int w = 0; w < 4; w++) set[w] |= (x >> 5) == w ? 1u << (x & 31) : 0u;
                 d++;
-                const int p = s_par[x];
+                const int p = sh.par[x];
                 if (p < 0 || p >= x) break;
                 x = p;
             }
 #pragma unroll
             for (int w = 0; w < 4; w++) s_anc[i][w] = set[w];
-            s_depth[i] = d;
+            s_depth[i] = (uint8_t)d;
         }
         __syncthreads();
     }
-    const uint32_t tmem = tmem_holder;
-    const uint32_t tm_s = tmem, tm_o = tmem + 256;       // strip s: S at + 128 s, O at + 128 s
+    const uint32_t tmem = sh.tmem;
+    const uint32_t tm_s = tmem, tm_o = tmem + 2 * BN;    // strip s: S at + BN s, O at + D s
 
     if (warp < 4) {
-        su_regs_dec<SU_REGS_FEW>();
+        su_regs_dec<SuShape<D>::FEW>();
         if (warp == 0) {
             // ------------------------------------------------ copies
-            const int boxes = TREE ? SU_BN >> a.box_log2 : 1;
+            const int boxes = TREE ? BN >> a.box_log2 : 1;
             bool ok = true;
             int n = 0;
             for (int b = c0; b < c1 && ok; b++, n++) {
@@ -357,7 +382,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                 int row = 0;
                 bool mine = lane == 0;
                 if (cached) {
-                    const int key = t.key0 + b * SU_BN + (lane << a.box_log2);
+                    const int key = t.key0 + b * BN + (lane << a.box_log2);
                     mine = lane < boxes && key < t.kend;
                     if (mine) {
                         const int pg = key >> a.page_log2, id = __ldg(t.table + pg);
@@ -365,7 +390,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                         row = id * a.page_size + (key - (pg << a.page_log2));
                     }
                 } else {
-                    row = t.begin + (b - t.nblk_c) * SU_BN;
+                    row = t.begin + (b - t.nblk_c) * BN;
                 }
                 const unsigned go = __ballot_sync(0xFFFFFFFFu, mine);
                 const uint32_t off = cached ? (uint32_t)lane << (a.box_log2 + 7) : 0u;   // this box's first row
@@ -382,7 +407,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                     const CUtensorMap *map = cached ? (kv ? &mvc : &mkc) : (kv ? &mv : &mk);
                     if (mine)
 #pragma unroll
-                        for (int c = 0; c < DC; c++) su_tma(dst + c * SU_SUB, map, 64 * c, t.kvh, row, full);
+                        for (int c = 0; c < DC; c++) su_tma(dst + c * KSUB, map, 64 * c, t.kvh, row, full);
                 }
             }
             // every issued copy lands before the CTA can exit
@@ -397,7 +422,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
             // the instructions take comes from warp-uniform values (broadcast
             // once), so descriptors stay in uniform registers. Issued by a lone
             // lane, moving them there took longer than the products.
-            constexpr uint32_t id_s = su_idesc(F16, SU_BN, false), id_o = su_idesc(F16, D, true);
+            constexpr uint32_t id_s = su_idesc(F16, BN, false), id_o = su_idesc(F16, D, true);
             auto same = [](int x) { return __shfl_sync(0xFFFFFFFFu, x, 0); };
             const bool one = su_elect();
             const int u0 = same(c0), u1 = same(c1), g0 = same(f0), g1 = same(f1), h0 = same(e0), h1 = same(e1);
@@ -407,7 +432,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
             const uint32_t ts = (uint32_t)same((int)tm_s), to = (uint32_t)same((int)tm_o);
             // operand descriptors: the address field counts 16 bytes, and shared
             // memory ends before it overflows
-            const uint64_t dq = umma::desc_sw128(qs), dk = umma::desc_sw128(ks), dv = su_desc_v(vs);
+            const uint64_t dq = umma::desc_sw128(qs), dk = umma::desc_sw128(ks), dv = su_desc_v(vs, KSUB);
             uint32_t once = 0;                           // blocks that one of their two strips has scored
             bool ok = su_wait(&qfull, 0, a.status, SUE_Q);
             umma::fence_after();
@@ -417,7 +442,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                 ok = ok && su_wait(&kfull[st], use & 1, a.status, SUE_KFULL);
                 if (!ok) return;
                 umma::fence_after();
-                const uint64_t q = dq + (uint32_t)((ualt ? 0 : s) * (KVB >> 4)), k = dk + (uint32_t)(st * (KVB >> 4));
+                const uint64_t q = dq + (uint32_t)((ualt ? 0 : s) * (QB >> 4)), k = dk + (uint32_t)(st * (KVB >> 4));
                 const uint32_t bit = 1u << (b & 31);
                 const bool both = !ualt && b >= g1 && b < h0;    // two strips read this block
                 const bool last = !both || (once & bit);
@@ -425,8 +450,8 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                 if (one) {
 #pragma unroll
                     for (int kk = 0; kk < D / 16; kk++) {
-                        const int at = ((kk >> 2) * SU_SUB + 32 * (kk & 3)) >> 4;
-                        su_mma(ts + 128 * s, q + at, k + at, id_s, kk > 0);
+                        su_mma(ts + BN * s, q + (((kk >> 2) * SU_SUB + 32 * (kk & 3)) >> 4),
+                               k + (((kk >> 2) * KSUB + 32 * (kk & 3)) >> 4), id_s, kk > 0);
                     }
                     umma::commit(&sfull[s]);
                     if (last) umma::commit(&kempty[st]);
@@ -451,8 +476,8 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                     const bool last = s == 1 || ualt || b < g1;  // strip 1 comes second
                     if (one) {
 #pragma unroll
-                        for (int kk = 0; kk < SU_BN / 16; kk++)
-                            su_mma_ta(to + 128 * s, ts + 128 * s + 8 * kk, v + (2048 >> 4) * kk, id_o, kk > 0 ? 1u : more);
+                        for (int kk = 0; kk < BN / 16; kk++)
+                            su_mma_ta(to + D * s, ts + BN * s + 8 * kk, v + (2048 >> 4) * kk, id_o, kk > 0 ? 1u : more);
                         if (last) umma::commit(&vempty[st]);
                     }
                     __syncwarp();
@@ -473,12 +498,12 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
             __syncwarp();
         }
     } else {
-        su_regs_inc<SU_REGS_MANY>();
+        su_regs_inc<SuShape<D>::MANY>();
         // ------------------------------------------------ softmax
         const int s = (warp - 4) >> 2, i = (threadIdx.x - 128) & 127;    // strip; row, and key in prepared values
         const int row0 = alt ? 0 : 128 * s, rows = min(128, t.rows - row0);
         {
-            uint8_t *q = qs + (alt ? 0 : s) * KVB;
+            uint8_t *q = qs + (alt ? 0 : s) * QB;
 #pragma unroll
             for (int e = 0; e < QN; e++) {
                 const int x = q_i + e * q_n, r = x / (D / 8), ch = x - r * (D / 8);
@@ -494,7 +519,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
         const int tok_lo = (t.r0 + row0) / a.G, tok_hi = (t.r0 + row0 + rows - 1) / a.G;
         const int depth = TREE ? s_depth[tok] : 0;
         const uint32_t quarter = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t sp_s = tm_s + 128 * s + quarter, sp_o = tm_o + 128 * s + quarter;
+        const uint32_t sp_s = tm_s + BN * s + quarter, sp_o = tm_o + D * s + quarter;
         float m = -INFINITY, l = 0.0f;
         uint32_t turn = 0;
         bool ok = true;
@@ -502,15 +527,15 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
         int full_lo, full_hi;
         if constexpr (TREE) {
             const int back = t.ctx + t.len - a.window;   // no key below this is in every row's window
-            full_lo = back <= t.key0 ? 0 : (back - t.key0 + SU_BN - 1) / SU_BN;
-            full_hi = (t.kend - t.key0) / SU_BN;         // at least 0 where there are cached blocks
+            full_lo = back <= t.key0 ? 0 : (back - t.key0 + BN - 1) / BN;
+            full_hi = (t.kend - t.key0) / BN;         // at least 0 where there are cached blocks
         } else {
             const int back = tok_hi - a.window + 1;
-            full_lo = back <= 0 ? 0 : (back + SU_BN - 1) / SU_BN;
-            full_hi = (tok_lo + 1) / SU_BN;
+            full_lo = back <= 0 ? 0 : (back + BN - 1) / BN;
+            full_hi = (tok_lo + 1) / BN;
         }
         auto is_full = [full_lo, full_hi](int b) { return b >= full_lo && b < full_hi; };
-        const SaTile *tp = &s_t;
+        const SaTile *tp = &sh.t;
         auto in_pool = [&](int key) {
             if (key >= tp->kend) return false;
             const int id = __ldg(tp->table + (key >> a.page_log2));
@@ -519,14 +544,15 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
         for (int b = first; b < end; b += step, turn++) {
             // ---- the mask
             const bool masked = !is_full(b) || (TREE && lost);
-            uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+            constexpr int W = BN / 32;                   // mask words of a block
+            uint32_t vis[W];
             ok = __all_sync(0xFFFFFFFFu, su_wait(&sfull[s], turn & 1, a.status, SUE_S));
             if (!ok) break;
             const bool cached = TREE && b < tp->nblk_c;
-            const int base = (TREE ? (cached ? tp->key0 + b * SU_BN : (b - tp->nblk_c) * SU_BN) : b * SU_BN);
+            const int base = (TREE ? (cached ? tp->key0 + b * BN : (b - tp->nblk_c) * BN) : b * BN);
             // keys that are not there: behind the sequence, the nodes or the
             // cache, or on a missing page
-            if (masked && (cached ? lost || base + SU_BN > tp->kend : base + SU_BN > tp->len)) {
+            if (masked && (cached ? lost || base + BN > tp->kend : base + BN > tp->len)) {
                 // values of absent keys become zeros (what the copies left, or
                 // brought from the next sequence, may be no number). Behind
                 // this block's scores lie the products of every block before
@@ -535,12 +561,12 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                 const int n = b - c0, st = n % a.nst;
                 ok = __all_sync(0xFFFFFFFFu, su_wait(&vfull[st], (n / a.nst) & 1, a.status, SUE_VFULL));
                 if (!ok) break;
-                if (!(cached ? in_pool(base + i) : base + i < tp->len)) {
+                if (i < BN && !(cached ? in_pool(base + i) : base + i < tp->len)) {
                     uint8_t *v = vs + st * KVB + i * 128;
 #pragma unroll
                     for (int c = 0; c < DC; c++)
 #pragma unroll
-                        for (int x = 0; x < 8; x++) *reinterpret_cast<uint4 *>(v + c * SU_SUB + 16 * x) = make_uint4(0, 0, 0, 0);
+                        for (int x = 0; x < 8; x++) *reinterpret_cast<uint4 *>(v + c * KSUB + 16 * x) = make_uint4(0, 0, 0, 0);
                 }
                 su_fence_async();
             }
@@ -548,38 +574,41 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                 if (cached) {
                     const int pos = tp->ctx + depth, lo = a.window > pos ? 0 : pos - a.window + 1 - base;
 #pragma unroll
-                    for (int w = 0; w < 4; w++) {
+                    for (int w = 0; w < W; w++) {
                         vis[w] = su_range(lo, tp->kend - 1 - base, w);
                         if (lost) vis[w] &= __ballot_sync(0xFFFFFFFFu, in_pool(base + 32 * w + lane));
                     }
                 } else if (TREE) {
 #pragma unroll
-                    for (int w = 0; w < 4; w++) vis[w] = s_anc[tok][w];
+                    for (int w = 0; w < W; w++) vis[w] = s_anc[tok][base / 32 + w];
                     if (depth >= a.window)
-                        for (int x = 0; x < tp->len; x++)
-                            if (depth - s_depth[x] >= a.window) vis[x >> 5] &= ~(1u << (x & 31));
+                        for (int x = base; x < min(tp->len, base + BN); x++)
+                            if (depth - s_depth[x] >= a.window) {
+#pragma unroll
+                                for (int w = 0; w < W; w++) vis[w] &= (x - base) >> 5 == w ? ~(1u << (x & 31)) : ~0u;
+                            }
                 } else {
                     const int lo = a.window > tok ? 0 : tok - a.window + 1 - base;
 #pragma unroll
-                    for (int w = 0; w < 4; w++) vis[w] = su_range(lo, tok - base, w);
+                    for (int w = 0; w < W; w++) vis[w] = su_range(lo, tok - base, w);
                 }
             }
             if (live) {
                 umma::fence_after();
-                uint32_t x[128];
+                uint32_t x[BN];
 #pragma unroll
-                for (int c = 0; c < 4; c++) su_ld32(sp_s + 32 * c, x + 32 * c);
+                for (int c = 0; c < BN / 32; c++) su_ld32(sp_s + 32 * c, x + 32 * c);
                 su_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 4; c++) su_loaded32(x + 32 * c);
+                for (int c = 0; c < BN / 32; c++) su_loaded32(x + 32 * c);
                 if (masked) {
 #pragma unroll
-                    for (int k = 0; k < 128; k++)
+                    for (int k = 0; k < BN; k++)
                         if (!((vis[k >> 5] >> (k & 31)) & 1u)) x[k] = 0xFF800000u;
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < 128; k += 8)
+                for (int k = 0; k < BN; k += 8)
 #pragma unroll
                     for (int e = 0; e < 4; e++)
                         top[e] = su_max3(top[e], __uint_as_float(x[k + 2 * e]), __uint_as_float(x[k + 2 * e + 1]));
@@ -605,7 +634,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                 const uint64_t scale2 = su_f2(a.scale2, a.scale2), shift2 = su_f2(-use, -use);
                 uint64_t sum[2] = {su_f2(l, 0.0f), su_f2(0.0f, 0.0f)};
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < BN / 32; c++) {
                     uint32_t w[16];
 #pragma unroll
                     for (int k = 0; k < 16; k++) {
@@ -637,26 +666,26 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
             const SaTile &t = *tp;
             const bool vv = values && a.v != nullptr;
             if (TREE && blk < t.nblk_c) {
-                const int key = t.key0 + blk * SU_BN + j;
+                const int key = t.key0 + blk * BN + j;
                 return key < t.kend ? sa_cached(a, t, vv ? a.vc : a.kc, key, D) : nullptr;
             }
-            const int key = (TREE ? blk - t.nblk_c : blk) * SU_BN + j;
+            const int key = (TREE ? blk - t.nblk_c : blk) * BN + j;
             if (key >= t.len) return nullptr;
             return reinterpret_cast<const uint16_t *>(vv ? a.v : a.k) + (size_t)(t.begin + key) * (vv ? a.ldv : a.ldk) +
                    (size_t)t.kvh * D;
         };
-        auto sees = [tp, row_of, ap = &a0, dp = &s_depth[0], an = &s_anc[0]](int tok, int blk, int j) -> bool {
+        auto sees = [tp, row_of, ap = &a0, dp = s_depth, an = s_anc](int tok, int blk, int j) -> bool {
             const SaArgs &a = *ap;
             const SaTile &t = *tp;
             if constexpr (TREE) {
                 if (blk < t.nblk_c) {
-                    const int key = t.key0 + blk * SU_BN + j;
+                    const int key = t.key0 + blk * BN + j;
                     return key < t.kend && t.ctx - key + dp[tok] < a.window && row_of(blk, j, false) != nullptr;
                 }
-                const int x = (blk - t.nblk_c) * SU_BN + j;
+                const int x = (blk - t.nblk_c) * BN + j;
                 return x < t.len && (an[tok][x >> 5] >> (x & 31) & 1) && dp[tok] - dp[x] < a.window;
             } else {
-                const int key = blk * SU_BN + j;
+                const int key = blk * BN + j;
                 return key <= tok && tok - key < a.window;
             }
         };
@@ -667,11 +696,13 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
         // strip's warps, which get the other strip's share of it through xch.
         constexpr int PN = D == 128 ? 16 : 8;            // 16-byte pieces of a row per pass
         constexpr int XN = D / 8;                        // 16-byte pieces of half a row of floats
-        uint8_t *out = alt ? ks + 65536 + (warp - 4) * (PN * 512) : qs + s * KVB + (warp & 3) * (PN * 512);
+        constexpr int XH = 128 * XN * 16;                // bytes of one strip's share
+        static_assert(2 * XH + 8 * PN * 512 <= 2 * 2 * KVB || 2 * XH + 8 * PN * 512 <= 2 * SU_MAX_STAGES * KVB, "stages");
+        uint8_t *out = alt ? ks + 2 * XH + (warp - 4) * (PN * 512) : qs + s * QB + (warp & 3) * (PN * 512);
         float f_own = 1.0f;
         const int col0 = alt ? s * (D / 2) : 0, ncol = alt ? D / 2 : D;
         if (alt) {
-            float2 *ml = reinterpret_cast<float2 *>(ks + 65536);
+            float2 *ml = reinterpret_cast<float2 *>(ks + 2 * XH);
             su_bar<256>(1);                              // both strips' products are complete: the stages are free
             ml[128 * s + i] = make_float2(m, l);
             su_bar<256>(1);
@@ -682,7 +713,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
             l = l * f_own + other.y * sa_exp2(other.x - use);
             m = top;
             if (live) {
-                uint8_t *x = ks + (s ^ 1) * 32768 + i * (XN * 16);
+                uint8_t *x = ks + (s ^ 1) * XH + i * (XN * 16);
                 for (int c = 0; c < D / 2; c += 16) {
                     uint32_t o[16];
                     if (any) su_ld16(sp_o + (s ^ 1) * (D / 2) + c, o);
@@ -710,7 +741,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
             char *dst = part ? reinterpret_cast<char *>(a.po + id * D + col0)
                              : reinterpret_cast<char *>(reinterpret_cast<uint16_t *>(a.o) + (size_t)(t.begin + tok) * a.ldo +
                                                         (size_t)head * D + col0);
-            const uint8_t *x = ks + s * 32768 + i * (XN * 16);
+            const uint8_t *x = ks + s * XH + i * (XN * 16);
             const int mine = min(32, rows - 32 * (warp & 3));    // rows of this warp
             int piece = 0;                               // of the pass
             for (int c = 0; c < ncol; c += 16) {         // a loop: its code is cold at every launch
@@ -779,9 +810,9 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
                 ts.blk1 = end;
             }
             const int threads = alt ? 256 : 128, thread = alt ? threadIdx.x - 128 : i;
-            if (sa_suspect<D, F16, false>(ts, SU_BN, thread, threads, is_full, row_of)) s_odd[who] = 2;
+            if (sa_suspect<D, F16, false>(ts, BN, thread, threads, is_full, row_of)) s_odd[who] = 2;
             alt ? su_bar<256>(1) : su_bar<128>(2 + s);
-            if (s_odd[who] == 2) serve_slow_rows<D, F16, false>(a, ts, SU_BN, thread >> 5, threads >> 5, sees, row_of);
+            if (s_odd[who] == 2) serve_slow_rows<D, F16, false>(a, ts, BN, thread >> 5, threads >> 5, sees, row_of);
         }
         if (TREE && t.parts > 1) {
             // the tile's last split to finish joins them all
@@ -804,7 +835,7 @@ __global__ void __launch_bounds__(SU_THREADS, 1) serve_umma_kernel(const __grid_
     __syncthreads();
     if (warp == 1) {
         umma::fence_after();
-        umma::tmem_dealloc(tmem, 512);
+        umma::tmem_dealloc(tmem, TM_COLS);
     }
 }
 
@@ -819,16 +850,18 @@ static inline int su_map(CUtensorMap *map, const void *base, int D, int heads, i
 template <int D, bool F16>
 int serve_umma_launch(SaArgs a, bool tree, cudaStream_t st)
 {
-    constexpr int KVB = D / 64 * SU_SUB;
+    using S = SuShape<D>;
+    constexpr int QB = D / 64 * SU_SUB, KVB = D / 64 * S::BN * 128;
     int r;
     CUtensorMap mk, mv, mkc, mvc;
-    if ((r = su_map(&mk, a.k, D, a.hkv, a.nt, a.ldk, SU_BN, F16))) return r;
-    if ((r = su_map(&mv, a.v ? a.v : a.k, D, a.hkv, a.nt, a.v ? a.ldv : a.ldk, SU_BN, F16))) return r;
+    if ((r = su_map(&mk, a.k, D, a.hkv, a.nt, a.ldk, S::BN, F16))) return r;
+    if ((r = su_map(&mv, a.v ? a.v : a.k, D, a.hkv, a.nt, a.v ? a.ldv : a.ldk, S::BN, F16))) return r;
     mkc = mk;
     mvc = mv;
     dim3 grid;
     if (tree) {
-        a.box_log2 = a.page_log2 < 7 ? a.page_log2 : 7;
+        const int bn_log2 = S::BN == 64 ? 6 : 7;
+        a.box_log2 = a.page_log2 < bn_log2 ? a.page_log2 : bn_log2;
         if (a.n_pages > 0) {
             const int64_t slots = (int64_t)a.n_pages * a.page_size;
             const long row = (long)a.hkv * D;
@@ -842,8 +875,12 @@ int serve_umma_launch(SaArgs a, bool tree, cudaStream_t st)
         if (tiles > INT_MAX) return dsv4cu_set_error(DSV4CU_ERR_ARG, "prompt_attn: %lld row tiles", (long long)tiles);
         grid = dim3((unsigned)tiles, a.hkv, 1);
     }
-    a.nst = min(SU_MAX_STAGES, (SA_SMEM_MAX - (a.two ? 2 : 1) * KVB) / (2 * KVB));
-    const size_t smem = (size_t)((a.two ? 2 : 1) + 2 * a.nst) * KVB + 1024;
+    // as many stages as fit: 227 KB for one CTA; half of the SM's 228 KB less
+    // the 1 KB that each CTA costs for two
+    constexpr int LIMIT = S::CTAS == 2 ? 113 * 1024 : 227 * 1024;
+    const int fixed = (a.two ? 2 : 1) * QB + (int)sizeof(SuShared);
+    a.nst = min(SU_MAX_STAGES, (LIMIT - fixed) / (2 * KVB));
+    const size_t smem = fixed + (size_t)2 * a.nst * KVB;
     auto kern = tree ? serve_umma_kernel<D, F16, true> : serve_umma_kernel<D, F16, false>;
     static SmemLimit lim[2];
     DSV4CU_CUDA_TRY(smem_limit(lim[tree], (const void *)kern, (int)smem));
@@ -854,7 +891,7 @@ int serve_umma_launch(SaArgs a, bool tree, cudaStream_t st)
         DSV4CU_CUDA_TRY(cudaFuncGetAttributes(&f, (const void *)kern));
         regs[tree] = f.numRegs;
     }
-    if (regs[tree] * SU_THREADS < SU_REGS_FEW * 128 + SU_REGS_MANY * 256)
+    if (regs[tree] * SU_THREADS < S::FEW * 128 + S::MANY * 256)
         return dsv4cu_set_error(DSV4CU_ERR_UNSUPPORTED, "serving attention: launched with %d registers a thread", regs[tree]);
     kern<<<grid, SU_THREADS, smem, st>>>(mk, mv, mkc, mvc, a);
     DSV4CU_LAUNCH_CHECK();
