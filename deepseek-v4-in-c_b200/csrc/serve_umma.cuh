@@ -200,8 +200,8 @@ DSV4CU_DEV uint32_t su_range(int lo, int hi, int word)
     return l > h ? 0u : (0xFFFFFFFFu << l) & (0xFFFFFFFFu >> (31 - h));
 }
 
-// What a CTA shares besides the operand tiles; it lies behind them, so that
-// three stages of 128-key blocks and a strip's queries fit.
+// What a CTA shares besides the operand tiles, in front of them. Three stages
+// of 128-key blocks and a strip's queries then fill the 227 KB exactly.
 struct SuShared {
     uint64_t kfull[SU_MAX_STAGES], kempty[SU_MAX_STAGES], vfull[SU_MAX_STAGES], vempty[SU_MAX_STAGES];
     uint64_t sfull[2], pfull[2], ofull[2], qfull, drain;
@@ -212,6 +212,8 @@ struct SuShared {
     int16_t par[SA_MAX_NODES];
     uint8_t depth[SA_MAX_NODES];
 };
+constexpr int SU_SHARED = 3072;
+static_assert(sizeof(SuShared) <= SU_SHARED, "the tiles start on the swizzle's period");
 
 template <int D, bool F16, bool TREE>
 __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kernel(const __grid_constant__ CUtensorMap mk,
@@ -224,8 +226,8 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
     constexpr int KSUB = BN * 128, QB = DC * SU_SUB, KVB = DC * KSUB;   // bytes: block's tile, strip's queries, block
     constexpr int TM_COLS = 2 * BN + 2 * D;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t *qs = smem, *ks = qs + (a.two ? 2 : 1) * QB, *vs = ks + a.nst * KVB;
-    SuShared &sh = *reinterpret_cast<SuShared *>(vs + a.nst * KVB);
+    SuShared &sh = *reinterpret_cast<SuShared *>(smem);
+    uint8_t *qs = smem + SU_SHARED, *ks = qs + (a.two ? 2 : 1) * QB, *vs = ks + a.nst * KVB;
     uint64_t *kfull = sh.kfull, *kempty = sh.kempty, *vfull = sh.vfull, *vempty = sh.vempty, *sfull = sh.sfull,
              *pfull = sh.pfull, *ofull = sh.ofull;
     uint64_t &qfull = sh.qfull, &drain = sh.drain;
@@ -878,7 +880,7 @@ int serve_umma_launch(SaArgs a, bool tree, cudaStream_t st)
     // as many stages as fit: 227 KB for one CTA; half of the SM's 228 KB less
     // the 1 KB that each CTA costs for two
     constexpr int LIMIT = S::CTAS == 2 ? 113 * 1024 : 227 * 1024;
-    const int fixed = (a.two ? 2 : 1) * QB + (int)sizeof(SuShared);
+    const int fixed = (a.two ? 2 : 1) * QB + SU_SHARED;
     a.nst = min(SU_MAX_STAGES, (LIMIT - fixed) / (2 * KVB));
     const size_t smem = fixed + (size_t)2 * a.nst * KVB;
     auto kern = tree ? serve_umma_kernel<D, F16, true> : serve_umma_kernel<D, F16, false>;
