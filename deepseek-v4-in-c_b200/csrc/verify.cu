@@ -22,8 +22,8 @@
 // no memory. What needs the whole row is a sum that each CTA takes over its
 // slice and stores into the others' shared memory (one cluster barrier per
 // sum; two sets of slots, so the next sum does not disturb readers). A row
-// comes from memory once; later sums and the rescan of the one warp's segment
-// that holds the token find it in L2.
+// comes from memory once; later sums and the rescan of the one segment that
+// holds the token find it in L2.
 #include <math.h>
 
 #include <cooperative_groups.h>
@@ -35,7 +35,7 @@ namespace cg = cooperative_groups;
 
 constexpr int VER_MAX_NODES = 128;
 constexpr int VER_THREADS = 256;
-constexpr int VER_BATCH = 16;         // loads a lane has in flight
+constexpr int VER_BATCH = 32;         // elements a lane has in flight, of one row or of both
 constexpr int VER_WARPS = VER_THREADS / 32;
 constexpr int VER_CL = 8;             // CTAs per request: the largest portable cluster
 enum { VER_BAD_TREE = 76 };           // more than VER_MAX_NODES nodes (dsv4cu_ctx_status)
@@ -153,7 +153,25 @@ DSV4CU_DEV double ver_segment(const Rest &r, int lo, int hi, int lane)
     bool plain = true;                           // no refused token lies in this segment
     if (!LESS)
         for (int i = 0; i < r.k; i++) plain = plain && (r.gone[i] < lo || r.gone[i] >= hi);
-    if (plain) {
+    if (plain && (((uintptr_t)(r.p + lo) | (LESS ? (uintptr_t)(r.q + lo) : 0)) & 15u) == 0) {
+        const float4 *p = reinterpret_cast<const float4 *>(r.p + lo) + lane;
+        const float4 *q = reinterpret_cast<const float4 *>(r.q + lo) + lane;
+        for (; x0 + 32 * B <= hi; x0 += 32 * B, p += 8 * B, q += 8 * B) {
+            float4 pv[B / 4], qv[B / 4];
+#pragma unroll
+            for (int j = 0; j < B / 4; j++) {
+                pv[j] = __ldg(p + 32 * j);
+                if (LESS) qv[j] = __ldg(q + 32 * j);
+            }
+#pragma unroll
+            for (int j = 0; j < B / 4; j++) {
+                s[0] += LESS ? ver_less(pv[j].x, qv[j].x, r.c) : (double)pv[j].x;
+                s[1] += LESS ? ver_less(pv[j].y, qv[j].y, r.c) : (double)pv[j].y;
+                s[0] += LESS ? ver_less(pv[j].z, qv[j].z, r.c) : (double)pv[j].z;
+                s[1] += LESS ? ver_less(pv[j].w, qv[j].w, r.c) : (double)pv[j].w;
+            }
+        }
+    } else if (plain) {
         const float *p = r.p + lo + lane, *q = r.q + lo + lane;
         for (; x0 + 32 * B <= hi; x0 += 32 * B, p += 32 * B, q += 32 * B) {
             float pv[B], qv[B];
@@ -331,21 +349,48 @@ __global__ void __cluster_dims__(VER_CL, 1, 1) __launch_bounds__(VER_THREADS, 4)
         wsel = wlast;
         wbefore = lbefore;
     }
-    if (warp != wsel) return;
-    double base = wbefore;
+    // that warp's segment once more, cut over all warps; the one that holds the
+    // threshold looks at its elements in order
+    const int slo = min(hi, lo + wsel * seg), shi = min(hi, slo + seg);
+    const int sub = ((seg + VER_WARPS - 1) / VER_WARPS + 31) & ~31;
+    const int blo = min(shi, slo + warp * sub), bhi = min(shi, blo + sub);
+    const double mine = r.q && r.k ? ver_segment<true>(r, blo, bhi, lane) : ver_segment<false>(r, blo, bhi, lane);
+    __syncthreads();                             // part is read
+    if (lane == 0) part[warp] = mine;
+    __syncthreads();
+    int sel = -1, last = -1;
+    double base = 0.0, lastbase = 0.0;
+    run = wbefore;
+    for (int w = 0; w < VER_WARPS && sel < 0; w++) {
+        if (part[w] > 0.0) {
+            last = w;
+            lastbase = run;
+        }
+        if (run + part[w] > want) {
+            sel = w;
+            base = run;
+        }
+        run += part[w];
+    }
+    if (sel < 0) {                               // rounding of the segment's sum: the last piece with mass
+        sel = last;
+        base = lastbase;
+    }
+    if (sel < 0) sel = 0;
+    if (warp != sel) return;
     int found = -1, lastpos = -1;
-    for (int x1 = wlo; x1 < whi && found < 0; x1 += 256) {
+    for (int x1 = blo; x1 < bhi && found < 0; x1 += 256) {
         float pw[8], qw[8];                      // eight steps' loads at once
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int x = x1 + 32 * j + lane;
-            pw[j] = x < whi ? __ldg(r.p + x) : 0.0f;
-            qw[j] = x < whi && r.q && r.k ? __ldg(r.q + x) : 0.0f;
+            pw[j] = x < bhi ? __ldg(r.p + x) : 0.0f;
+            qw[j] = x < bhi && r.q && r.k ? __ldg(r.q + x) : 0.0f;
         }
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int x0 = x1 + 32 * j;
-            if (x0 >= whi || found >= 0) break;
+            if (x0 >= bhi || found >= 0) break;
             const double v = ver_rest(r, pw[j], qw[j], x0 + lane);
             double c = v;
 #pragma unroll
@@ -360,7 +405,7 @@ __global__ void __cluster_dims__(VER_CL, 1, 1) __launch_bounds__(VER_THREADS, 4)
             base += __shfl_sync(0xFFFFFFFFu, c, 31);
         }
     }
-    if (found < 0) found = lastpos;              // rounding of the segment's sum: its last token with mass
+    if (found < 0) found = lastpos;              // the piece's last token with mass
     if (lane == 0) a.next[b] = found;
 }
 
