@@ -180,7 +180,7 @@ struct SaTile {
     int begin, len;       // token range of the request / sequence
     int r0, rows;         // first row of the tile, rows in it
     int kvh;
-    int ctx, kend, key0;  // tree: cached tokens, those that the table holds, first key of the first cached block
+    int ctx, kend, key0;  // tree: cached tokens, those that the table holds; first key of the first (cached) block
     int nblk_c, blk0, blk1;   // cached blocks; this CTA's range of blocks (cached first, then nodes)
     int split, parts;     // tree: which split of how many
     const int *table;
@@ -491,9 +491,9 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
     if (t.rows <= 0) return;
     const int t_lo = t.r0 / a.G, t_hi = (t.r0 + t.rows - 1) / a.G;
     if constexpr (!TREE) {
-        const int first = a.window > t_lo ? 0 : t_lo - a.window + 1;
-        t.blk0 = first / BN;
-        t.blk1 = t_hi / BN + 1;
+        t.key0 = a.window > t_lo ? 0 : t_lo - a.window + 1;   // blocks start at the first key of the window
+        t.blk0 = 0;
+        t.blk1 = (t_hi - t.key0) / BN + 1;
     }
     if constexpr (TREE) {
         // ancestors-or-self as bit sets, depths; a parent that does not come
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
             const int key = t.key0 + blk * BN + j;
             return key < t.kend ? sa_cached(a, t, vv ? a.vc : a.kc, key, D) : nullptr;
         }
-        const int key = (TREE ? blk - t.nblk_c : blk) * BN + j;
+        const int key = TREE ? (blk - t.nblk_c) * BN + j : t.key0 + blk * BN + j;
         if (key >= t.len) return nullptr;
         return reinterpret_cast<const uint16_t *>(vv ? a.v : a.k) + (size_t)(t.begin + key) * (vv ? a.ldv : a.ldk) +
                (size_t)t.kvh * D;
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
             const int x = (blk - t.nblk_c) * BN + j;
             return x < t.len && (s_anc[tok][x >> 6] >> (x & 63) & 1) && s_depth[tok] - s_depth[x] < a.window;
         } else {
-            const int key = blk * BN + j;
+            const int key = t.key0 + blk * BN + j;
             return key <= tok && tok - key < a.window;
         }
     };
@@ -567,17 +567,6 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
         }
         sa_commit();
     };
-    if (tid < 2) s_bad[tid] = -1;
-    if (tid < BM) {
-        s_m[tid] = -INFINITY;
-        s_l[tid] = 0.0f;
-    }
-    __syncthreads();
-    find_rows(t.blk0);
-    if (t.blk0 + 1 < t.blk1) find_rows(t.blk0 + 1);
-    __syncthreads();
-    issue(t.blk0);
-
     // ---- this warp's dims of the queries as mma fragments: rows g / g + 8 of
     // m tile mt, dims DW * warp + 16 kk + 2c.. / 2c + 8..
     uint32_t qa[2][KS][TERMS][4];
@@ -605,6 +594,17 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
                 }
         }
 
+    if (tid < 2) s_bad[tid] = -1;
+    if (tid < BM) {
+        s_m[tid] = -INFINITY;
+        s_l[tid] = 0.0f;
+    }
+    __syncthreads();
+    find_rows(t.blk0);
+    if (t.blk0 + 1 < t.blk1) find_rows(t.blk0 + 1);
+    __syncthreads();
+    issue(t.blk0);
+
     const int arow = (lane & 7) + 8 * ((lane >> 3) & 1), acol = 8 * (lane >> 4);
     const int brow = (lane & 7) + 8 * (lane >> 4), bcol = 8 * ((lane >> 3) & 1);
     const int d0 = DW * warp;
@@ -620,7 +620,8 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
             const int e = t.key0 + (blk + 1) * BN;
             return blk < t.nblk_c && e <= t.kend && t.ctx + t.len - (e - BN) <= ap->window;
         } else {
-            return (blk + 1) * BN - 1 <= t_lo && t_hi - blk * BN < ap->window;
+            const int base = t.key0 + blk * BN;
+            return base + BN - 1 <= t_lo && t_hi - base < ap->window;
         }
     };
 

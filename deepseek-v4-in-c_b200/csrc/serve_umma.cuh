@@ -277,15 +277,19 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
     if (t.rows <= 0) return;
     const int tok_end = (t.r0 + t.rows - 1) / a.G;       // the CTA's last token
     const bool alt = t.rows <= 128;                      // one strip: even and odd blocks
+    if constexpr (!TREE) {                               // blocks start at the first key of the window
+        const int tok = t.r0 / a.G;
+        t.key0 = a.window > tok ? 0 : tok - a.window + 1;
+    }
     // strip s: rows [row0, row0 + n), key blocks from `first` to `end` by `step`
     auto strip_first = [&](int s) {
         if constexpr (TREE) return t.blk0 + (alt ? s : 0);
         const int tok = (t.r0 + (alt ? 0 : 128 * s)) / a.G, lo = a.window > tok ? 0 : tok - a.window + 1;
-        return lo / BN + (alt ? s : 0);
+        return (lo - t.key0) / BN + (alt ? s : 0);
     };
     auto strip_end = [&](int s) {
         if constexpr (TREE) return t.blk1;
-        return (alt || s ? tok_end : (t.r0 + 127) / a.G) / BN + 1;
+        return ((alt || s ? tok_end : (t.r0 + 127) / a.G) - t.key0) / BN + 1;
     };
     const int f0 = strip_first(0), f1 = strip_first(1), e0 = strip_end(0), e1 = strip_end(1), step = alt ? 2 : 1;
     if constexpr (!TREE) {
@@ -392,7 +396,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
                         row = id * a.page_size + (key - (pg << a.page_log2));
                     }
                 } else {
-                    row = t.begin + (b - t.nblk_c) * BN;
+                    row = t.begin + (TREE ? (b - t.nblk_c) * BN : t.key0 + b * BN);
                 }
                 const unsigned go = __ballot_sync(0xFFFFFFFFu, mine);
                 const uint32_t off = cached ? (uint32_t)lane << (a.box_log2 + 7) : 0u;   // this box's first row
@@ -532,9 +536,9 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
             full_lo = back <= t.key0 ? 0 : (back - t.key0 + BN - 1) / BN;
             full_hi = (t.kend - t.key0) / BN;         // at least 0 where there are cached blocks
         } else {
-            const int back = tok_hi - a.window + 1;
+            const int back = tok_hi - a.window + 1 - t.key0;
             full_lo = back <= 0 ? 0 : (back + BN - 1) / BN;
-            full_hi = (tok_lo + 1) / BN;
+            full_hi = (tok_lo + 1 - t.key0) / BN;
         }
         auto is_full = [full_lo, full_hi](int b) { return b >= full_lo && b < full_hi; };
         const SaTile *tp = &sh.t;
@@ -551,7 +555,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
             ok = __all_sync(0xFFFFFFFFu, su_wait(&sfull[s], turn & 1, a.status, SUE_S));
             if (!ok) break;
             const bool cached = TREE && b < tp->nblk_c;
-            const int base = (TREE ? (cached ? tp->key0 + b * BN : (b - tp->nblk_c) * BN) : b * BN);
+            const int base = TREE && !cached ? (b - tp->nblk_c) * BN : tp->key0 + b * BN;
             // keys that are not there: behind the sequence, the nodes or the
             // cache, or on a missing page
             if (masked && (cached ? lost || base + BN > tp->kend : base + BN > tp->len)) {
@@ -671,7 +675,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
                 const int key = t.key0 + blk * BN + j;
                 return key < t.kend ? sa_cached(a, t, vv ? a.vc : a.kc, key, D) : nullptr;
             }
-            const int key = (TREE ? blk - t.nblk_c : blk) * BN + j;
+            const int key = TREE ? (blk - t.nblk_c) * BN + j : t.key0 + blk * BN + j;
             if (key >= t.len) return nullptr;
             return reinterpret_cast<const uint16_t *>(vv ? a.v : a.k) + (size_t)(t.begin + key) * (vv ? a.ldv : a.ldk) +
                    (size_t)t.kvh * D;
@@ -687,7 +691,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
                 const int x = (blk - t.nblk_c) * BN + j;
                 return x < t.len && (an[tok][x >> 5] >> (x & 31) & 1) && dp[tok] - dp[x] < a.window;
             } else {
-                const int key = blk * BN + j;
+                const int key = t.key0 + blk * BN + j;
                 return key <= tok && tok - key < a.window;
             }
         };
