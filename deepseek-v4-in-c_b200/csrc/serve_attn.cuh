@@ -8,8 +8,7 @@
 //
 // A tile is 32 rows of one key head: row r is (token r / G, head r % G) of the
 // G query heads that share it, so grouped heads read a key once. The keys come
-// in blocks of BN through cp.async into 16-byte-swizzled shared memory, two
-// stages where they fit. The NW warps of a CTA each own D / NW of the head's
+// in blocks of BN, a bulk copy per row, into two stages of shared memory. The NW warps of a CTA each own D / NW of the head's
 // dims for the whole pass - of the queries (mma fragments in registers), of
 // the scores' contraction, and of the output's columns - so a head dim of 512
 // needs no more than 255 registers a thread, and where the values are the key
@@ -32,19 +31,20 @@
 // output is not finite looks (sa_suspect) for a non-finite value behind a mask
 // - with three weight terms, whose last ones may be 0, also for a visible
 // infinity - and if there is one, serve_slow_rows computes the tile again from
-// visible keys only. Rows outside a sequence and pages outside the pool arrive
-// as zeros (cp.async with a source size of 0) and are masked.
+// visible keys only. Rows outside a sequence and pages outside the pool are
+// zeros in shared memory and are masked.
 #pragma once
 
 #include <limits.h>
 
 #include "serve.h"
+#include "tma_gemv.cuh"
 
 namespace dsv4cu {
 
 constexpr int SA_MAX_NODES = 128;
 constexpr float SA_LOG2E = 1.4426950408889634f;
-enum { SA_BAD_NODES = 75 };           // a tree with more nodes than max_nodes (dsv4cu_ctx_status)
+enum { SA_BAD_NODES = 75, SA_COPY = 77 };   // dsv4cu_ctx_status: more nodes than max_nodes, a copy that did not arrive
 
 struct SaArgs {
     const void *q, *k, *v;            // packed rows; v == NULL: the key rows are the values
@@ -93,14 +93,36 @@ DSV4CU_DEV SaSpan sa_span(const SaArgs &a, int b, int BN)
 }
 
 DSV4CU_DEV uint32_t sa_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-DSV4CU_DEV void sa_cp16(void *dst, const void *src, bool there)
+// One contiguous copy, counted in bytes on `bar`; addresses and size multiples
+// of 16.
+DSV4CU_DEV void sa_bulk(void *dst, const void *src, uint32_t bytes, uint64_t *bar)
 {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sa_smem(dst)), "l"(src), "r"(there ? 16 : 0)
-                 : "memory");
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(sa_smem(dst)), "l"(src), "r"(bytes), "r"(sa_smem(bar)) : "memory");
 }
-DSV4CU_DEV void sa_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-DSV4CU_DEV void sa_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+DSV4CU_DEV void sa_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Bounded wait that polls: no suspend hint and no look at the clock on the
+// way to a phase that completes in time.
+DSV4CU_DEV bool sa_poll(uint64_t *bar, uint32_t parity, int *err, int code)
+{
+    const uint32_t a = sa_smem(bar);
+    uint64_t t0 = 0;
+    for (uint32_t i = 1;; i++) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\t"
+                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                     "selp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(a), "r"(parity) : "memory");
+        if (ok) return true;
+        if ((i & 1023u) == 0u) {
+            const uint64_t now = globaltimer_ns();
+            if (t0 == 0) t0 = now;
+            else if (now - t0 > MBAR_TIMEOUT_NS) break;
+        }
+    }
+    atomicCAS(err, 0, code);
+    return false;
+}
 DSV4CU_DEV void sa_ldsm4(uint32_t (&r)[4], const void *p)
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -168,13 +190,6 @@ DSV4CU_DEV bool sa_nonfinite(uint32_t w)
     constexpr uint32_t E = F16 ? 0x7C00u : 0x7F80u;
     return (w & E) == E || (w & (E << 16)) == (E << 16);
 }
-// Element (row, col) of a swizzled tile of D columns; col a multiple of 8.
-template <int D>
-DSV4CU_DEV uint16_t *sa_at(uint16_t *base, int row, int col)
-{
-    return base + row * D + ((((col >> 3) ^ (row & 7)) << 3) | (col & 7));
-}
-
 // The rows and keys of one CTA.
 struct SaTile {
     int begin, len;       // token range of the request / sequence
@@ -434,7 +449,8 @@ constexpr int sa_warps(int D) { return D >= 128 ? 8 : 4; }
 template <int D, int BN, int TERMS, bool F16, bool TREE>
 __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const __grid_constant__ SaArgs a)
 {
-    constexpr int NW = sa_warps(D), THREADS = 32 * NW, BM = SA_BM, C16 = D / 8;
+    constexpr int NW = sa_warps(D), THREADS = 32 * NW, BM = SA_BM;
+    constexpr int RS = D + 8;                            // row stride of keys and values: 16 bytes over, so ldmatrix rows spread
     constexpr int DW = D / NW, KS = DW / 16, ON = DW / 8;   // dims of a warp, their k steps, their output n tiles
     constexpr int OG = ON < 4 ? ON : 4;                  // output n tiles accumulated at a time
     constexpr int SS = BN + 8, PS = BN + 8;              // row strides of partial scores and weights
@@ -445,13 +461,14 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
     extern __shared__ __align__(128) uint16_t sa_sm[];
     __shared__ int s_par[TREE ? SA_MAX_NODES : 1], s_depth[TREE ? SA_MAX_NODES : 1];
     __shared__ unsigned long long s_anc[TREE ? SA_MAX_NODES : 1][2];
-    __shared__ const uint16_t *s_row[2][2][BN];          // [slot][keys, values]: rows of a block, NULL outside
+    __shared__ __align__(8) uint64_t s_full[2];
+    __shared__ uint8_t s_there[2][BN];                   // the key is there
     __shared__ int s_bad[2];                             // block with a missing row
     __shared__ float s_alpha[BM], s_m[BM], s_l[BM];
     const bool shared_v = a.v == nullptr;
-    const int stage_el = (shared_v ? 1 : 2) * BN * D;
-    uint16_t *kvs = sa_sm;                               // [nst][shared_v ? 1 : 2][BN][D]
-    float *part = reinterpret_cast<float *>(kvs + a.nst * stage_el);   // [NW][BM][SS]
+    const int stage_el = (shared_v ? 1 : 2) * BN * RS;
+    uint16_t *kvs = sa_sm;                               // [2][shared_v ? 1 : 2][BN][RS]
+    float *part = reinterpret_cast<float *>(kvs + 2 * stage_el);       // [NW][BM][SS]
     uint16_t *ps = reinterpret_cast<uint16_t *>(part + NW * BM * SS);  // [TERMS][BM][PS]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
 
@@ -544,29 +561,49 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
             return key <= tok && tok - key < a.window;
         }
     };
-    // rows of block blk into slot blk & 1 (a barrier before their use)
-    auto find_rows = [&](int blk) {
-        if (tid < BN) {
-            const uint16_t *k = row(blk, tid, false);
-            s_row[blk & 1][0][tid] = k;
-            if (!shared_v) s_row[blk & 1][1][tid] = row(blk, tid, true);
-            if (!k) s_bad[blk & 1] = blk;
+    // Thread j < BN brings row j of every block: a copy of the whole row, or
+    // zeros where there is none. The row's address is looked up a block ahead.
+    const uint16_t *next_k = nullptr, *next_v = nullptr;
+    auto look_up = [&](int blk) {
+        next_k = next_v = nullptr;
+        if (tid < BN && blk < t.blk1) {
+            next_k = row(blk, tid, false);
+            if (!shared_v) next_v = row(blk, tid, true);
         }
     };
-    auto issue = [&](int blk) {
-        uint16_t *kd = kvs + (a.nst == 2 ? blk & 1 : 0) * stage_el;
-        const int ch = tid % C16;
-#pragma unroll
-        for (int j = tid / C16; j < BN; j += THREADS / C16) {
-            const uint16_t *k = s_row[blk & 1][0][j];
-            sa_cp16(sa_at<D>(kd, j, 8 * ch), k ? k + 8 * ch : (const uint16_t *)a.q, k != nullptr);
-            if (!shared_v) {
-                const uint16_t *v = s_row[blk & 1][1][j];
-                sa_cp16(sa_at<D>(kd + BN * D, j, 8 * ch), v ? v + 8 * ch : (const uint16_t *)a.q, v != nullptr);
+    auto issue = [&](int blk) {                          // the rows of the last look_up
+        if (tid >= BN) return;
+        const int st = (blk - t.blk0) & 1;
+        uint16_t *dst = kvs + st * stage_el + tid * RS;
+        s_there[st][tid] = next_k != nullptr;
+        if (next_k) {
+            mbar_arrive_expect_tx(&s_full[st], (shared_v ? 1 : 2) * D * 2);
+            sa_bulk(dst, next_k, D * 2, &s_full[st]);
+            if (!shared_v) sa_bulk(dst + BN * RS, next_v, D * 2, &s_full[st]);
+        } else {
+            s_bad[st] = blk;
+            for (int c = 0; c < D; c += 8) {
+                *reinterpret_cast<uint4 *>(dst + c) = make_uint4(0, 0, 0, 0);
+                if (!shared_v) *reinterpret_cast<uint4 *>(dst + BN * RS + c) = make_uint4(0, 0, 0, 0);
             }
+            sa_fence_async();                            // before a later copy into the same place
+            mbar_arrive(&s_full[st]);
         }
-        sa_commit();
     };
+    if (tid < 2) {
+        s_bad[tid] = -1;
+        mbar_init(&s_full[tid], BN);
+    }
+    if (tid == 0) fence_mbar_init();
+    if (tid < BM) {
+        s_m[tid] = -INFINITY;
+        s_l[tid] = 0.0f;
+    }
+    __syncthreads();
+    look_up(t.blk0);
+    issue(t.blk0);
+    look_up(t.blk0 + 1);
+
     // ---- this warp's dims of the queries as mma fragments: rows g / g + 8 of
     // m tile mt, dims DW * warp + 16 kk + 2c.. / 2c + 8..
     uint32_t qa[2][KS][TERMS][4];
@@ -594,17 +631,6 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
                 }
         }
 
-    if (tid < 2) s_bad[tid] = -1;
-    if (tid < BM) {
-        s_m[tid] = -INFINITY;
-        s_l[tid] = 0.0f;
-    }
-    __syncthreads();
-    find_rows(t.blk0);
-    if (t.blk0 + 1 < t.blk1) find_rows(t.blk0 + 1);
-    __syncthreads();
-    issue(t.blk0);
-
     const int arow = (lane & 7) + 8 * ((lane >> 3) & 1), acol = 8 * (lane >> 4);
     const int brow = (lane & 7) + 8 * (lane >> 4), bcol = 8 * ((lane >> 3) & 1);
     const int d0 = DW * warp;
@@ -625,16 +651,17 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
         }
     };
 
+    bool arrives = true;
     for (int blk = t.blk0; blk < t.blk1; blk++) {
-        if (a.nst == 2 && blk + 1 < t.blk1) {
-            issue(blk + 1);
-            sa_wait<1>();
-        } else {
-            sa_wait<0>();
+        const int st = (blk - t.blk0) & 1;
+        if (blk + 1 < t.blk1) {
+            issue(blk + 1);                              // into the stage that the block before this one left
+            look_up(blk + 2);
         }
-        __syncthreads();
-        uint16_t *kt = kvs + (a.nst == 2 ? blk & 1 : 0) * stage_el, *vt = shared_v ? kt : kt + BN * D;
-        const bool full = is_full(blk) && s_bad[blk & 1] != blk;
+        // after a copy that does not arrive nothing is waited for any more
+        if (arrives) arrives = sa_poll(&s_full[st], ((blk - t.blk0) >> 1) & 1, a.status, SA_COPY);
+        uint16_t *kt = kvs + st * stage_el, *vt = shared_v ? kt : kt + BN * RS;
+        const bool full = is_full(blk) && s_bad[st] != blk;
         // ---- partial scores over the warp's dims
 #pragma unroll
         for (int n = 0; n < BN / 8; n += 4) {            // eight accumulators at a time cover the product's latency
@@ -643,7 +670,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
             for (int kk = 0; kk < KS; kk++) {
                 uint32_t b[2][4];
 #pragma unroll
-                for (int u = 0; u < 2; u++) sa_ldsm4(b[u], sa_at<D>(kt, 8 * n + 16 * u + brow, d0 + 16 * kk + bcol));
+                for (int u = 0; u < 2; u++) sa_ldsm4(b[u], kt + (8 * n + 16 * u + brow) * RS + d0 + 16 * kk + bcol);
 #pragma unroll
                 for (int x = TERMS - 1; x >= 0; x--)
 #pragma unroll
@@ -689,7 +716,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
                 if (!full) {
                     bool see;
                     if (TREE && blk < t.nblk_c)
-                        see = s_row[blk & 1][0][scol + e] != nullptr &&
+                        see = s_there[st][scol + e] &&
                               t.ctx - (t.key0 + blk * BN + scol + e) + s_depth[stok] < a.window;
                     else
                         see = vis(stok, blk, scol + e);
@@ -736,7 +763,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
                 uint32_t b[OG / 2][4];
 #pragma unroll
                 for (int n = 0; n < OG / 2; n++) {
-                    sa_ldsm4_t(b[n], sa_at<D>(vt, 16 * kk + arow, d0 + 8 * n0 + 16 * n + acol));
+                    sa_ldsm4_t(b[n], vt + (16 * kk + arow) * RS + d0 + 8 * n0 + 16 * n + acol);
                 }
 #pragma unroll
                 for (int x = TERMS - 1; x >= 0; x--) {
@@ -758,9 +785,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
 #pragma unroll
                     for (int e = 0; e < 4; e++) o[mt][n0 + n][e] = fmaf(o[mt][n0 + n][e], al[mt][e >> 1], acc[mt][n][e]);
         }
-        if (blk + 2 < t.blk1) find_rows(blk + 2);        // this block's rows are used up (its mask is read)
         __syncthreads();                                 // this stage, the weights and s_alpha are free
-        if (a.nst == 1 && blk + 1 < t.blk1) issue(blk + 1);
     }
     bool done = false;
     {
@@ -777,33 +802,49 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
             done = true;
         }
     }
+    // rows through shared memory (every block is used up), so that whole lines
+    // are stored
+    constexpr int OS = D + 4;
+    float *ob = reinterpret_cast<float *>(sa_sm);        // [BM][OS]
+    const bool in_parts = t.parts > 1;
+    if (!done) {
 #pragma unroll
-    for (int mt = 0; mt < 2; mt++)
+        for (int mt = 0; mt < 2; mt++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int r = 16 * mt + g + 8 * h;
-            if (done || r >= t.rows) continue;
-            const int pr = t.r0 + r, tok = pr / a.G, head = t.kvh * a.G + pr % a.G, col = d0 + 2 * c;
-            if (t.parts > 1) {
-                const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + tok) * a.hq + head;
+            for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int n = 0; n < ON; n++)
-                    *reinterpret_cast<float2 *>(a.po + id * D + col + 8 * n) = make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
-                if (warp == 0 && c == 0) {
-                    a.pm[id] = s_m[r];
-                    a.pl[id] = s_l[r];
-                }
-            } else {
-                const float inv = sa_inv(s_l[r], s_m[r], a.sink, head);
-                const size_t at = (size_t)(t.begin + tok) * a.ldo + (size_t)head * D + col;
-#pragma unroll
-                for (int n = 0; n < ON; n++) {
-                    const float x = o[mt][n][2 * h] * inv, y = o[mt][n][2 * h + 1] * inv;
-                    if constexpr (QF32) *reinterpret_cast<float2 *>(reinterpret_cast<float *>(a.o) + at + 8 * n) = make_float2(x, y);
-                    else *reinterpret_cast<uint32_t *>(reinterpret_cast<uint16_t *>(a.o) + at + 8 * n) = sa_pack<F16>(x, y);
-                }
+                    *reinterpret_cast<float2 *>(ob + (16 * mt + g + 8 * h) * OS + d0 + 8 * n + 2 * c) =
+                        make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
+        if (tid < t.rows) {
+            const int head = t.kvh * a.G + (t.r0 + tid) % a.G;
+            s_alpha[tid] = in_parts ? 1.0f : sa_inv(s_l[tid], s_m[tid], a.sink, head);
+            if (in_parts) {
+                const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + (t.r0 + tid) / a.G) * a.hq + head;
+                a.pm[id] = s_m[tid];
+                a.pl[id] = s_l[tid];
             }
         }
+    }
+    __syncthreads();
+    for (int x = tid; x < (done ? 0 : t.rows * (D / 8)); x += THREADS) {
+        const int r = x / (D / 8), col = (x - r * (D / 8)) * 8, pr = t.r0 + r, tok = pr / a.G,
+                  head = t.kvh * a.G + pr - tok * a.G;
+        const float f = s_alpha[r];
+        float4 y = *reinterpret_cast<const float4 *>(ob + r * OS + col), z = *reinterpret_cast<const float4 *>(ob + r * OS + col + 4);
+        y = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+        z = make_float4(z.x * f, z.y * f, z.z * f, z.w * f);
+        const size_t at = (size_t)(t.begin + tok) * a.ldo + (size_t)head * D + col;
+        if (in_parts || QF32) {
+            float *dst = in_parts ? a.po + ((size_t)t.split * a.nt * a.hq + (size_t)(t.begin + tok) * a.hq + head) * D + col
+                                  : reinterpret_cast<float *>(a.o) + at;
+            *reinterpret_cast<float4 *>(dst) = y;
+            *reinterpret_cast<float4 *>(dst + 4) = z;
+        } else {
+            *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.o) + at) =
+                make_uint4(sa_pack<F16>(y.x, y.y), sa_pack<F16>(y.z, y.w), sa_pack<F16>(z.x, z.y), sa_pack<F16>(z.z, z.w));
+        }
+    }
     if (TREE && t.parts > 1) {
         // the tile's last split to finish joins them all
         __threadfence();
@@ -828,14 +869,15 @@ constexpr int SA_SMEM_MAX = 220 * 1024;      // of 227 KB: the static arrays com
 static inline int sa_block(int D, bool shared_v) { return D == 512 && !shared_v ? 32 : 64; }
 
 template <int D, int BN, int TERMS, bool F16, bool TREE>
-int serve_attn_launch(SaArgs a, cudaStream_t st)
+int serve_attn_launch(const SaArgs &a, cudaStream_t st)
 {
     auto kern = serve_attn_kernel<D, BN, TERMS, F16, TREE>;
     constexpr int NW = sa_warps(D);
-    const size_t stage = (size_t)(a.v ? 2 : 1) * BN * D * 2;
-    const size_t rest = (size_t)NW * SA_BM * (BN + 8) * 4 + (size_t)TERMS * SA_BM * (BN + 8) * 2;
-    a.nst = rest + 2 * stage <= SA_SMEM_MAX ? 2 : 1;
-    const size_t smem = rest + a.nst * stage;
+    static_assert((size_t)SA_BM * (D + 4) * 4 <= (size_t)2 * BN * (D + 8) * 2, "the output rows fit the stages");
+    const size_t smem = (size_t)(a.v ? 4 : 2) * BN * (D + 8) * 2 + (size_t)NW * SA_BM * (BN + 8) * 4 +
+                        (size_t)TERMS * SA_BM * (BN + 8) * 2;
+    static_assert((size_t)(D == 512 && BN == 64 ? 2 : 4) * BN * (D + 8) * 2 + (size_t)NW * SA_BM * (BN + 8) * 4 +
+                      (size_t)TERMS * SA_BM * (BN + 8) * 2 <= SA_SMEM_MAX, "shared memory");
     static SmemLimit lim;
     DSV4CU_CUDA_TRY(smem_limit(lim, (const void *)kern, (int)smem));
     dim3 grid;

@@ -32,7 +32,6 @@
 #include <cuda.h>
 
 #include "serve_attn.cuh"
-#include "tma_gemv.cuh"
 #include "tmap.h"
 #include "umma.cuh"
 
@@ -114,7 +113,6 @@ DSV4CU_DEV void su_loaded32(uint32_t *r)
     asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
 }
 DSV4CU_DEV void su_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-DSV4CU_DEV void su_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 template <int N>
 DSV4CU_DEV void su_bar(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory"); }
 template <int R>
@@ -169,30 +167,6 @@ DSV4CU_DEV void su_tma(void *dst, const CUtensorMap *map, int x, int head, int r
                  " [%0], [%1, {%2, %3, %4}], [%5];"
                  ::"r"(umma::saddr(dst)), "l"(map), "r"(x), "r"(head), "r"(row), "r"(umma::saddr(bar)) : "memory");
 }
-// Bounded wait that polls: no suspend hint and no look at the clock on the
-// way to a phase that completes in time (a strip's products and softmax wait
-// for each other every block).
-DSV4CU_DEV bool su_wait(uint64_t *bar, uint32_t parity, int *err, int code)
-{
-    const uint32_t a = umma::saddr(bar);
-    uint64_t t0 = 0;
-    for (uint32_t i = 1;; i++) {
-        uint32_t ok;
-        asm volatile("{\n\t.reg .pred p;\n\t"
-                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-                     "selp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(ok) : "r"(a), "r"(parity) : "memory");
-        if (ok) return true;
-        if ((i & 1023u) == 0u) {
-            const uint64_t now = globaltimer_ns();
-            if (t0 == 0) t0 = now;
-            else if (now - t0 > MBAR_TIMEOUT_NS) break;
-        }
-    }
-    atomicCAS(err, 0, code);
-    return false;
-}
-
 // Bits lo .. hi of 128 as four words (empty where lo > hi).
 DSV4CU_DEV uint32_t su_range(int lo, int hi, int word)
 {
@@ -404,7 +378,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
 #pragma unroll
                 for (int kv = 0; kv < 2; kv++) {
                     uint64_t *full = kv ? &vfull[st] : &kfull[st], *empty = kv ? &vempty[st] : &kempty[st];
-                    if (lane == 0 && u > 0) ok = su_wait(empty, (u - 1) & 1, a.status, kv ? SUE_VEMPTY : SUE_KEMPTY);
+                    if (lane == 0 && u > 0) ok = sa_poll(empty, (u - 1) & 1, a.status, kv ? SUE_VEMPTY : SUE_KEMPTY);
                     ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
                     if (!ok) break;
                     if (lane == 0) mbar_arrive_expect_tx(full, bytes);
@@ -440,12 +414,12 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
             // memory ends before it overflows
             const uint64_t dq = umma::desc_sw128(qs), dk = umma::desc_sw128(ks), dv = su_desc_v(vs, KSUB);
             uint32_t once = 0;                           // blocks that one of their two strips has scored
-            bool ok = su_wait(&qfull, 0, a.status, SUE_Q);
+            bool ok = sa_poll(&qfull, 0, a.status, SUE_Q);
             umma::fence_after();
             // scores of strip s against block b: its key stage and phase
             auto scores = [&](int s, int b) {
                 const int n = b - u0, use = n / nst, st = n - use * nst;
-                ok = ok && su_wait(&kfull[st], use & 1, a.status, SUE_KFULL);
+                ok = ok && sa_poll(&kfull[st], use & 1, a.status, SUE_KFULL);
                 if (!ok) return;
                 umma::fence_after();
                 const uint64_t q = dq + (uint32_t)((ualt ? 0 : s) * (QB >> 4)), k = dk + (uint32_t)(st * (KVB >> 4));
@@ -472,8 +446,8 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
                     if (ualt ? ((b - u0) & 1) != s : s ? b < g1 : b >= h0) continue;   // strip 0 ends first, strip 1 starts last
-                    ok = ok && su_wait(&pfull[s], turn[s] & 1, a.status, SUE_P) &&
-                         su_wait(&vfull[st], phase, a.status, SUE_VFULL);
+                    ok = ok && sa_poll(&pfull[s], turn[s] & 1, a.status, SUE_P) &&
+                         sa_poll(&vfull[st], phase, a.status, SUE_VFULL);
                     ok = __all_sync(0xFFFFFFFFu, ok);
                     if (!ok) break;
                     umma::fence_after();
@@ -515,7 +489,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
                 const int x = q_i + e * q_n, r = x / (D / 8), ch = x - r * (D / 8);
                 if (r < 128) *reinterpret_cast<uint4 *>(q + (ch >> 3) * SU_SUB + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = qw[e];
             }
-            su_fence_async();
+            sa_fence_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&qfull);
         }
@@ -552,7 +526,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
             const bool masked = !is_full(b) || (TREE && lost);
             constexpr int W = BN / 32;                   // mask words of a block
             uint32_t vis[W];
-            ok = __all_sync(0xFFFFFFFFu, su_wait(&sfull[s], turn & 1, a.status, SUE_S));
+            ok = __all_sync(0xFFFFFFFFu, sa_poll(&sfull[s], turn & 1, a.status, SUE_S));
             if (!ok) break;
             const bool cached = TREE && b < tp->nblk_c;
             const int base = TREE && !cached ? (b - tp->nblk_c) * BN : tp->key0 + b * BN;
@@ -565,7 +539,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
                 // it, so the stage's last use is over and its barrier is at
                 // most one phase away: the parity below means this block.
                 const int n = b - c0, st = n % a.nst;
-                ok = __all_sync(0xFFFFFFFFu, su_wait(&vfull[st], (n / a.nst) & 1, a.status, SUE_VFULL));
+                ok = __all_sync(0xFFFFFFFFu, sa_poll(&vfull[st], (n / a.nst) & 1, a.status, SUE_VFULL));
                 if (!ok) break;
                 if (i < BN && !(cached ? in_pool(base + i) : base + i < tp->len)) {
                     uint8_t *v = vs + st * KVB + i * 128;
@@ -574,7 +548,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
 #pragma unroll
                         for (int x = 0; x < 8; x++) *reinterpret_cast<uint4 *>(v + c * KSUB + 16 * x) = make_uint4(0, 0, 0, 0);
                 }
-                su_fence_async();
+                sa_fence_async();
             }
             if (masked) {
                 if (cached) {
@@ -664,7 +638,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
         }
         // ---- outputs
         const bool any = first < end;
-        if (any) ok = ok && __all_sync(0xFFFFFFFFu, su_wait(&ofull[s], 0, a.status, SUE_O));
+        if (any) ok = ok && __all_sync(0xFFFFFFFFu, sa_poll(&ofull[s], 0, a.status, SUE_O));
         umma::fence_after();
         const SaArgs &a0 = a;
         auto row_of = [tp, ap = &a0](int blk, int j, bool values) -> const uint16_t * {
