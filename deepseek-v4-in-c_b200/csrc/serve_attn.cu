@@ -22,7 +22,7 @@ static int check_common(const char *what, const Common &c)
     if (c.n_heads <= 0 || c.n_kv <= 0 || c.n_heads % c.n_kv)
         return dsv4cu_set_error(DSV4CU_ERR_ARG, "%s: %d query heads over %d key heads", what, c.n_heads, c.n_kv);
     if (c.window < 0) return dsv4cu_set_error(DSV4CU_ERR_ARG, "%s: window %d", what, c.window);
-    if (!(c.scale > 0.0f) || isinf(c.scale)) return dsv4cu_set_error(DSV4CU_ERR_ARG, "%s: scale must be positive and finite", what);
+    if (!(c.scale > 0.0f) || isinf(c.scale * SA_LOG2E)) return dsv4cu_set_error(DSV4CU_ERR_ARG, "%s: scale must be positive and finite", what);
     if (!elem_known(c.q_type) || !elem_known(c.kv_type) || c.kv_type == DSV4CU_F32 ||
         (c.q_type != c.kv_type && !(c.q_type == DSV4CU_F32 && c.kv_type == DSV4CU_BF16)))
         return dsv4cu_set_error(DSV4CU_ERR_UNSUPPORTED, "%s: queries of type %d over keys of type %d", what, c.q_type,
@@ -33,6 +33,7 @@ static int check_common(const char *what, const Common &c)
         return dsv4cu_set_error(DSV4CU_ERR_ARG, "%s: too many heads or tokens", what);
     if (c.n_req == 0 || c.nt == 0) return DSV4CU_OK;
     if (!c.o || !c.q || !c.k) return dsv4cu_set_error(DSV4CU_ERR_ARG, "%s: NULL argument", what);
+    if (c.o == c.q || c.o == c.k || c.o == c.v) return dsv4cu_set_error(DSV4CU_ERR_ARG, "%s: o may not lie over an input", what);
     const int qs = elem_bytes(c.q_type), ks = elem_bytes(c.kv_type);
     const int64_t qrow = (int64_t)c.n_heads * c.head_dim, krow = (int64_t)c.n_kv * c.head_dim;
     if (c.ldo < qrow || c.ldq < qrow || c.ldk < krow || (c.v && c.ldv < krow))

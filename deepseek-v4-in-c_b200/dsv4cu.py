@@ -758,14 +758,14 @@ class Device:
 
     def _rows(self, what, t, heads, dim, dtype=None):
         """Packed token rows [nt][heads][dim], any stride between tokens: that stride in elements."""
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.get_device() != self.device or \
+        shape, stride = t.shape, t.stride()
+        if len(shape) != 3 or shape[1] != heads or shape[2] != dim or t.get_device() != self.device or \
                 t.dtype not in self._elem or (dtype is not None and t.dtype is not dtype):
             raise DSV4CUError(f"{what}: needs rows [tokens][{heads}][{dim}] on cuda:{self.device}, got {t.dtype} "
-                              f"{tuple(t.shape)} on {t.device}")
-        step, head, one = t.stride()
-        if (one != 1 and dim > 1) or (head != dim and heads > 1):
-            raise DSV4CUError(f"{what}: the heads of a token must be contiguous, got strides {t.stride()}")
-        return step if t.shape[0] > 1 else heads * dim
+                              f"{tuple(shape)} on {t.device}")
+        if (stride[2] != 1 and dim > 1) or (stride[1] != dim and heads > 1):
+            raise DSV4CUError(f"{what}: the heads of a token must be contiguous, got strides {stride}")
+        return stride[0] if shape[0] > 1 else heads * dim
 
     def _sink(self, what, sink, heads):
         if sink is None:

@@ -633,7 +633,9 @@ int dsv4cu_head(dsv4cu_ctx *ctx, float *logits, int *best, const float *x, const
  * other calls: reserve it (dsv4cu_ctx_reserve) before capturing, do not let
  * it grow while captured graphs are alive, and give streams or graphs that
  * run at the same time a context each. Index arrays are device int32; what
- * they hold is clamped or skipped, never read or written through. */
+ * they hold is clamped or skipped, never read or written through. Outputs may
+ * not lie over inputs except where a call says so. Results do not depend on
+ * timing: the same call gives the same bits. */
 enum { DSV4CU_F32 = 0, DSV4CU_BF16 = 1, DSV4CU_F16 = 2 };   /* element types */
 
 /* Block tables and slot maps from request lengths. Request b holds held[b]

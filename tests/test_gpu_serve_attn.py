@@ -377,3 +377,89 @@ def test_one_node_is_the_prompts_last_token(dev):
     want, bound = servefix.attend(q[-1:], k, v, torch.ones(1, n, dtype=torch.bool, device="cuda"), dim ** -0.5)
     for got in (one, o[-1:]):
         servefix.check_close(got, want, bound(torch.bfloat16, torch.bfloat16))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,kv", [(64, 2), (128, 2), (512, 1)])
+def test_same_call_same_bits(dev, kind, dim, kv):
+    """Splits that finish in any order are joined in one: repeated calls, and calls after others, agree bit for bit."""
+    import torch
+    args, s = _tree(dev, [4000, 900, 0, 2111], [6, 1, 3, 17], 4 * kv, kv, dim, kind, page=64, sink=True)
+    o, q = args[0], args[1]
+    first = o.clone()
+    for i in range(6):
+        o.fill_(7.0)
+        dev.tree_attn(*args, sink=s)
+        if i % 2:
+            _prompt(dev, [100], 4, 2, dim, kind)
+        assert torch.equal(o, first)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 512])
+def test_two_contexts_on_two_streams(dev, kind, dim):
+    """Calls that run at the same time on streams of their own, each with its own context, as one after the other."""
+    import torch
+    import dsv4cu
+    other = dsv4cu.Device(dev.device)
+    try:
+        cases = [_tree(dev, [3000, 500], [4, 2], 8, 2, dim, kind, page=64, seed=i) for i in range(2)]
+        want = [c[0][0].clone() for c in cases]
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        graphs = []
+        for d, st, (args, s) in zip((dev, other), streams, cases):
+            d.L.dsv4cu_ctx_reserve(d.ctx, 1 << 27)
+            args[0].fill_(7.0)
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                for _ in range(20):
+                    d.tree_attn(*args, sink=s)
+            graphs.append(g)
+        for _ in range(3):
+            for g, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    g.replay()
+        torch.cuda.synchronize()
+        for w, (args, _) in zip(want, cases):
+            assert torch.equal(args[0], w)
+        assert other.status_code() == 0
+    finally:
+        other.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 512])
+def test_prompt_captured_and_replayed(dev, kind, dim):
+    """A captured prompt pass of a padded batch follows the offsets it finds: rows behind the last sequence stay."""
+    import torch
+    qt, ct = (getattr(torch, x) for x in kind)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    n = 700
+    q, k, v = (_rows(gen, n, h, dim, t) for h, t in ((4, qt), (2, ct), (2, ct)))
+    o, cu = _out(n, 4, dim, qt), _i([0, 0, 0, 0])
+    dev.prompt_attn(o, q, k, v, cu, 0.1)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        dev.prompt_attn(o, q, k, v, cu, 0.1)
+    for at in ([0, 700, 700, 700], [0, 1, 130, 600], [5, 5, 300, 301]):
+        cu.copy_(_i(at))
+        o.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        for b in range(3):
+            r = slice(at[b], at[b + 1])
+            if at[b] == at[b + 1]:
+                continue
+            want, bound = servefix.attend(q[r], k[r], v[r], servefix.causal_seen(at[b + 1] - at[b], 0).cuda(), 0.1)
+            servefix.check_close(o[r], want, bound(qt, ct), f"{at} sequence {b}")
+        assert bool((o[at[-1]:] == 7.0).all()) and bool((o[:at[0]] == 7.0).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompt_windows_of_wide_tiles(dev, dim):
+    """One query head per key head: a tile's strips start blocks apart, each in its own part of the window."""
+    for window in (1, 30, 64, 127, 128, 129, 300):
+        _prompt(dev, [900, 40], 2, 2, dim, KINDS[0], window=window)

@@ -83,7 +83,7 @@ def test_paged_write_refuses(L, ctx, kw, code):
 
 def _prompt(**kw):
     import dsv4cu
-    base = dict(o=P, q=P, k=P, v=P, ldo=512, ldq=512, ldk=128, ldv=128, q_type=1, kv_type=1, cu=P, n_req=1, nt=4,
+    base = dict(o=2 * P, q=P, k=P, v=P, ldo=512, ldq=512, ldk=128, ldv=128, q_type=1, kv_type=1, cu=P, n_req=1, nt=4,
                 n_heads=8, n_kv=2, head_dim=64, window=0, scale=0.125, sink=None)
     base.update(kw)
     return dsv4cu.PromptAttnArgs(**base)
@@ -91,7 +91,7 @@ def _prompt(**kw):
 
 def _tree(**kw):
     import dsv4cu
-    base = dict(o=P, q=P, k=P, v=P, k_cache=P, v_cache=P, ldo=512, ldq=512, ldk=128, ldv=128, q_type=1, kv_type=1,
+    base = dict(o=2 * P, q=P, k=P, v=P, k_cache=P, v_cache=P, ldo=512, ldq=512, ldk=128, ldv=128, q_type=1, kv_type=1,
                 table=P, ctx_len=P, cu=P, parent=P, n_req=1, nt=4, n_heads=8, n_kv=2, head_dim=64, page_size=16,
                 n_pages=8, max_pages=4, max_nodes=4, max_ctx=64, window=0, scale=0.125, sink=None)
     base.update(kw)
@@ -100,7 +100,8 @@ def _tree(**kw):
 
 BOTH = [(dict(n_req=-1), ARG), (dict(nt=-1), ARG), (dict(n_heads=0), ARG), (dict(n_kv=0), ARG), (dict(n_kv=3), ARG),
         (dict(window=-1), ARG), (dict(scale=0.0), ARG), (dict(scale=-1.0), ARG), (dict(scale=float("inf")), ARG),
-        (dict(scale=float("nan")), ARG), (dict(kv_type=0, q_type=0), UNSUPPORTED), (dict(kv_type=2), UNSUPPORTED),
+        (dict(scale=float("nan")), ARG),
+        (dict(scale=3.0e38), ARG), (dict(o=P), ARG), (dict(kv_type=0, q_type=0), UNSUPPORTED), (dict(kv_type=2), UNSUPPORTED),
         (dict(q_type=0, kv_type=2), UNSUPPORTED), (dict(q_type=5), UNSUPPORTED), (dict(head_dim=96), UNSUPPORTED),
         (dict(head_dim=0), UNSUPPORTED), (dict(o=None), ARG), (dict(q=None), ARG), (dict(k=None), ARG),
         (dict(cu=None), ARG), (dict(ldq=511), ARG), (dict(ldo=448), ARG), (dict(ldk=64), ARG), (dict(ldv=64), ARG),
