@@ -24,9 +24,18 @@
 // log2) above it: weights stay below 2^8, sums and products are exact to the
 // same relative rounding, and the outputs in TMEM are seldom rescaled.
 //
-// Bound by: the exponentials (16 per clock and SM against 128 x 128 scores per
-// block and strip: 1024 clocks, as long as the strip's two products at head
-// dim 128), then the tensor core; for trees of few rows the cache's bytes.
+// Bound by: per block and strip at head dim 128, 1024 clocks of products
+// against 1024 of exponentials (16 a clock and SM for 128 x 128 scores), which
+// the turns overlap; at head dim 64 the exponentials; for trees of few rows the
+// cache's bytes. Measured on one B200:
+//   32768 causal tokens, 64 heads over 8, 128 dims: 13.6 ms in a short run
+//   (1290 TFLOP/s, 0.77 of the measured bf16 rate), 15.5 to 16 ms repeated at
+//   the power limit; products and copies alone take 11.8 ms.
+//   29 prompts, 16001 tokens, 16 heads over 4, 64 dims: 92 us, 107 us with one
+//   CTA of 128-key blocks per SM.
+//   32 trees of 8 to 16 nodes over up to 32000 tokens, 64 heads over 8: 501 us
+//   in a short run (5.8 TB/s, 0.89 of the measured copy rate), 588 us repeated;
+//   606 us with two stages instead of three.
 #pragma once
 
 #include <cuda.h>

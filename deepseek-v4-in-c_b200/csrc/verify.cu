@@ -24,6 +24,14 @@
 // sum; two sets of slots, so the next sum does not disturb readers). A row
 // comes from memory once; later sums and the rescan of the one segment that
 // holds the token find it in L2.
+//
+// Bound by latency: a request's sums come one after the other (1.6 on average
+// over sampled trees of 8, up to 4), each a few batches of loads, a conversion
+// of every element to double (16 a clock and SM) and a cluster barrier. 64
+// trees over 129280 tokens: 29 us, where the bytes of one row of p and one of
+// draft each take 10 us; one chain of 5 over 32000: 7.7 us. Four CTAs of 256
+// threads per SM keep all 64 clusters resident; asking for a row's slice in L2
+// ahead of its loads changed nothing (31.7 us).
 #include <math.h>
 
 #include <cooperative_groups.h>
