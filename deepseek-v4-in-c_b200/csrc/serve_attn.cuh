@@ -73,8 +73,7 @@ struct SaArgs {
     float *pm, *pl, *po;              // partials [splits][nt * hq](, D), splits > 1
     int *counters;                    // [n_req][hkv][row_tiles], zero between calls: splits done
     int *status;
-    int nst;                          // key stages in shared memory
-    int two, box_log2;                // tcgen05 kernel: two row tiles per CTA; rows of a cached copy's box
+    int nst, two, box_log2;           // tcgen05 kernel: stages, two strips of rows per CTA, rows of a cached copy's box
 };
 
 // The key blocks of request b of a tree call: blocks of BN cached keys from
