@@ -110,6 +110,8 @@ static int tree_check(const dsv4cu_tree_attn_args *a, const Common &c)
     if (a->max_nodes <= 0 || a->max_nodes > SA_MAX_NODES)
         return dsv4cu_set_error(DSV4CU_ERR_ARG, "tree_attn: max_nodes %d not in 1 .. %d", a->max_nodes, SA_MAX_NODES);
     if (c.n_req > 65535) return dsv4cu_set_error(DSV4CU_ERR_ARG, "tree_attn: %d requests", c.n_req);
+    if ((int64_t)a->max_nodes * c.n_heads > INT_MAX)      // row numbers of a request stay in 32 bits
+        return dsv4cu_set_error(DSV4CU_ERR_ARG, "tree_attn: %d nodes of %d heads", a->max_nodes, c.n_heads);
     if ((c.v == nullptr) != (a->v_cache == nullptr) && a->n_pages > 0)
         return dsv4cu_set_error(DSV4CU_ERR_ARG, "tree_attn: v and v_cache go together");
     if (c.n_req == 0 || c.nt == 0) return DSV4CU_OK;

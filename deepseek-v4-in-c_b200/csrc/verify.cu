@@ -42,6 +42,7 @@ namespace dsv4cu {
 namespace cg = cooperative_groups;
 
 constexpr int VER_MAX_NODES = 128;
+constexpr int VER_MAX_VOCAB = 1 << 30; // indexes a step past the row's end stay in 32 bits
 constexpr int VER_THREADS = 256;
 constexpr int VER_BATCH = 32;         // elements a lane has in flight, of one row or of both
 constexpr int VER_WARPS = VER_THREADS / 32;
@@ -127,6 +128,9 @@ __global__ void __launch_bounds__(128) verify_greedy_kernel(const VerifyArgs a)
     __syncwarp();
     ver_write(a, b, begin, n, line[warp], acc, lane, 32);
 }
+
+DSV4CU_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+DSV4CU_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // The remainder of the current row after the refusals so far. With draft
 // probabilities the refusals' masses add up: max(max(p - c0 q, 0) - c1 q, 0) =
@@ -225,6 +229,7 @@ __global__ void __cluster_dims__(VER_CL, 1, 1) __launch_bounds__(VER_THREADS, 4)
         if (rank == 0 && tid == 0) ver_refuse(a, b, begin, n);
         return;
     }
+    cluster_arrive();
     for (int i = tid; i < n; i += VER_THREADS) {
         const int par = __ldg(a.parent + begin + i), x = __ldg(a.tokens + begin + i);
         s_u[i] = __ldg(a.u + begin + i);
@@ -236,6 +241,9 @@ __global__ void __cluster_dims__(VER_CL, 1, 1) __launch_bounds__(VER_THREADS, 4)
     }
     if (tid == 0) line[0] = 0;
     __syncthreads();
+    // no CTA stores into another's shared memory before that one has started:
+    // each has said so above, while its loads were on their way
+    cluster_wait();
     // this CTA's slice and this warp's segment of it, multiples of 32 elements
     const int per = ((a.vocab + VER_CL - 1) / VER_CL + 31) & ~31;
     const int lo = min(a.vocab, rank * per), hi = min(a.vocab, lo + per);
@@ -458,7 +466,7 @@ extern "C" int dsv4cu_verify_sample(dsv4cu_ctx *ctx, int *accepted, int *next, i
 {
     int r = verify_check(ctx, "verify_sample", accepted, next, path, tokens, parent, cu, slot, slot_out, n_req, nt);
     if (r || n_req == 0) return r;
-    if (vocab <= 0 || ldp < vocab || (draft && ldd < vocab))
+    if (vocab <= 0 || vocab > VER_MAX_VOCAB || ldp < vocab || (draft && ldd < vocab))
         return dsv4cu_set_error(DSV4CU_ERR_ARG, "verify_sample: vocab %d, row strides %ld and %ld", vocab, ldp, ldd);
     if (n_req > 0x7FFFFFFF / VER_CL) return dsv4cu_set_error(DSV4CU_ERR_ARG, "verify_sample: %d requests", n_req);
     if (nt > 0 && (!p || !u)) return dsv4cu_set_error(DSV4CU_ERR_ARG, "verify_sample: NULL probabilities");

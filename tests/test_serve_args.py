@@ -147,3 +147,11 @@ def test_verify_refuses_slots_and_shapes(L, ctx):
     s = lambda p=P, ldp=8, d=None, ldd=0, u=P, vocab=8: L.dsv4cu_verify_sample(  # noqa: E731
         ctx, P, P, P, P, P, P, p, ldp, d, ldd, u, vocab, None, None, 1, 1, None)
     assert s(p=None) == s(ldp=7) == s(d=P, ldd=7) == s(u=None) == s(vocab=0) == ARG
+
+
+def test_row_numbers_and_vocabularies_past_32_bits_are_refused(L, ctx):
+    a = _tree(n_heads=1 << 24, n_kv=1, nt=1, max_nodes=128, ldq=1 << 30, ldo=1 << 30)
+    assert L.dsv4cu_tree_attn(ctx, C.byref(a), None) == ARG and b"128 nodes" in L.dsv4cu_last_error()
+    assert L.dsv4cu_tree_attn_workspace(ctx, C.byref(a)) == 0
+    v = (1 << 30) + 1
+    assert L.dsv4cu_verify_sample(ctx, P, P, P, P, P, P, P, v, None, 0, P, v, None, None, 1, 1, None) == ARG
