@@ -38,9 +38,10 @@
 // value row is multiplied by a weight of exactly 0, which is only harmless
 // when the value is finite: 0 x infinity and 0 x NaN are NaN. So a tile whose
 // output is not finite looks (sa_suspect) for a non-finite value behind a mask
-// - with three weight terms, whose last ones may be 0, also for a visible
-// infinity - and if there is one, serve_slow_rows computes the tile again from
-// visible keys only. Rows outside a sequence and pages outside the pool are
+// - where a visible weight may also be 0 in 16 bits though it is not (the last
+// of three terms, an f16 weight below 2^-25), also for a visible infinity, of
+// keys too, whose queries have terms - and if there is one, serve_slow_rows
+// computes the tile again from visible keys only. Rows outside a sequence and pages outside the pool are
 // zeros in shared memory and are masked.
 #pragma once
 
@@ -275,8 +276,9 @@ DSV4CU_DEV float sa_inv(float l, float m, const float *sink, int head)
 
 // Whether a value of the tile's blocks could have made its output non-finite
 // against the mask: a value that is not finite in a block that a mask crosses
-// (full(block) false), or with ALL an infinite one anywhere. This thread's share
-// of the keys; rows are read from memory, D / 8 pieces each.
+// (full(block) false), or with ALL an infinite one anywhere, of the keys as
+// well. This thread's share of the keys; rows are read from memory, D / 8
+// pieces each.
 template <int D, bool F16, bool ALL, class Full, class Row>
 DSV4CU_DEV bool sa_suspect(const SaTile &t, int BN, int thread, int threads, Full full, Row row)
 {
@@ -287,14 +289,17 @@ DSV4CU_DEV bool sa_suspect(const SaTile &t, int BN, int thread, int threads, Ful
         if (!masked && !ALL) continue;
         for (int x = thread; x < BN * (D / 8); x += threads) {
             const int j = x / (D / 8);
-            const uint16_t *v = row(blk, j, true);
-            if (!v) continue;
-            const uint4 w = __ldg(reinterpret_cast<const uint4 *>(v + (x - j * (D / 8)) * 8));
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (masked) found = found || sa_nonfinite<F16>(u[e]);
-                else found = found || (u[e] & (E | M)) == E || ((u[e] >> 16) & (E | M)) == E;
+            for (int kv = ALL ? 0 : 1; kv < 2; kv++) {
+                const uint16_t *v = row(blk, j, kv == 1);
+                if (!v) continue;
+                const uint4 w = __ldg(reinterpret_cast<const uint4 *>(v + (x - j * (D / 8)) * 8));
+                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if (masked && kv == 1) found = found || sa_nonfinite<F16>(u[e]);
+                    else found = found || (u[e] & (E | M)) == E || ((u[e] >> 16) & (E | M)) == E;
+                }
             }
         }
     }
@@ -795,6 +800,9 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
         }
         __syncthreads();                                 // this stage, the weights and s_alpha are free
     }
+    // no copy is on its way any more when the stages are written over
+    for (int blk = max(t.blk0, t.blk1 - 2); !arrives && blk < t.blk1; blk++)
+        sa_poll(&s_full[(blk - t.blk0) & 1], ((blk - t.blk0) >> 1) & 1, a.status, SA_COPY);
     bool done = false;
     {
         bool odd = false;
@@ -805,7 +813,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
 #pragma unroll
                 for (int e = 0; e < 4; e++) odd = odd || (16 * mt + g + 8 * (e >> 1) < t.rows && !isfinite(o[mt][n][e]));
         if (__syncthreads_or(odd) &&
-            __syncthreads_or(sa_suspect<D, F16, (TERMS > 1)>(t, BN, tid, THREADS, is_full, row))) {
+            __syncthreads_or(sa_suspect<D, F16, (TERMS > 1 || F16)>(t, BN, tid, THREADS, is_full, row))) {
             serve_slow_rows<D, F16, QF32>(a, t, BN, warp, NW, vis, row);
             done = true;
         }

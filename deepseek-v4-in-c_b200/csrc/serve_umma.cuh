@@ -792,7 +792,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
                 ts.blk1 = end;
             }
             const int threads = alt ? 256 : 128, thread = alt ? threadIdx.x - 128 : i;
-            if (sa_suspect<D, F16, false>(ts, BN, thread, threads, is_full, row_of)) s_odd[who] = 2;
+            if (sa_suspect<D, F16, F16>(ts, BN, thread, threads, is_full, row_of)) s_odd[who] = 2;
             alt ? su_bar<256>(1) : su_bar<128>(2 + s);
             if (s_odd[who] == 2) serve_slow_rows<D, F16, false>(a, ts, BN, thread >> 5, threads >> 5, sees, row_of);
         }

@@ -118,6 +118,24 @@ def test_prompt_nonfinite_values_stay_behind_the_mask(dev, kind, dim):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_prompt_visible_infinities(dev, kind, dim):
+    """A key of -inf where every query is positive weighs nothing; an infinite value behind a small weight stays one."""
+    import torch
+
+    def edit(q, k, v):
+        q[:, :, 0] = 1.5                                   # one term: the others of fp32 queries are 0
+        k[3, :, 0] = float("-inf")
+        k[100, 1, 0] = float("-inf")
+        k[70, :, 1:] = 0.0
+        k[70, :, 0] = -25.0 * dim ** 0.5                   # score -37.5, weight about 2^-54
+        v[70, 0, 5], v[70, 1, 9] = float("inf"), float("-inf")
+
+    o = _prompt(dev, [170, 90], 4, 2, dim, kind, edit=edit)
+    assert bool(torch.isinf(o[80, 0, 5])) and bool(torch.isfinite(o[80, 0, 6])) and bool(torch.isfinite(o[30]).all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_prompt_large_scores(dev, kind):
     """Scores in the hundreds: the running maximum moves often, weights underflow to 0."""
     def edit(q, k, v):
