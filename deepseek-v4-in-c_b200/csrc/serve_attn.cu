@@ -180,6 +180,7 @@ extern "C" int dsv4cu_prompt_attn(dsv4cu_ctx *ctx, const dsv4cu_prompt_attn_args
     DSV4CU_CUDA_TRY(guard.enter(ctx->device));
     SaArgs s = fill_common(c, a->cu, a->sink);
     s.status = ctx->status;
+    s.sms = ctx->sm_count;
     return serve_attn_run(s, c, false, use_umma(c), (cudaStream_t)stream);
 }
 

@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
     t.ctx = t.kend = t.key0 = t.nblk_c = t.split = 0;
     t.parts = 1;
     t.table = nullptr;
-    t.kvh = blockIdx.y;
+    t.kvh = !TREE && a.heads_first ? blockIdx.x : blockIdx.y;
     if constexpr (TREE) {
         const int b = blockIdx.z;
         const SaSpan sp = sa_span(a, b, BN);
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
         t.blk1 = min(sp.nblk, t.blk0 + sp.per);
     } else {
         int tile;
-        sa_find(a.cu, a.n_req, a.nt, a.G, rows_cta, gridDim.x - 1 - blockIdx.x, t.begin, t.len, tile);
+        sa_find(a, rows_cta, t.begin, t.len, tile);
         if (t.begin < 0) return;
         t.r0 = tile * rows_cta;
     }
@@ -855,7 +855,7 @@ int serve_umma_launch(SaArgs a, bool tree, cudaStream_t st)
         a.two = 1;
         const int64_t tiles = (int64_t)a.nt * a.G / 256 + min(a.n_req, a.nt);
         if (tiles > INT_MAX) return dsv4cu_set_error(DSV4CU_ERR_ARG, "prompt_attn: %lld row tiles", (long long)tiles);
-        grid = dim3((unsigned)tiles, a.hkv, 1);
+        grid = sa_prompt_grid(a, tiles, a.sms * S::CTAS);
     }
     // as many stages as fit: 227 KB for one CTA; half of the SM's 228 KB less
     // the 1 KB that each CTA costs for two
