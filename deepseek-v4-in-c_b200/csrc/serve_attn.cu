@@ -61,7 +61,7 @@ static SaArgs fill_common(const Common &c, const int *cu, const float *sink)
     s.nt = c.nt;
     s.hq = c.n_heads;
     s.hkv = c.n_kv;
-    s.G = c.n_heads / c.n_kv;
+    sa_set_group(s, c.n_heads / c.n_kv);
     s.window = c.window ? c.window : INT_MAX;
     s.scale2 = c.scale * SA_LOG2E;
     s.splits = 1;

@@ -63,6 +63,7 @@ struct SaArgs {
     long ldq, ldk, ldv, ldo;          // elements between tokens
     const int *cu;                    // [n_req + 1]
     int n_req, nt, hq, hkv, G;
+    unsigned g_mul, g_shift;          // x / G for 0 <= x < 2^31: sa_token
     int window;                       // keys a row may look back over, INT_MAX: all
     float scale2;                     // scale * log2 e
     // tree
@@ -77,6 +78,17 @@ struct SaArgs {
     int sms, heads_first;             // prompts: SMs, order of the grid (sa_prompt_grid)
     int nst, two, box_log2;           // tcgen05 kernel: stages, two strips of rows per CTA, rows of a cached copy's box
 };
+
+// Token of a request's row: row / G, by a multiplication (Granlund and
+// Montgomery 1994; m = g_mul below 2^32, rows below 2^31, so the sum fits).
+static inline void sa_set_group(SaArgs &a, int G)
+{
+    a.G = G;
+    a.g_shift = 0;
+    while ((1ll << a.g_shift) < G) a.g_shift++;
+    a.g_mul = (unsigned)((((1ull << a.g_shift) - (unsigned)G) << 32) / (unsigned)G + 1);
+}
+DSV4CU_DEV int sa_token(const SaArgs &a, int row) { return (int)((__umulhi((unsigned)row, a.g_mul) + (unsigned)row) >> a.g_shift); }
 
 // The key blocks of request b of a tree call: blocks of BN cached keys from
 // key0 on (no row looks further back than the shallowest one, at position
@@ -383,7 +395,7 @@ __device__ __noinline__ void serve_slow_rows(const SaArgs &a, const SaTile &t, i
     const int lane = threadIdx.x & 31;
     constexpr int E = D / 32;
     for (int r = warp; r < t.rows; r += warps) {
-        const int tok = (t.r0 + r) / a.G, head = t.kvh * a.G + (t.r0 + r) % a.G;
+        const int tok = sa_token(a, t.r0 + r), head = t.kvh * a.G + t.r0 + r - tok * a.G;
         const size_t qat = (size_t)(t.begin + tok) * a.ldq + (size_t)head * D;
         float m = -INFINITY, l = 0.0f, o[E];
 #pragma unroll
@@ -451,7 +463,7 @@ DSV4CU_DEV void sa_join(const SaArgs &a, const SaTile &t, float *sm, int tid, in
     float *inv = sm + parts * rows;
     float *ls = inv + rows;                              // [parts][rows]
     for (int x = tid; x < parts * rows; x += threads) {
-        const int p = x / rows, r = x - p * rows, pr = t.r0 + r, tok = pr / a.G, head = t.kvh * a.G + pr - tok * a.G;
+        const int p = x / rows, r = x - p * rows, pr = t.r0 + r, tok = sa_token(a, pr), head = t.kvh * a.G + pr - tok * a.G;
         const size_t id = (size_t)(t.begin + tok) * a.hq + head + p * step;
         sm[x] = __ldcg(a.pm + id);
         ls[x] = __ldcg(a.pl + id);
@@ -469,7 +481,7 @@ DSV4CU_DEV void sa_join(const SaArgs &a, const SaTile &t, float *sm, int tid, in
             sm[s * rows + r] = f;
             if (f != 0.0f) l = fmaf(ls[s * rows + r], f, l);   // factor 0: a split without a visible key
         }
-        inv[r] = sa_inv(l, m, a.sink, t.kvh * a.G + (t.r0 + r) % a.G);
+        inv[r] = sa_inv(l, m, a.sink, t.kvh * a.G + t.r0 + r - sa_token(a, t.r0 + r) * a.G);
     }
     sync();
     constexpr int B = 8;                                 // splits read at once, of two pieces each
@@ -481,7 +493,7 @@ DSV4CU_DEV void sa_join(const SaArgs &a, const SaTile &t, float *sm, int tid, in
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const int x = min(x0 + u * threads, rows * (D / 4) - 1);   // the last piece twice where there is no second
-            const int r = x / (D / 4), c = (x - r * (D / 4)) * 4, pr = t.r0 + r, tok = pr / a.G,
+            const int r = x / (D / 4), c = (x - r * (D / 4)) * 4, pr = t.r0 + r, tok = sa_token(a, pr),
                       head = t.kvh * a.G + pr - tok * a.G;
             o[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             row[u] = r;
@@ -585,7 +597,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
     }
     t.rows = min(BM, t.len * a.G - t.r0);
     if (t.rows <= 0) return;
-    const int t_lo = t.r0 / a.G, t_hi = (t.r0 + t.rows - 1) / a.G;
+    const int t_lo = sa_token(a, t.r0), t_hi = sa_token(a, t.r0 + t.rows - 1);
     if constexpr (!TREE) {
         t.key0 = a.window > t_lo ? 0 : t_lo - a.window + 1;   // blocks start at the first key of the window
         t.blk0 = 0;
@@ -690,7 +702,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
     for (int mt = 0; mt < 2; mt++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int r = 16 * mt + g + 8 * h, pr = t.r0 + min(r, t.rows - 1), tok = pr / a.G, head = t.kvh * a.G + pr % a.G;
+            const int r = 16 * mt + g + 8 * h, pr = t.r0 + min(r, t.rows - 1), tok = sa_token(a, pr), head = t.kvh * a.G + pr - tok * a.G;
             const size_t at = (size_t)(t.begin + tok) * a.ldq + (size_t)head * D + DW * warp + 2 * c;
 #pragma unroll
             for (int kk = 0; kk < KS; kk++)
@@ -714,7 +726,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
     const int brow = (lane & 7) + 8 * (lane >> 4), bcol = 8 * ((lane >> 3) & 1);
     const int d0 = DW * warp;
     const bool second = t.rows > 16;                     // rows 16 .. 31 exist
-    const int srow = tid / TPR, scol = (tid % TPR) * CPT, stok = (t.r0 + min(srow, t.rows - 1)) / a.G;
+    const int srow = tid / TPR, scol = (tid % TPR) * CPT, stok = sa_token(a, t.r0 + min(srow, t.rows - 1));
     float o[2][ON][4];
 #pragma unroll
     for (int mt = 0; mt < 2; mt++)
@@ -899,10 +911,10 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
                     *reinterpret_cast<float2 *>(ob + (16 * mt + g + 8 * h) * OS + d0 + 8 * n + 2 * c) =
                         make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
         if (tid < t.rows) {
-            const int head = t.kvh * a.G + (t.r0 + tid) % a.G;
+            const int tok = sa_token(a, t.r0 + tid), head = t.kvh * a.G + t.r0 + tid - tok * a.G;
             s_alpha[tid] = in_parts ? 1.0f : sa_inv(s_l[tid], s_m[tid], a.sink, head);
             if (in_parts) {
-                const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + (t.r0 + tid) / a.G) * a.hq + head;
+                const size_t id = (size_t)t.split * a.nt * a.hq + (size_t)(t.begin + tok) * a.hq + head;
                 a.pm[id] = s_m[tid];
                 a.pl[id] = s_l[tid];
             }
@@ -910,7 +922,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
     }
     __syncthreads();
     for (int x = tid; x < (done ? 0 : t.rows * (D / 8)); x += THREADS) {
-        const int r = x / (D / 8), col = (x - r * (D / 8)) * 8, pr = t.r0 + r, tok = pr / a.G,
+        const int r = x / (D / 8), col = (x - r * (D / 8)) * 8, pr = t.r0 + r, tok = sa_token(a, pr),
                   head = t.kvh * a.G + pr - tok * a.G;
         const float f = s_alpha[r];
         float4 y = *reinterpret_cast<const float4 *>(ob + r * OS + col), z = *reinterpret_cast<const float4 *>(ob + r * OS + col + 4);

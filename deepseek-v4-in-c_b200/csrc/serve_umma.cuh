@@ -254,21 +254,21 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
     }
     t.rows = min(rows_cta, t.len * a.G - t.r0);
     if (t.rows <= 0) return;
-    const int tok_end = (t.r0 + t.rows - 1) / a.G;       // the CTA's last token
+    const int tok_end = sa_token(a, t.r0 + t.rows - 1);       // the CTA's last token
     const bool alt = t.rows <= 128;                      // one strip: even and odd blocks
     if constexpr (!TREE) {                               // blocks start at the first key of the window
-        const int tok = t.r0 / a.G;
+        const int tok = sa_token(a, t.r0);
         t.key0 = a.window > tok ? 0 : tok - a.window + 1;
     }
     // strip s: rows [row0, row0 + n), key blocks from `first` to `end` by `step`
     auto strip_first = [&](int s) {
         if constexpr (TREE) return t.blk0 + (alt ? s : 0);
-        const int tok = (t.r0 + (alt ? 0 : 128 * s)) / a.G, lo = a.window > tok ? 0 : tok - a.window + 1;
+        const int tok = sa_token(a, t.r0 + (alt ? 0 : 128 * s)), lo = a.window > tok ? 0 : tok - a.window + 1;
         return (lo - t.key0) / BN + (alt ? s : 0);
     };
     auto strip_end = [&](int s) {
         if constexpr (TREE) return t.blk1;
-        return ((alt || s ? tok_end : (t.r0 + 127) / a.G) - t.key0) / BN + 1;
+        return ((alt || s ? tok_end : sa_token(a, t.r0 + 127)) - t.key0) / BN + 1;
     };
     const int f0 = strip_first(0), f1 = strip_first(1), e0 = strip_end(0), e1 = strip_end(1), step = alt ? 2 : 1;
     if constexpr (!TREE) {
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
             const int x = q_i + e * q_n, r = x / (D / 8), ch = x - r * (D / 8);
             qw[e] = make_uint4(0, 0, 0, 0);
             if (r < n) {
-                const int pr = t.r0 + 128 * q_s + r, tok = pr / a.G, head = t.kvh * a.G + pr - tok * a.G;
+                const int pr = t.r0 + 128 * q_s + r, tok = sa_token(a, pr), head = t.kvh * a.G + pr - tok * a.G;
                 qw[e] = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) +
                                                               (size_t)(t.begin + tok) * a.ldq + (size_t)head * D + 8 * ch));
             }
@@ -497,8 +497,8 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
         }
         const int first = s ? f1 : f0, end = s ? e1 : e0;
         const bool live = 32 * (warp & 3) < rows;        // this warp has rows
-        const int pr = t.r0 + row0 + min(i, max(0, rows - 1)), tok = pr / a.G, head = t.kvh * a.G + pr - tok * a.G;
-        const int tok_lo = (t.r0 + row0) / a.G, tok_hi = (t.r0 + row0 + rows - 1) / a.G;
+        const int pr = t.r0 + row0 + min(i, max(0, rows - 1)), tok = sa_token(a, pr), head = t.kvh * a.G + pr - tok * a.G;
+        const int tok_lo = sa_token(a, t.r0 + row0), tok_hi = sa_token(a, t.r0 + row0 + rows - 1);
         const int depth = TREE ? s_depth[tok] : 0;
         const uint32_t quarter = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t sp_s = tm_s + BN * s + quarter, sp_o = tm_o + D * s + quarter;
