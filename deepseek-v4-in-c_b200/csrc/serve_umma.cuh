@@ -120,6 +120,17 @@ DSV4CU_DEV void su_loaded32(uint32_t *r)
 DSV4CU_DEV void su_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 template <int N>
 DSV4CU_DEV void su_bar(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory"); }
+template <int N>
+DSV4CU_DEV void su_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(N) : "memory"); }
+// The same with an OR over the threads.
+template <int N>
+DSV4CU_DEV int su_bar_or(int id, int x)
+{
+    int r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"(x), "r"(id), "n"(N) : "memory");
+    return r;
+}
 template <int R>
 DSV4CU_DEV void su_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R)); }
 template <int R>
@@ -277,539 +288,546 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
     }
     const int c0 = f0, c1 = e1;                          // all blocks of the CTA: the second strip ends last
 
-    // The softmax warps' queries are on their way while the rest is set up:
-    // strip s by its own warps, a single strip by all.
-    constexpr int QN = D / 8;                            // 16-byte pieces of a thread
-    uint4 qw[QN];
-    const int q_s = alt ? 0 : (warp - 4) >> 2, q_n = alt ? 256 : 128, q_i = (threadIdx.x - 128) & (q_n - 1);
-    if (warp >= 4) {
-        const int n = min(128, t.rows - 128 * q_s);
-#pragma unroll
-        for (int e = 0; e < QN; e++) {
-            const int x = q_i + e * q_n, r = x / (D / 8), ch = x - r * (D / 8);
-            qw[e] = make_uint4(0, 0, 0, 0);
-            if (r < n) {
-                const int pr = t.r0 + 128 * q_s + r, tok = sa_token(a, pr), head = t.kvh * a.G + pr - tok * a.G;
-                qw[e] = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) +
-                                                              (size_t)(t.begin + tok) * a.ldq + (size_t)head * D + 8 * ch));
+    if (warp == 0) {
+        // the copies start as soon as their barriers are set up
+        if (lane == 0) {
+            sh.t = t;
+            for (int s = 0; s < SU_MAX_STAGES; s++) {
+                mbar_init(&kfull[s], 1);
+                mbar_init(&kempty[s], 1);
+                mbar_init(&vfull[s], 1);
+                mbar_init(&vempty[s], 1);
             }
-        }
-    }
-    if (threadIdx.x == 0) {
-        sh.t = t;
-        for (int s = 0; s < SU_MAX_STAGES; s++) {
-            mbar_init(&kfull[s], 1);
-            mbar_init(&kempty[s], 1);
-            mbar_init(&vfull[s], 1);
-            mbar_init(&vempty[s], 1);
-        }
-        for (int s = 0; s < 2; s++) {
-            mbar_init(&sfull[s], 1);
-            mbar_init(&pfull[s], 4);
-            mbar_init(&ofull[s], 1);
-            s_odd[s] = 0;
-        }
-        mbar_init(&qfull, 8);
-        mbar_init(&drain, 1);
-        fence_mbar_init();
-    }
-    if (warp == 1) {
-        umma::tmem_alloc(&sh.tmem, TM_COLS);
-        umma::tmem_relinquish();
-    }
-    int lost = 0;                                        // a page of these blocks is not in the pool
-    if constexpr (TREE) {
-        const int k_lo = t.key0 + t.blk0 * BN, k_hi = min(t.kend, t.key0 + min(t.blk1, t.nblk_c) * BN);
-        if (k_lo < k_hi)
-            for (int pg = k_lo / a.page_size + threadIdx.x; pg <= (k_hi - 1) / a.page_size; pg += SU_THREADS) {
-                const int id = __ldg(t.table + pg);
-                lost |= id < 0 || id >= a.n_pages;
+            for (int s = 0; s < 2; s++) {
+                mbar_init(&sfull[s], 1);
+                mbar_init(&pfull[s], 4);
+                mbar_init(&ofull[s], 1);
+                s_odd[s] = 0;
             }
-        for (int i = threadIdx.x; i < t.len; i += SU_THREADS) sh.par[i] = (int16_t)max(-1, min(__ldg(a.parent + t.begin + i), SA_MAX_NODES));
-    }
-    umma::fence_before();
-    lost = __syncthreads_or(lost);
-    umma::fence_after();
-    if constexpr (TREE) {
-        for (int i = threadIdx.x; i < t.len; i += SU_THREADS) {
-            uint32_t set[4] = {0, 0, 0, 0};
-            int d = -1, x = i;
-            for (;;) {
-#pragma unroll
-                for (int w = 0; w < 4; w++) set[w] |= (x >> 5) == w ? 1u << (x & 31) : 0u;
-                d++;
-                const int p = sh.par[x];
-                if (p < 0 || p >= x) break;
-                x = p;
-            }
-#pragma unroll
-            for (int w = 0; w < 4; w++) s_anc[i][w] = set[w];
-            s_depth[i] = (uint8_t)d;
+            mbar_init(&qfull, 8);
+            mbar_init(&drain, 1);
+            fence_mbar_init();
         }
-        __syncthreads();
-    }
-    const uint32_t tmem = sh.tmem;
-    const uint32_t tm_s = tmem, tm_o = tmem + 2 * BN;    // strip s: S at + BN s, O at + D s
-
-    if (warp < 4) {
+        __syncwarp();
+        su_arrive<SU_THREADS>(4);
         su_regs_dec<SuShape<D>::FEW>();
-        if (warp == 0) {
-            // ------------------------------------------------ copies
-            const int boxes = TREE ? BN >> a.box_log2 : 1;
-            bool ok = true;
-            int n = 0;
-            for (int b = c0; b < c1 && ok; b++, n++) {
-                const int st = n % a.nst, u = n / a.nst;
-                const bool cached = TREE && b < t.nblk_c;
-                int row = 0;
-                bool mine = lane == 0;
-                if (cached) {
-                    const int key = t.key0 + b * BN + (lane << a.box_log2);
-                    mine = lane < boxes && key < t.kend;
-                    if (mine) {
-                        const int pg = key >> a.page_log2, id = __ldg(t.table + pg);
-                        mine = id >= 0 && id < a.n_pages;
-                        row = id * a.page_size + (key - (pg << a.page_log2));
-                    }
-                } else {
-                    row = t.begin + (TREE ? (b - t.nblk_c) * BN : t.key0 + b * BN);
+        // ------------------------------------------------ copies
+        const int boxes = TREE ? BN >> a.box_log2 : 1;
+        bool ok = true;
+        int n = 0;
+        for (int b = c0; b < c1 && ok; b++, n++) {
+            const int st = n % a.nst, u = n / a.nst;
+            const bool cached = TREE && b < t.nblk_c;
+            int row = 0;
+            bool mine = lane == 0;
+            if (cached) {
+                const int key = t.key0 + b * BN + (lane << a.box_log2);
+                mine = lane < boxes && key < t.kend;
+                if (mine) {
+                    const int pg = key >> a.page_log2, id = __ldg(t.table + pg);
+                    mine = id >= 0 && id < a.n_pages;
+                    row = id * a.page_size + (key - (pg << a.page_log2));
                 }
-                const unsigned go = __ballot_sync(0xFFFFFFFFu, mine);
-                const uint32_t off = cached ? (uint32_t)lane << (a.box_log2 + 7) : 0u;   // this box's first row
-                const uint32_t bytes = cached ? (uint32_t)__popc(go) * DC << (a.box_log2 + 7) : (uint32_t)KVB;
-#pragma unroll
-                for (int kv = 0; kv < 2; kv++) {
-                    uint64_t *full = kv ? &vfull[st] : &kfull[st], *empty = kv ? &vempty[st] : &kempty[st];
-                    if (lane == 0 && u > 0) ok = sa_poll(empty, (u - 1) & 1, a.status, kv ? SUE_VEMPTY : SUE_KEMPTY);
-                    ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
-                    if (!ok) break;
-                    if (lane == 0) mbar_arrive_expect_tx(full, bytes);
-                    __syncwarp();
-                    uint8_t *dst = (kv ? vs : ks) + st * KVB + off;
-                    const CUtensorMap *map = cached ? (kv ? &mvc : &mkc) : (kv ? &mv : &mk);
-                    if (mine)
-#pragma unroll
-                        for (int c = 0; c < DC; c++) su_tma(dst + c * KSUB, map, 64 * c, t.kvh, row, full);
-                }
+            } else {
+                row = t.begin + (TREE ? (b - t.nblk_c) * BN : t.key0 + b * BN);
             }
-            // every issued copy lands before the CTA can exit
-            if (lane == 0)
-                for (int j = max(0, n - a.nst); j < n; j++) {
-                    mbar_wait(&kfull[j % a.nst], (j / a.nst) & 1, nullptr, 0);
-                    mbar_wait(&vfull[j % a.nst], (j / a.nst) & 1, nullptr, 0);
-                }
-        } else if (warp == 1) {
-            // ------------------------------------------------ products
-            // The whole warp walks the blocks and one elected lane issues: what
-            // the instructions take comes from warp-uniform values (broadcast
-            // once), so descriptors stay in uniform registers. Issued by a lone
-            // lane, moving them there took longer than the products.
-            constexpr uint32_t id_s = su_idesc(F16, BN, false), id_o = su_idesc(F16, D, true);
-            auto same = [](int x) { return __shfl_sync(0xFFFFFFFFu, x, 0); };
-            const bool one = su_elect();
-            const int u0 = same(c0), u1 = same(c1), g0 = same(f0), g1 = same(f1), h0 = same(e0), h1 = same(e1);
-            const int nst = a.nst;
-            const bool ualt = same(alt) != 0;
-            const int ustep = ualt ? 2 : 1;
-            const uint32_t ts = (uint32_t)same((int)tm_s), to = (uint32_t)same((int)tm_o);
-            // operand descriptors: the address field counts 16 bytes, and shared
-            // memory ends before it overflows
-            const uint64_t dq = umma::desc_sw128(qs), dk = umma::desc_sw128(ks), dv = su_desc_v(vs, KSUB);
-            uint32_t once = 0;                           // blocks that one of their two strips has scored
-            bool ok = sa_poll(&qfull, 0, a.status, SUE_Q);
-            umma::fence_after();
-            // scores of strip s against block b: its key stage and phase
-            auto scores = [&](int s, int b) {
-                const int n = b - u0, use = n / nst, st = n - use * nst;
-                ok = ok && sa_poll(&kfull[st], use & 1, a.status, SUE_KFULL);
-                if (!ok) return;
-                umma::fence_after();
-                const uint64_t q = dq + (uint32_t)((ualt ? 0 : s) * (QB >> 4)), k = dk + (uint32_t)(st * (KVB >> 4));
-                const uint32_t bit = 1u << (b & 31);
-                const bool both = !ualt && b >= g1 && b < h0;    // two strips read this block
-                const bool last = !both || (once & bit);
-                once = both && !last ? once | bit : once & ~bit;
-                if (one) {
+            const unsigned go = __ballot_sync(0xFFFFFFFFu, mine);
+            const uint32_t off = cached ? (uint32_t)lane << (a.box_log2 + 7) : 0u;   // this box's first row
+            const uint32_t bytes = cached ? (uint32_t)__popc(go) * DC << (a.box_log2 + 7) : (uint32_t)KVB;
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; kk++) {
-                        su_mma(ts + BN * s, q + (((kk >> 2) * SU_SUB + 32 * (kk & 3)) >> 4),
-                               k + (((kk >> 2) * KSUB + 32 * (kk & 3)) >> 4), id_s, kk > 0);
-                    }
-                    umma::commit(&sfull[s]);
-                    if (last) umma::commit(&kempty[st]);
-                }
+            for (int kv = 0; kv < 2; kv++) {
+                uint64_t *full = kv ? &vfull[st] : &kfull[st], *empty = kv ? &vempty[st] : &kempty[st];
+                if (lane == 0 && u > 0) ok = sa_poll(empty, (u - 1) & 1, a.status, kv ? SUE_VEMPTY : SUE_KEMPTY);
+                ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_expect_tx(full, bytes);
                 __syncwarp();
-            };
-            if (g0 < h0) scores(0, g0);
-            if (g1 < h1) scores(1, g1);
-            uint32_t turn[2] = {0, 0};
-            int st = 0, phase = 0;
-            for (int b = u0; b < u1 && ok; b++) {
+                uint8_t *dst = (kv ? vs : ks) + st * KVB + off;
+                const CUtensorMap *map = cached ? (kv ? &mvc : &mkc) : (kv ? &mv : &mk);
+                if (mine)
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    if (ualt ? ((b - u0) & 1) != s : s ? b < g1 : b >= h0) continue;   // strip 0 ends first, strip 1 starts last
-                    ok = ok && sa_poll(&pfull[s], turn[s] & 1, a.status, SUE_P) &&
-                         sa_poll(&vfull[st], phase, a.status, SUE_VFULL);
-                    ok = __all_sync(0xFFFFFFFFu, ok);
-                    if (!ok) break;
-                    umma::fence_after();
-                    const uint64_t v = dv + (uint32_t)(st * (KVB >> 4));
-                    const uint32_t more = turn[s] > 0;
-                    const bool last = s == 1 || ualt || b < g1;  // strip 1 comes second
-                    if (one) {
-#pragma unroll
-                        for (int kk = 0; kk < BN / 16; kk++)
-                            su_mma_ta(to + D * s, ts + BN * s + 8 * kk, v + (2048 >> 4) * kk, id_o, kk > 0 ? 1u : more);
-                        if (last) umma::commit(&vempty[st]);
-                    }
-                    __syncwarp();
-                    turn[s]++;
-                    if (b + ustep < (s ? h1 : h0)) scores(s, b + ustep);
-                    else if (one) umma::commit(&ofull[s]);
-                }
-                if (++st == nst) {
-                    st = 0;
-                    phase ^= 1;
-                }
+                    for (int c = 0; c < DC; c++) su_tma(dst + c * KSUB, map, 64 * c, t.kvh, row, full);
             }
-            // the products in flight complete before TMEM is released
-            if (one) {
-                umma::commit(&drain);
-                mbar_wait(&drain, 0, a.status, SUE_DRAIN);
-            }
-            __syncwarp();
         }
+        // every issued copy lands before the CTA can exit
+        if (lane == 0)
+            for (int j = max(0, n - a.nst); j < n; j++) {
+                mbar_wait(&kfull[j % a.nst], (j / a.nst) & 1, nullptr, 0);
+                mbar_wait(&vfull[j % a.nst], (j / a.nst) & 1, nullptr, 0);
+            }
     } else {
-        su_regs_inc<SuShape<D>::MANY>();
-        // ------------------------------------------------ softmax
-        const int s = (warp - 4) >> 2, i = (threadIdx.x - 128) & 127;    // strip; row, and key in prepared values
-        const int row0 = alt ? 0 : 128 * s, rows = min(128, t.rows - row0);
-        {
-            uint8_t *q = qs + (alt ? 0 : s) * QB;
+        // The softmax warps' queries are on their way while the rest is set up:
+        // strip s by its own warps, a single strip by all.
+        constexpr int QN = D / 8;                            // 16-byte pieces of a thread
+        uint4 qw[QN];
+        const int q_s = alt ? 0 : (warp - 4) >> 2, q_n = alt ? 256 : 128, q_i = (threadIdx.x - 128) & (q_n - 1);
+        if (warp >= 4) {
+            const int n = min(128, t.rows - 128 * q_s);
 #pragma unroll
             for (int e = 0; e < QN; e++) {
                 const int x = q_i + e * q_n, r = x / (D / 8), ch = x - r * (D / 8);
-                if (r < 128) *reinterpret_cast<uint4 *>(q + (ch >> 3) * SU_SUB + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = qw[e];
+                qw[e] = make_uint4(0, 0, 0, 0);
+                if (r < n) {
+                    const int pr = t.r0 + 128 * q_s + r, tok = sa_token(a, pr), head = t.kvh * a.G + pr - tok * a.G;
+                    qw[e] = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) +
+                                                                  (size_t)(t.begin + tok) * a.ldq + (size_t)head * D + 8 * ch));
+                }
             }
-            sa_fence_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&qfull);
         }
-        const int first = s ? f1 : f0, end = s ? e1 : e0;
-        const bool live = 32 * (warp & 3) < rows;        // this warp has rows
-        const int pr = t.r0 + row0 + min(i, max(0, rows - 1)), tok = sa_token(a, pr), head = t.kvh * a.G + pr - tok * a.G;
-        const int tok_lo = sa_token(a, t.r0 + row0), tok_hi = sa_token(a, t.r0 + row0 + rows - 1);
-        const int depth = TREE ? s_depth[tok] : 0;
-        const uint32_t quarter = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t sp_s = tm_s + BN * s + quarter, sp_o = tm_o + D * s + quarter;
-        float m = -INFINITY, l = 0.0f;
-        uint32_t turn = 0;
-        bool ok = true;
-        // blocks full_lo .. full_hi - 1 are crossed by no mask (missing pages aside)
-        int full_lo, full_hi;
+        if (warp == 1) {
+            umma::tmem_alloc(&sh.tmem, TM_COLS);
+            umma::tmem_relinquish();
+        }
+        int lost = 0;                                        // a page of these blocks is not in the pool
         if constexpr (TREE) {
-            const int back = t.ctx + t.len - a.window;   // no key below this is in every row's window
-            full_lo = back <= t.key0 ? 0 : (back - t.key0 + BN - 1) / BN;
-            full_hi = (t.kend - t.key0) / BN;         // at least 0 where there are cached blocks
-        } else {
-            const int back = tok_hi - a.window + 1 - t.key0;
-            full_lo = back <= 0 ? 0 : (back + BN - 1) / BN;
-            full_hi = (tok_lo + 1 - t.key0) / BN;
+            const int k_lo = t.key0 + t.blk0 * BN, k_hi = min(t.kend, t.key0 + min(t.blk1, t.nblk_c) * BN);
+            if (k_lo < k_hi)
+                for (int pg = k_lo / a.page_size + threadIdx.x - 32; pg <= (k_hi - 1) / a.page_size; pg += SU_THREADS - 32) {
+                    const int id = __ldg(t.table + pg);
+                    lost |= id < 0 || id >= a.n_pages;
+                }
+            for (int i = threadIdx.x - 32; i < t.len; i += SU_THREADS - 32) sh.par[i] = (int16_t)max(-1, min(__ldg(a.parent + t.begin + i), SA_MAX_NODES));
         }
-        auto is_full = [full_lo, full_hi](int b) { return b >= full_lo && b < full_hi; };
-        const SaTile *tp = &sh.t;
-        auto in_pool = [&](int key) {
-            if (key >= tp->kend) return false;
-            const int id = __ldg(tp->table + (key >> a.page_log2));
-            return id >= 0 && id < a.n_pages;
-        };
-        for (int b = first; b < end; b += step, turn++) {
-            // ---- the mask
-            const bool masked = !is_full(b) || (TREE && lost);
-            constexpr int W = BN / 32;                   // mask words of a block
-            uint32_t vis[W];
-            ok = __all_sync(0xFFFFFFFFu, sa_poll(&sfull[s], turn & 1, a.status, SUE_S));
-            if (!ok) break;
-            const bool cached = TREE && b < tp->nblk_c;
-            const int base = TREE && !cached ? (b - tp->nblk_c) * BN : tp->key0 + b * BN;
-            // keys that are not there: behind the sequence, the nodes or the
-            // cache, or on a missing page
-            if (masked && (cached ? lost || base + BN > tp->kend : base + BN > tp->len)) {
-                // values of absent keys become zeros (what the copies left, or
-                // brought from the next sequence, may be no number). Behind
-                // this block's scores lie the products of every block before
-                // it, so the stage's last use is over and its barrier is at
-                // most one phase away: the parity below means this block.
-                const int n = b - c0, st = n % a.nst;
-                ok = __all_sync(0xFFFFFFFFu, sa_poll(&vfull[st], (n / a.nst) & 1, a.status, SUE_VFULL));
-                if (!ok) break;
-                if (i < BN && !(cached ? in_pool(base + i) : base + i < tp->len)) {
-                    uint8_t *v = vs + st * KVB + i * 128;
+        umma::fence_before();
+        su_bar<SU_THREADS>(4);                          // the barriers are set up, TMEM is there
+        if constexpr (TREE) lost = su_bar_or<SU_THREADS - 32>(5, lost);
+        umma::fence_after();
+        if constexpr (TREE) {
+            for (int i = threadIdx.x - 32; i < t.len; i += SU_THREADS - 32) {
+                uint32_t set[4] = {0, 0, 0, 0};
+                int d = -1, x = i;
+                for (;;) {
 #pragma unroll
-                    for (int c = 0; c < DC; c++)
+                    for (int w = 0; w < 4; w++) set[w] |= (x >> 5) == w ? 1u << (x & 31) : 0u;
+                    d++;
+                    const int p = sh.par[x];
+                    if (p < 0 || p >= x) break;
+                    x = p;
+                }
 #pragma unroll
-                        for (int x = 0; x < 8; x++) *reinterpret_cast<uint4 *>(v + c * KSUB + 16 * x) = make_uint4(0, 0, 0, 0);
+                for (int w = 0; w < 4; w++) s_anc[i][w] = set[w];
+                s_depth[i] = (uint8_t)d;
+            }
+            su_bar<SU_THREADS - 32>(5);
+        }
+        const uint32_t tmem = sh.tmem;
+        const uint32_t tm_s = tmem, tm_o = tmem + 2 * BN;    // strip s: S at + BN s, O at + D s
+
+        if (warp < 4) {
+            su_regs_dec<SuShape<D>::FEW>();
+            if (warp == 1) {
+                // ------------------------------------------------ products
+                // The whole warp walks the blocks and one elected lane issues: what
+                // the instructions take comes from warp-uniform values (broadcast
+                // once), so descriptors stay in uniform registers. Issued by a lone
+                // lane, moving them there took longer than the products.
+                constexpr uint32_t id_s = su_idesc(F16, BN, false), id_o = su_idesc(F16, D, true);
+                auto same = [](int x) { return __shfl_sync(0xFFFFFFFFu, x, 0); };
+                const bool one = su_elect();
+                const int u0 = same(c0), u1 = same(c1), g0 = same(f0), g1 = same(f1), h0 = same(e0), h1 = same(e1);
+                const int nst = a.nst;
+                const bool ualt = same(alt) != 0;
+                const int ustep = ualt ? 2 : 1;
+                const uint32_t ts = (uint32_t)same((int)tm_s), to = (uint32_t)same((int)tm_o);
+                // operand descriptors: the address field counts 16 bytes, and shared
+                // memory ends before it overflows
+                const uint64_t dq = umma::desc_sw128(qs), dk = umma::desc_sw128(ks), dv = su_desc_v(vs, KSUB);
+                uint32_t once = 0;                           // blocks that one of their two strips has scored
+                bool ok = sa_poll(&qfull, 0, a.status, SUE_Q);
+                umma::fence_after();
+                // scores of strip s against block b: its key stage and phase
+                auto scores = [&](int s, int b) {
+                    const int n = b - u0, use = n / nst, st = n - use * nst;
+                    ok = ok && sa_poll(&kfull[st], use & 1, a.status, SUE_KFULL);
+                    if (!ok) return;
+                    umma::fence_after();
+                    const uint64_t q = dq + (uint32_t)((ualt ? 0 : s) * (QB >> 4)), k = dk + (uint32_t)(st * (KVB >> 4));
+                    const uint32_t bit = 1u << (b & 31);
+                    const bool both = !ualt && b >= g1 && b < h0;    // two strips read this block
+                    const bool last = !both || (once & bit);
+                    once = both && !last ? once | bit : once & ~bit;
+                    if (one) {
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; kk++) {
+                            su_mma(ts + BN * s, q + (((kk >> 2) * SU_SUB + 32 * (kk & 3)) >> 4),
+                                   k + (((kk >> 2) * KSUB + 32 * (kk & 3)) >> 4), id_s, kk > 0);
+                        }
+                        umma::commit(&sfull[s]);
+                        if (last) umma::commit(&kempty[st]);
+                    }
+                    __syncwarp();
+                };
+                if (g0 < h0) scores(0, g0);
+                if (g1 < h1) scores(1, g1);
+                uint32_t turn[2] = {0, 0};
+                int st = 0, phase = 0;
+                for (int b = u0; b < u1 && ok; b++) {
+#pragma unroll
+                    for (int s = 0; s < 2; s++) {
+                        if (ualt ? ((b - u0) & 1) != s : s ? b < g1 : b >= h0) continue;   // strip 0 ends first, strip 1 starts last
+                        ok = ok && sa_poll(&pfull[s], turn[s] & 1, a.status, SUE_P) &&
+                             sa_poll(&vfull[st], phase, a.status, SUE_VFULL);
+                        ok = __all_sync(0xFFFFFFFFu, ok);
+                        if (!ok) break;
+                        umma::fence_after();
+                        const uint64_t v = dv + (uint32_t)(st * (KVB >> 4));
+                        const uint32_t more = turn[s] > 0;
+                        const bool last = s == 1 || ualt || b < g1;  // strip 1 comes second
+                        if (one) {
+#pragma unroll
+                            for (int kk = 0; kk < BN / 16; kk++)
+                                su_mma_ta(to + D * s, ts + BN * s + 8 * kk, v + (2048 >> 4) * kk, id_o, kk > 0 ? 1u : more);
+                            if (last) umma::commit(&vempty[st]);
+                        }
+                        __syncwarp();
+                        turn[s]++;
+                        if (b + ustep < (s ? h1 : h0)) scores(s, b + ustep);
+                        else if (one) umma::commit(&ofull[s]);
+                    }
+                    if (++st == nst) {
+                        st = 0;
+                        phase ^= 1;
+                    }
+                }
+                // the products in flight complete before TMEM is released
+                if (one) {
+                    umma::commit(&drain);
+                    mbar_wait(&drain, 0, a.status, SUE_DRAIN);
+                }
+                __syncwarp();
+            }
+        } else {
+            su_regs_inc<SuShape<D>::MANY>();
+            // ------------------------------------------------ softmax
+            const int s = (warp - 4) >> 2, i = (threadIdx.x - 128) & 127;    // strip; row, and key in prepared values
+            const int row0 = alt ? 0 : 128 * s, rows = min(128, t.rows - row0);
+            {
+                uint8_t *q = qs + (alt ? 0 : s) * QB;
+#pragma unroll
+                for (int e = 0; e < QN; e++) {
+                    const int x = q_i + e * q_n, r = x / (D / 8), ch = x - r * (D / 8);
+                    if (r < 128) *reinterpret_cast<uint4 *>(q + (ch >> 3) * SU_SUB + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = qw[e];
                 }
                 sa_fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&qfull);
             }
-            if (masked) {
-                if (cached) {
-                    const int pos = tp->ctx + depth, lo = a.window > pos ? 0 : pos - a.window + 1 - base;
+            const int first = s ? f1 : f0, end = s ? e1 : e0;
+            const bool live = 32 * (warp & 3) < rows;        // this warp has rows
+            const int pr = t.r0 + row0 + min(i, max(0, rows - 1)), tok = sa_token(a, pr), head = t.kvh * a.G + pr - tok * a.G;
+            const int tok_lo = sa_token(a, t.r0 + row0), tok_hi = sa_token(a, t.r0 + row0 + rows - 1);
+            const int depth = TREE ? s_depth[tok] : 0;
+            const uint32_t quarter = (uint32_t)(32 * (warp & 3)) << 16;
+            const uint32_t sp_s = tm_s + BN * s + quarter, sp_o = tm_o + D * s + quarter;
+            float m = -INFINITY, l = 0.0f;
+            uint32_t turn = 0;
+            bool ok = true;
+            // blocks full_lo .. full_hi - 1 are crossed by no mask (missing pages aside)
+            int full_lo, full_hi;
+            if constexpr (TREE) {
+                const int back = t.ctx + t.len - a.window;   // no key below this is in every row's window
+                full_lo = back <= t.key0 ? 0 : (back - t.key0 + BN - 1) / BN;
+                full_hi = (t.kend - t.key0) / BN;         // at least 0 where there are cached blocks
+            } else {
+                const int back = tok_hi - a.window + 1 - t.key0;
+                full_lo = back <= 0 ? 0 : (back + BN - 1) / BN;
+                full_hi = (tok_lo + 1 - t.key0) / BN;
+            }
+            auto is_full = [full_lo, full_hi](int b) { return b >= full_lo && b < full_hi; };
+            const SaTile *tp = &sh.t;
+            auto in_pool = [&](int key) {
+                if (key >= tp->kend) return false;
+                const int id = __ldg(tp->table + (key >> a.page_log2));
+                return id >= 0 && id < a.n_pages;
+            };
+            for (int b = first; b < end; b += step, turn++) {
+                // ---- the mask
+                const bool masked = !is_full(b) || (TREE && lost);
+                constexpr int W = BN / 32;                   // mask words of a block
+                uint32_t vis[W];
+                ok = __all_sync(0xFFFFFFFFu, sa_poll(&sfull[s], turn & 1, a.status, SUE_S));
+                if (!ok) break;
+                const bool cached = TREE && b < tp->nblk_c;
+                const int base = TREE && !cached ? (b - tp->nblk_c) * BN : tp->key0 + b * BN;
+                // keys that are not there: behind the sequence, the nodes or the
+                // cache, or on a missing page
+                if (masked && (cached ? lost || base + BN > tp->kend : base + BN > tp->len)) {
+                    // values of absent keys become zeros (what the copies left, or
+                    // brought from the next sequence, may be no number). Behind
+                    // this block's scores lie the products of every block before
+                    // it, so the stage's last use is over and its barrier is at
+                    // most one phase away: the parity below means this block.
+                    const int n = b - c0, st = n % a.nst;
+                    ok = __all_sync(0xFFFFFFFFu, sa_poll(&vfull[st], (n / a.nst) & 1, a.status, SUE_VFULL));
+                    if (!ok) break;
+                    if (i < BN && !(cached ? in_pool(base + i) : base + i < tp->len)) {
+                        uint8_t *v = vs + st * KVB + i * 128;
 #pragma unroll
-                    for (int w = 0; w < W; w++) {
-                        vis[w] = su_range(lo, tp->kend - 1 - base, w);
-                        if (lost) vis[w] &= __ballot_sync(0xFFFFFFFFu, in_pool(base + 32 * w + lane));
+                        for (int c = 0; c < DC; c++)
+#pragma unroll
+                            for (int x = 0; x < 8; x++) *reinterpret_cast<uint4 *>(v + c * KSUB + 16 * x) = make_uint4(0, 0, 0, 0);
                     }
-                } else if (TREE) {
-#pragma unroll
-                    for (int w = 0; w < W; w++) vis[w] = s_anc[tok][base / 32 + w];
-                    if (depth >= a.window)
-                        for (int x = base; x < min(tp->len, base + BN); x++)
-                            if (depth - s_depth[x] >= a.window) {
-#pragma unroll
-                                for (int w = 0; w < W; w++) vis[w] &= (x - base) >> 5 == w ? ~(1u << (x & 31)) : ~0u;
-                            }
-                } else {
-                    const int lo = a.window > tok ? 0 : tok - a.window + 1 - base;
-#pragma unroll
-                    for (int w = 0; w < W; w++) vis[w] = su_range(lo, tok - base, w);
+                    sa_fence_async();
                 }
-            }
-            if (live) {
-                umma::fence_after();
-                uint32_t x[BN];
-#pragma unroll
-                for (int c = 0; c < BN / 32; c++) su_ld32(sp_s + 32 * c, x + 32 * c);
-                su_wait_ld();
-#pragma unroll
-                for (int c = 0; c < BN / 32; c++) su_loaded32(x + 32 * c);
                 if (masked) {
+                    if (cached) {
+                        const int pos = tp->ctx + depth, lo = a.window > pos ? 0 : pos - a.window + 1 - base;
 #pragma unroll
-                    for (int k = 0; k < BN; k++)
-                        if (!((vis[k >> 5] >> (k & 31)) & 1u)) x[k] = 0xFF800000u;
+                        for (int w = 0; w < W; w++) {
+                            vis[w] = su_range(lo, tp->kend - 1 - base, w);
+                            if (lost) vis[w] &= __ballot_sync(0xFFFFFFFFu, in_pool(base + 32 * w + lane));
+                        }
+                    } else if (TREE) {
+#pragma unroll
+                        for (int w = 0; w < W; w++) vis[w] = s_anc[tok][base / 32 + w];
+                        if (depth >= a.window)
+                            for (int x = base; x < min(tp->len, base + BN); x++)
+                                if (depth - s_depth[x] >= a.window) {
+#pragma unroll
+                                    for (int w = 0; w < W; w++) vis[w] &= (x - base) >> 5 == w ? ~(1u << (x & 31)) : ~0u;
+                                }
+                    } else {
+                        const int lo = a.window > tok ? 0 : tok - a.window + 1 - base;
+#pragma unroll
+                        for (int w = 0; w < W; w++) vis[w] = su_range(lo, tok - base, w);
+                    }
                 }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (live) {
+                    umma::fence_after();
+                    uint32_t x[BN];
 #pragma unroll
-                for (int k = 0; k < BN; k += 8)
+                    for (int c = 0; c < BN / 32; c++) su_ld32(sp_s + 32 * c, x + 32 * c);
+                    su_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        top[e] = su_max3(top[e], __uint_as_float(x[k + 2 * e]), __uint_as_float(x[k + 2 * e + 1]));
-                float mrow = su_max3(su_max3(top[0], top[1], top[2]), top[3], top[3]) * a.scale2;
-                if (mrow == INFINITY) mrow = __uint_as_float(0x7FC00000u);   // inf - inf: the row is NaN, as NaN scores make it
-                const bool move = !(mrow <= m + SU_LAZY);
-                if (__any_sync(0xFFFFFFFFu, move)) {
-                    const float to = move ? mrow : m, alpha = move ? sa_exp2(m - to) : 1.0f;
-                    m = to;
-                    l *= alpha;
-                    if (turn > 0) {                      // the products so far are complete: S came behind them
+                    for (int c = 0; c < BN / 32; c++) su_loaded32(x + 32 * c);
+                    if (masked) {
+#pragma unroll
+                        for (int k = 0; k < BN; k++)
+                            if (!((vis[k >> 5] >> (k & 31)) & 1u)) x[k] = 0xFF800000u;
+                    }
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int k = 0; k < BN; k += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            top[e] = su_max3(top[e], __uint_as_float(x[k + 2 * e]), __uint_as_float(x[k + 2 * e + 1]));
+                    float mrow = su_max3(su_max3(top[0], top[1], top[2]), top[3], top[3]) * a.scale2;
+                    if (mrow == INFINITY) mrow = __uint_as_float(0x7FC00000u);   // inf - inf: the row is NaN, as NaN scores make it
+                    const bool move = !(mrow <= m + SU_LAZY);
+                    if (__any_sync(0xFFFFFFFFu, move)) {
+                        const float to = move ? mrow : m, alpha = move ? sa_exp2(m - to) : 1.0f;
+                        m = to;
+                        l *= alpha;
+                        if (turn > 0) {                      // the products so far are complete: S came behind them
 #pragma unroll 2
-                        for (int c = 0; c < D; c += 16) {    // few columns at a time: the scores stay in registers
-                            uint32_t o[16];
-                            su_ld16(sp_o + c, o);
+                            for (int c = 0; c < D; c += 16) {    // few columns at a time: the scores stay in registers
+                                uint32_t o[16];
+                                su_ld16(sp_o + c, o);
 #pragma unroll
-                            for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-                            su_st16(sp_o + c, o);
+                                for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                                su_st16(sp_o + c, o);
+                            }
+                        }
+                    }
+                    const float use = m == -INFINITY ? 0.0f : m;
+                    const uint64_t scale2 = su_f2(a.scale2, a.scale2), shift2 = su_f2(-use, -use);
+                    uint64_t sum[2] = {su_f2(l, 0.0f), su_f2(0.0f, 0.0f)};
+#pragma unroll
+                    for (int c = 0; c < BN / 32; c++) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int k = 0; k < 16; k++) {
+                            float p, q;
+                            su_unf2(su_fma2(su_u2(x[32 * c + 2 * k], x[32 * c + 2 * k + 1]), scale2, shift2), p, q);
+                            p = sa_exp2(p);
+                            q = sa_exp2(q);
+                            sum[k & 1] = su_add2(sum[k & 1], su_f2(p, q));
+                            w[k] = sa_pack<F16>(p, q);
+                        }
+                        su_st16(sp_s + 16 * c, w);
+                    }
+                    float s0, s1;
+                    su_unf2(su_add2(sum[0], sum[1]), s0, s1);
+                    l = s0 + s1;
+                    su_wait_st();
+                    umma::fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pfull[s]);
+            }
+            // ---- outputs
+            const bool any = first < end;
+            if (any) ok = ok && __all_sync(0xFFFFFFFFu, sa_poll(&ofull[s], 0, a.status, SUE_O));
+            umma::fence_after();
+            const SaArgs &a0 = a;
+            auto row_of = [tp, ap = &a0](int blk, int j, bool values) -> const uint16_t * {
+                const SaArgs &a = *ap;
+                const SaTile &t = *tp;
+                const bool vv = values && a.v != nullptr;
+                if (TREE && blk < t.nblk_c) {
+                    const int key = t.key0 + blk * BN + j;
+                    return key < t.kend ? sa_cached(a, t, vv ? a.vc : a.kc, key, D) : nullptr;
+                }
+                const int key = TREE ? (blk - t.nblk_c) * BN + j : t.key0 + blk * BN + j;
+                if (key >= t.len) return nullptr;
+                return reinterpret_cast<const uint16_t *>(vv ? a.v : a.k) + (size_t)(t.begin + key) * (vv ? a.ldv : a.ldk) +
+                       (size_t)t.kvh * D;
+            };
+            auto sees = [tp, row_of, ap = &a0, dp = s_depth, an = s_anc](int tok, int blk, int j) -> bool {
+                const SaArgs &a = *ap;
+                const SaTile &t = *tp;
+                if constexpr (TREE) {
+                    if (blk < t.nblk_c) {
+                        const int key = t.key0 + blk * BN + j;
+                        return key < t.kend && t.ctx - key + dp[tok] < a.window && row_of(blk, j, false) != nullptr;
+                    }
+                    const int x = (blk - t.nblk_c) * BN + j;
+                    return x < t.len && (an[tok][x >> 5] >> (x & 31) & 1) && dp[tok] - dp[x] < a.window;
+                } else {
+                    const int key = t.key0 + blk * BN + j;
+                    return key <= tok && tok - key < a.window;
+                }
+            };
+            // A warp's rows go out through its own part of the shared memory that
+            // the products are done with, so that stores cover whole rows. With two
+            // strips that is the strip's queries; a single strip first adds its
+            // even and odd blocks: each half of the columns is finished by one
+            // strip's warps, which get the other strip's share of it through xch.
+            constexpr int PN = D == 128 ? 16 : 8;            // 16-byte pieces of a row per pass
+            constexpr int XN = D / 8;                        // 16-byte pieces of half a row of floats
+            constexpr int XH = 128 * XN * 16;                // bytes of one strip's share
+            static_assert(2 * XH + 8 * PN * 512 <= 2 * 2 * KVB || 2 * XH + 8 * PN * 512 <= 2 * SU_MAX_STAGES * KVB, "stages");
+            uint8_t *out = alt ? ks + 2 * XH + (warp - 4) * (PN * 512) : qs + s * QB + (warp & 3) * (PN * 512);
+            float f_own = 1.0f;
+            const int col0 = alt ? s * (D / 2) : 0, ncol = alt ? D / 2 : D;
+            if (alt) {
+                float2 *ml = reinterpret_cast<float2 *>(ks + 2 * XH);
+                su_bar<256>(1);                              // both strips' products are complete: the stages are free
+                ml[128 * s + i] = make_float2(m, l);
+                su_bar<256>(1);
+                const float2 other = ml[128 * (s ^ 1) + i];
+                const float top = m != m || other.x != other.x ? m + other.x : fmaxf(m, other.x);
+                const float use = top == -INFINITY ? 0.0f : top;
+                f_own = sa_exp2(m - use);
+                l = l * f_own + other.y * sa_exp2(other.x - use);
+                m = top;
+                if (live) {
+                    uint8_t *x = ks + (s ^ 1) * XH + i * (XN * 16);
+                    for (int c = 0; c < D / 2; c += 16) {
+                        uint32_t o[16];
+                        if (any) su_ld16(sp_o + (s ^ 1) * (D / 2) + c, o);
+#pragma unroll
+                        for (int k = 0; k < 16; k += 4) {
+                            float y[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) y[e] = any ? __uint_as_float(o[k + e]) * f_own : 0.0f;
+                            *reinterpret_cast<float4 *>(x + ((((c + k) >> 2) ^ (i & 7)) << 4)) = make_float4(y[0], y[1], y[2], y[3]);
                         }
                     }
                 }
-                const float use = m == -INFINITY ? 0.0f : m;
-                const uint64_t scale2 = su_f2(a.scale2, a.scale2), shift2 = su_f2(-use, -use);
-                uint64_t sum[2] = {su_f2(l, 0.0f), su_f2(0.0f, 0.0f)};
+                su_bar<256>(1);
+            }
+            bool odd = false;
+            if (live) {
+                const bool part = t.parts > 1;
+                const float inv = part ? 1.0f : sa_inv(l, m, a.sink, head);
+                const size_t row_id = (size_t)(t.begin + tok) * a.hq + head;
+                const size_t id = (size_t)t.split * a.nt * a.hq + row_id;
+                if (part && i < rows && (!alt || s == 0)) {
+                    a.pm[id] = m;
+                    a.pl[id] = l;
+                }
+                char *dst = part ? reinterpret_cast<char *>(a.po + id * D + col0)
+                                 : reinterpret_cast<char *>(reinterpret_cast<uint16_t *>(a.o) + (size_t)(t.begin + tok) * a.ldo +
+                                                            (size_t)head * D + col0);
+                const uint8_t *x = ks + s * XH + i * (XN * 16);
+                const int mine = min(32, rows - 32 * (warp & 3));    // rows of this warp
+                int piece = 0;                               // of the pass
+                for (int c = 0; c < ncol; c += 16) {         // a loop: its code is cold at every launch
+                    uint32_t o[16];
+                    if (any) su_ld16(sp_o + col0 + c, o);
+                    float y[16];
 #pragma unroll
-                for (int c = 0; c < BN / 32; c++) {
-                    uint32_t w[16];
+                    for (int k = 0; k < 16; k++) y[k] = any ? __uint_as_float(o[k]) * f_own : 0.0f;
+                    if (alt)
+#pragma unroll
+                        for (int k = 0; k < 16; k += 4) {
+                            const float4 z = *reinterpret_cast<const float4 *>(x + ((((c + k) >> 2) ^ (i & 7)) << 4));
+                            y[k] += z.x;
+                            y[k + 1] += z.y;
+                            y[k + 2] += z.z;
+                            y[k + 3] += z.w;
+                        }
 #pragma unroll
                     for (int k = 0; k < 16; k++) {
-                        float p, q;
-                        su_unf2(su_fma2(su_u2(x[32 * c + 2 * k], x[32 * c + 2 * k + 1]), scale2, shift2), p, q);
-                        p = sa_exp2(p);
-                        q = sa_exp2(q);
-                        sum[k & 1] = su_add2(sum[k & 1], su_f2(p, q));
-                        w[k] = sa_pack<F16>(p, q);
+                        odd = odd || !isfinite(y[k]);
+                        y[k] *= inv;
                     }
-                    su_st16(sp_s + 16 * c, w);
-                }
-                float s0, s1;
-                su_unf2(su_add2(sum[0], sum[1]), s0, s1);
-                l = s0 + s1;
-                su_wait_st();
-                umma::fence_before();
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&pfull[s]);
-        }
-        // ---- outputs
-        const bool any = first < end;
-        if (any) ok = ok && __all_sync(0xFFFFFFFFu, sa_poll(&ofull[s], 0, a.status, SUE_O));
-        umma::fence_after();
-        const SaArgs &a0 = a;
-        auto row_of = [tp, ap = &a0](int blk, int j, bool values) -> const uint16_t * {
-            const SaArgs &a = *ap;
-            const SaTile &t = *tp;
-            const bool vv = values && a.v != nullptr;
-            if (TREE && blk < t.nblk_c) {
-                const int key = t.key0 + blk * BN + j;
-                return key < t.kend ? sa_cached(a, t, vv ? a.vc : a.kc, key, D) : nullptr;
-            }
-            const int key = TREE ? (blk - t.nblk_c) * BN + j : t.key0 + blk * BN + j;
-            if (key >= t.len) return nullptr;
-            return reinterpret_cast<const uint16_t *>(vv ? a.v : a.k) + (size_t)(t.begin + key) * (vv ? a.ldv : a.ldk) +
-                   (size_t)t.kvh * D;
-        };
-        auto sees = [tp, row_of, ap = &a0, dp = s_depth, an = s_anc](int tok, int blk, int j) -> bool {
-            const SaArgs &a = *ap;
-            const SaTile &t = *tp;
-            if constexpr (TREE) {
-                if (blk < t.nblk_c) {
-                    const int key = t.key0 + blk * BN + j;
-                    return key < t.kend && t.ctx - key + dp[tok] < a.window && row_of(blk, j, false) != nullptr;
-                }
-                const int x = (blk - t.nblk_c) * BN + j;
-                return x < t.len && (an[tok][x >> 5] >> (x & 31) & 1) && dp[tok] - dp[x] < a.window;
-            } else {
-                const int key = t.key0 + blk * BN + j;
-                return key <= tok && tok - key < a.window;
-            }
-        };
-        // A warp's rows go out through its own part of the shared memory that
-        // the products are done with, so that stores cover whole rows. With two
-        // strips that is the strip's queries; a single strip first adds its
-        // even and odd blocks: each half of the columns is finished by one
-        // strip's warps, which get the other strip's share of it through xch.
-        constexpr int PN = D == 128 ? 16 : 8;            // 16-byte pieces of a row per pass
-        constexpr int XN = D / 8;                        // 16-byte pieces of half a row of floats
-        constexpr int XH = 128 * XN * 16;                // bytes of one strip's share
-        static_assert(2 * XH + 8 * PN * 512 <= 2 * 2 * KVB || 2 * XH + 8 * PN * 512 <= 2 * SU_MAX_STAGES * KVB, "stages");
-        uint8_t *out = alt ? ks + 2 * XH + (warp - 4) * (PN * 512) : qs + s * QB + (warp & 3) * (PN * 512);
-        float f_own = 1.0f;
-        const int col0 = alt ? s * (D / 2) : 0, ncol = alt ? D / 2 : D;
-        if (alt) {
-            float2 *ml = reinterpret_cast<float2 *>(ks + 2 * XH);
-            su_bar<256>(1);                              // both strips' products are complete: the stages are free
-            ml[128 * s + i] = make_float2(m, l);
-            su_bar<256>(1);
-            const float2 other = ml[128 * (s ^ 1) + i];
-            const float top = m != m || other.x != other.x ? m + other.x : fmaxf(m, other.x);
-            const float use = top == -INFINITY ? 0.0f : top;
-            f_own = sa_exp2(m - use);
-            l = l * f_own + other.y * sa_exp2(other.x - use);
-            m = top;
-            if (live) {
-                uint8_t *x = ks + (s ^ 1) * XH + i * (XN * 16);
-                for (int c = 0; c < D / 2; c += 16) {
-                    uint32_t o[16];
-                    if (any) su_ld16(sp_o + (s ^ 1) * (D / 2) + c, o);
+                    uint8_t *w = out + lane * (PN * 16);
+                    if (part) {
 #pragma unroll
-                    for (int k = 0; k < 16; k += 4) {
-                        float y[4];
+                        for (int k = 0; k < 16; k += 4)
+                            *reinterpret_cast<float4 *>(w + (((piece + k / 4) ^ (lane & 7)) << 4)) =
+                                make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]);
+                        piece += 4;
+                    } else {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) y[e] = any ? __uint_as_float(o[k + e]) * f_own : 0.0f;
-                        *reinterpret_cast<float4 *>(x + ((((c + k) >> 2) ^ (i & 7)) << 4)) = make_float4(y[0], y[1], y[2], y[3]);
+                        for (int k = 0; k < 16; k += 8)
+                            *reinterpret_cast<uint4 *>(w + (((piece + k / 8) ^ (lane & 7)) << 4)) =
+                                make_uint4(sa_pack<F16>(y[k], y[k + 1]), sa_pack<F16>(y[k + 2], y[k + 3]),
+                                           sa_pack<F16>(y[k + 4], y[k + 5]), sa_pack<F16>(y[k + 6], y[k + 7]));
+                        piece += 2;
                     }
-                }
-            }
-            su_bar<256>(1);
-        }
-        bool odd = false;
-        if (live) {
-            const bool part = t.parts > 1;
-            const float inv = part ? 1.0f : sa_inv(l, m, a.sink, head);
-            const size_t row_id = (size_t)(t.begin + tok) * a.hq + head;
-            const size_t id = (size_t)t.split * a.nt * a.hq + row_id;
-            if (part && i < rows && (!alt || s == 0)) {
-                a.pm[id] = m;
-                a.pl[id] = l;
-            }
-            char *dst = part ? reinterpret_cast<char *>(a.po + id * D + col0)
-                             : reinterpret_cast<char *>(reinterpret_cast<uint16_t *>(a.o) + (size_t)(t.begin + tok) * a.ldo +
-                                                        (size_t)head * D + col0);
-            const uint8_t *x = ks + s * XH + i * (XN * 16);
-            const int mine = min(32, rows - 32 * (warp & 3));    // rows of this warp
-            int piece = 0;                               // of the pass
-            for (int c = 0; c < ncol; c += 16) {         // a loop: its code is cold at every launch
-                uint32_t o[16];
-                if (any) su_ld16(sp_o + col0 + c, o);
-                float y[16];
-#pragma unroll
-                for (int k = 0; k < 16; k++) y[k] = any ? __uint_as_float(o[k]) * f_own : 0.0f;
-                if (alt)
-#pragma unroll
-                    for (int k = 0; k < 16; k += 4) {
-                        const float4 z = *reinterpret_cast<const float4 *>(x + ((((c + k) >> 2) ^ (i & 7)) << 4));
-                        y[k] += z.x;
-                        y[k + 1] += z.y;
-                        y[k + 2] += z.z;
-                        y[k + 3] += z.w;
-                    }
-#pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    odd = odd || !isfinite(y[k]);
-                    y[k] *= inv;
-                }
-                uint8_t *w = out + lane * (PN * 16);
-                if (part) {
-#pragma unroll
-                    for (int k = 0; k < 16; k += 4)
-                        *reinterpret_cast<float4 *>(w + (((piece + k / 4) ^ (lane & 7)) << 4)) =
-                            make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]);
-                    piece += 4;
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 16; k += 8)
-                        *reinterpret_cast<uint4 *>(w + (((piece + k / 8) ^ (lane & 7)) << 4)) =
-                            make_uint4(sa_pack<F16>(y[k], y[k + 1]), sa_pack<F16>(y[k + 2], y[k + 3]),
-                                       sa_pack<F16>(y[k + 4], y[k + 5]), sa_pack<F16>(y[k + 6], y[k + 7]));
-                    piece += 2;
-                }
-                if (piece == PN || c + 16 >= ncol) {     // the pass is full: 2^b pieces per row
-                    const int b = 31 - __clz(piece);
-                    __syncwarp();
+                    if (piece == PN || c + 16 >= ncol) {     // the pass is full: 2^b pieces per row
+                        const int b = 31 - __clz(piece);
+                        __syncwarp();
 #pragma unroll 4
-                    for (int e = 0; e < (mine << b); e += 32) {
-                        const int r = (e + lane) >> b, pc = (e + lane) & (piece - 1);
-                        char *d = reinterpret_cast<char *>(__shfl_sync(0xFFFFFFFFu, (unsigned long long)dst, r & 31));
-                        if (r < mine)
-                            *reinterpret_cast<uint4 *>(d + 16 * pc) =
-                                *reinterpret_cast<const uint4 *>(out + r * (PN * 16) + ((pc ^ (r & 7)) << 4));
+                        for (int e = 0; e < (mine << b); e += 32) {
+                            const int r = (e + lane) >> b, pc = (e + lane) & (piece - 1);
+                            char *d = reinterpret_cast<char *>(__shfl_sync(0xFFFFFFFFu, (unsigned long long)dst, r & 31));
+                            if (r < mine)
+                                *reinterpret_cast<uint4 *>(d + 16 * pc) =
+                                    *reinterpret_cast<const uint4 *>(out + r * (PN * 16) + ((pc ^ (r & 7)) << 4));
+                        }
+                        __syncwarp();
+                        dst += 16 * piece;
+                        piece = 0;
                     }
-                    __syncwarp();
-                    dst += 16 * piece;
-                    piece = 0;
                 }
+                odd = odd && i < rows;
             }
-            odd = odd && i < rows;
-        }
-        // a row that is not finite: was it a value behind the mask?
-        const int who = alt ? 0 : s;
-        if (odd) s_odd[who] = 1;
-        alt ? su_bar<256>(1) : su_bar<128>(2 + s);
-        if (s_odd[who]) {
-            SaTile ts = t;
-            ts.r0 = t.r0 + row0;
-            ts.rows = rows;
-            if (!alt) {
-                ts.blk0 = first;
-                ts.blk1 = end;
-            }
-            const int threads = alt ? 256 : 128, thread = alt ? threadIdx.x - 128 : i;
-            if (sa_suspect<D, F16, F16>(ts, BN, thread, threads, is_full, row_of)) s_odd[who] = 2;
+            // a row that is not finite: was it a value behind the mask?
+            const int who = alt ? 0 : s;
+            if (odd) s_odd[who] = 1;
             alt ? su_bar<256>(1) : su_bar<128>(2 + s);
-            if (s_odd[who] == 2) serve_slow_rows<D, F16, false>(a, ts, BN, thread >> 5, threads >> 5, sees, row_of);
-        }
-        if (TREE && t.parts > 1) {
-            // the tile's last split to finish joins them all
-            __threadfence();
-            su_bar<256>(1);
-            if (threadIdx.x == 128) {
-                int *count = a.counters + ((size_t)blockIdx.z * a.hkv + t.kvh) * a.row_tiles + blockIdx.x % a.row_tiles;
-                const bool last = atomicAdd(count, 1) == t.parts - 1;
-                if (last) *count = 0;
-                s_odd[0] = last;
+            if (s_odd[who]) {
+                SaTile ts = t;
+                ts.r0 = t.r0 + row0;
+                ts.rows = rows;
+                if (!alt) {
+                    ts.blk0 = first;
+                    ts.blk1 = end;
+                }
+                const int threads = alt ? 256 : 128, thread = alt ? threadIdx.x - 128 : i;
+                if (sa_suspect<D, F16, F16>(ts, BN, thread, threads, is_full, row_of)) s_odd[who] = 2;
+                alt ? su_bar<256>(1) : su_bar<128>(2 + s);
+                if (s_odd[who] == 2) serve_slow_rows<D, F16, false>(a, ts, BN, thread >> 5, threads >> 5, sees, row_of);
             }
-            su_bar<256>(1);
-            if (s_odd[0]) {
+            if (TREE && t.parts > 1) {
+                // the tile's last split to finish joins them all
                 __threadfence();
-                sa_join<D, F16, false>(a, t, reinterpret_cast<float *>(ks), threadIdx.x - 128, 256, [] { su_bar<256>(1); });
+                su_bar<256>(1);
+                if (threadIdx.x == 128) {
+                    int *count = a.counters + ((size_t)blockIdx.z * a.hkv + t.kvh) * a.row_tiles + blockIdx.x % a.row_tiles;
+                    const bool last = atomicAdd(count, 1) == t.parts - 1;
+                    if (last) *count = 0;
+                    s_odd[0] = last;
+                }
+                su_bar<256>(1);
+                if (s_odd[0]) {
+                    __threadfence();
+                    sa_join<D, F16, false>(a, t, reinterpret_cast<float *>(ks), threadIdx.x - 128, 256, [] { su_bar<256>(1); });
+                }
             }
         }
     }
@@ -817,7 +835,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
     __syncthreads();
     if (warp == 1) {
         umma::fence_after();
-        umma::tmem_dealloc(tmem, TM_COLS);
+        umma::tmem_dealloc(sh.tmem, TM_COLS);
     }
 }
 
