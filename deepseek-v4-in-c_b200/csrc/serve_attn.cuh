@@ -224,7 +224,7 @@ struct SaTile {
 };
 
 // Sequence and tile of the prompt CTA number `id`. Sequence b has
-// ceil(len * G / BM) tiles, and a later tile has more keys: CTAs start in the
+// ceil(len * G / 2^LOG) tiles, and a later tile has more keys: CTAs start in the
 // order of falling tile numbers over all sequences, so the short ones fill the
 // end (29 prompts of 16001 tokens, 16 heads over 4, 64 dims: 75 us, sequence
 // after sequence 91 us). For that a warp holds the tile counts of up to
@@ -234,7 +234,55 @@ struct SaTile {
 // (301 tokens of 64 heads of 512 dims, window 128: 77 against 70 us). All lanes
 // of the warp return the same; begin < 0: no such tile.
 constexpr int SA_SORTED = 128, SA_EVEN = 1024;
-DSV4CU_DEV void sa_find(const SaArgs &a, int BM, int &begin, int &len, int &tile)
+// Tiles of 2^log rows of n tokens; n * G fits 31 bits.
+DSV4CU_DEV int sa_tiles(int n, int G, int log) { return (int)(((unsigned)(n * G) + (1u << log) - 1u) >> log); }
+template <int R, int LOG>
+DSV4CU_DEV void sa_find_sorted(const int *cu, int n_req, int nt, int G, int id, int &begin, int &len, int &tile)
+{
+    const int lane = threadIdx.x & 31;
+    int lo[R], n[R], tiles[R], most = 0;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int b = 32 * r + lane;
+        lo[r] = n[r] = tiles[r] = 0;
+        if (b < n_req) {
+            lo[r] = max(0, min(__ldg(cu + b), nt));
+            n[r] = max(lo[r], min(__ldg(cu + b + 1), nt)) - lo[r];
+            tiles[r] = sa_tiles(n[r], G, LOG);
+        }
+        most = max(most, tiles[r]);
+    }
+    // the least x such that the tiles numbered x or higher are at most id
+    int none = -1, x = __reduce_max_sync(0xFFFFFFFFu, most), before = 0;
+    while (x - none > 1) {
+        const int mid = (x + none) >> 1;
+        int c = 0;
+#pragma unroll
+        for (int r = 0; r < R; r++) c += max(0, tiles[r] - mid);
+        c = __reduce_add_sync(0xFFFFFFFFu, c);
+        if (c <= id) {
+            x = mid;
+            before = c;
+        } else {
+            none = mid;
+        }
+    }
+    tile = x - 1;
+    int at = id - before;                            // among the sequences with a tile of this number
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const bool has = tile >= 0 && tiles[r] > tile;
+        const unsigned m = __ballot_sync(0xFFFFFFFFu, has);
+        const unsigned hit = __ballot_sync(0xFFFFFFFFu, has && __popc(m & ((1u << lane) - 1u)) == at);
+        if (hit && begin < 0) {
+            begin = __shfl_sync(0xFFFFFFFFu, lo[r], __ffs(hit) - 1);
+            len = __shfl_sync(0xFFFFFFFFu, n[r], __ffs(hit) - 1);
+        }
+        at -= __popc(m);
+    }
+}
+template <int LOG>
+DSV4CU_DEV void sa_find(const SaArgs &a, int &begin, int &len, int &tile)
 {
     const int *cu = a.cu, n_req = a.n_req, nt = a.nt, G = a.G;
     int id = a.heads_first ? blockIdx.y : blockIdx.x;
@@ -242,47 +290,8 @@ DSV4CU_DEV void sa_find(const SaArgs &a, int BM, int &begin, int &len, int &tile
     begin = -1;
     len = tile = 0;
     if (n_req <= SA_SORTED && a.window > SA_EVEN) {
-        constexpr int R = SA_SORTED / 32;
-        int lo[R], n[R], tiles[R], most = 0;
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            const int b = 32 * r + lane;
-            lo[r] = n[r] = tiles[r] = 0;
-            if (b < n_req) {
-                lo[r] = max(0, min(__ldg(cu + b), nt));
-                n[r] = max(lo[r], min(__ldg(cu + b + 1), nt)) - lo[r];
-                tiles[r] = (int)(((int64_t)n[r] * G + BM - 1) / BM);
-            }
-            most = max(most, tiles[r]);
-        }
-        // the least x such that the tiles numbered x or higher are at most id
-        int none = -1, x = __reduce_max_sync(0xFFFFFFFFu, most), before = 0;
-        while (x - none > 1) {
-            const int mid = (x + none) >> 1;
-            int c = 0;
-#pragma unroll
-            for (int r = 0; r < R; r++) c += max(0, tiles[r] - mid);
-            c = __reduce_add_sync(0xFFFFFFFFu, c);
-            if (c <= id) {
-                x = mid;
-                before = c;
-            } else {
-                none = mid;
-            }
-        }
-        tile = x - 1;
-        int at = id - before;                            // among the sequences with a tile of this number
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            const bool has = tile >= 0 && tiles[r] > tile;
-            const unsigned m = __ballot_sync(0xFFFFFFFFu, has);
-            const unsigned hit = __ballot_sync(0xFFFFFFFFu, has && __popc(m & ((1u << lane) - 1u)) == at);
-            if (hit && begin < 0) {
-                begin = __shfl_sync(0xFFFFFFFFu, lo[r], __ffs(hit) - 1);
-                len = __shfl_sync(0xFFFFFFFFu, n[r], __ffs(hit) - 1);
-            }
-            at -= __popc(m);
-        }
+        if (n_req <= 32) sa_find_sorted<1, LOG>(cu, n_req, nt, G, id, begin, len, tile);
+        else sa_find_sorted<SA_SORTED / 32, LOG>(cu, n_req, nt, G, id, begin, len, tile);
         return;
     }
     id = (a.heads_first ? gridDim.y : gridDim.x) - 1 - id;
@@ -294,7 +303,7 @@ DSV4CU_DEV void sa_find(const SaArgs &a, int BM, int &begin, int &len, int &tile
             lo = max(0, min(__ldg(cu + b), nt));
             n = max(lo, min(__ldg(cu + b + 1), nt)) - lo;
         }
-        const int mine = (int)(((int64_t)n * G + BM - 1) / BM);
+        const int mine = sa_tiles(n, G, LOG);
         int pre = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -591,7 +600,8 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
         t.blk1 = min(sp.nblk, t.blk0 + sp.per);
     } else {
         int tile;
-        sa_find(a, BM, t.begin, t.len, tile);
+        sa_find<5>(a, t.begin, t.len, tile);
+        static_assert(BM == 32, "rows of a tile");
         if (t.begin < 0) return;
         t.r0 = tile * BM;
     }

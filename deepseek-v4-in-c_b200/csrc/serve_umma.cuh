@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
         t.blk1 = min(sp.nblk, t.blk0 + sp.per);
     } else {
         int tile;
-        sa_find(a, rows_cta, t.begin, t.len, tile);
+        sa_find<8>(a, t.begin, t.len, tile);             // prompts always have two strips
         if (t.begin < 0) return;
         t.r0 = tile * rows_cta;
     }
