@@ -109,7 +109,8 @@ DSV4CU_DEV SaSpan sa_span(const SaArgs &a, int b, int BN)
     s.key0 = first / BN * BN;
     s.nblk_c = max(0, s.kend - s.key0 + BN - 1) / BN;
     s.nblk = s.nblk_c + (s.len + BN - 1) / BN;
-    s.per = max(a.chunk, (s.nblk + a.splits - 1) / a.splits);
+    s.per = a.chunk;                                     // (nblk <= chunk * splits where max_ctx was right)
+    if ((int64_t)a.chunk * a.splits < s.nblk) s.per = (s.nblk + a.splits - 1) / a.splits;
     s.used = (s.nblk + s.per - 1) / s.per;
     return s;
 }
@@ -581,7 +582,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
     if constexpr (TREE) {
         const int b = blockIdx.z;
         const SaSpan sp = sa_span(a, b, BN);
-        t.split = blockIdx.x / a.row_tiles;
+        t.split = a.row_tiles == 1 ? blockIdx.x : blockIdx.x / a.row_tiles;
         t.begin = sp.begin;
         t.len = sp.len;
         if (t.len > a.max_nodes) {                       // refused whole: its rows are left as they were
@@ -590,7 +591,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
         }
         if (t.split >= sp.used) return;
         t.parts = sp.used;
-        t.r0 = blockIdx.x % a.row_tiles * BM;
+        t.r0 = (blockIdx.x - t.split * a.row_tiles) * BM;
         t.ctx = sp.ctx;
         t.kend = sp.kend;
         t.table = a.table + (size_t)b * a.max_pages;

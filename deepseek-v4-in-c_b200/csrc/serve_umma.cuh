@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
     if constexpr (TREE) {
         const int b = blockIdx.z;
         const SaSpan sp = sa_span(a, b, BN);
-        t.split = blockIdx.x / a.row_tiles;
+        t.split = a.row_tiles == 1 ? blockIdx.x : blockIdx.x / a.row_tiles;
         t.begin = sp.begin;
         t.len = sp.len;
         if (t.len > a.max_nodes) {
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
         }
         if (t.split >= sp.used) return;
         t.parts = sp.used;
-        t.r0 = blockIdx.x % a.row_tiles * rows_cta;
+        t.r0 = (blockIdx.x - t.split * a.row_tiles) * rows_cta;
         t.ctx = sp.ctx;
         t.kend = sp.kend;
         t.table = a.table + (size_t)b * a.max_pages;
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
         if constexpr (TREE) {
             const int k_lo = t.key0 + t.blk0 * BN, k_hi = min(t.kend, t.key0 + min(t.blk1, t.nblk_c) * BN);
             if (k_lo < k_hi)
-                for (int pg = k_lo / a.page_size + threadIdx.x - 32; pg <= (k_hi - 1) / a.page_size; pg += SU_THREADS - 32) {
+                for (int pg = (k_lo >> a.page_log2) + threadIdx.x - 32; pg <= (k_hi - 1) >> a.page_log2; pg += SU_THREADS - 32) {
                     const int id = __ldg(t.table + pg);
                     lost |= id < 0 || id >= a.n_pages;
                 }
