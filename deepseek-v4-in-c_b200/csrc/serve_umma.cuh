@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
             }
             const int first = s ? f1 : f0, end = s ? e1 : e0;
             const bool live = 32 * (warp & 3) < rows;        // this warp has rows
-            const int pr = t.r0 + row0 + min(i, max(0, rows - 1)), tok = sa_token(a, pr), head = t.kvh * a.G + pr - tok * a.G;
+            const int tok = sa_token(a, t.r0 + row0 + min(i, max(0, rows - 1)));
             const int tok_lo = sa_token(a, t.r0 + row0), tok_hi = sa_token(a, t.r0 + row0 + rows - 1);
             const int depth = TREE ? s_depth[tok] : 0;
             const uint32_t quarter = (uint32_t)(32 * (warp & 3)) << 16;
@@ -656,6 +656,10 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
                 if (lane == 0) mbar_arrive(&pfull[s]);
             }
             // ---- outputs
+            // At head dim 128 a prompt's loop needs every register: its tile is
+            // read back (32768 causal tokens 16.1 -> 15.8 ms); elsewhere holding
+            // it is faster (64 dims 69 us, read back 71 us).
+            const SaTile &u = D == 128 && !TREE ? sh.t : t;
             const bool any = first < end;
             if (any) ok = ok && __all_sync(0xFFFFFFFFu, sa_poll(&ofull[s], 0, a.status, SUE_O));
             umma::fence_after();
@@ -729,16 +733,17 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
             }
             bool odd = false;
             if (live) {
-                const bool part = t.parts > 1;
+                const int head = u.kvh * a.G + u.r0 + row0 + min(i, max(0, rows - 1)) - tok * a.G;
+                const bool part = TREE && u.parts > 1;
                 const float inv = part ? 1.0f : sa_inv(l, m, a.sink, head);
-                const size_t row_id = (size_t)(t.begin + tok) * a.hq + head;
-                const size_t id = (size_t)t.split * a.nt * a.hq + row_id;
+                const size_t row_id = (size_t)(u.begin + tok) * a.hq + head;
+                const size_t id = (size_t)u.split * a.nt * a.hq + row_id;
                 if (part && i < rows && (!alt || s == 0)) {
                     a.pm[id] = m;
                     a.pl[id] = l;
                 }
                 char *dst = part ? reinterpret_cast<char *>(a.po + id * D + col0)
-                                 : reinterpret_cast<char *>(reinterpret_cast<uint16_t *>(a.o) + (size_t)(t.begin + tok) * a.ldo +
+                                 : reinterpret_cast<char *>(reinterpret_cast<uint16_t *>(a.o) + (size_t)(u.begin + tok) * a.ldo +
                                                             (size_t)head * D + col0);
                 const uint8_t *x = ks + s * XH + i * (XN * 16);
                 const int mine = min(32, rows - 32 * (warp & 3));    // rows of this warp
@@ -801,8 +806,8 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
             if (odd) s_odd[who] = 1;
             alt ? su_bar<256>(1) : su_bar<128>(2 + s);
             if (s_odd[who]) {
-                SaTile ts = t;
-                ts.r0 = t.r0 + row0;
+                SaTile ts = u;
+                ts.r0 = u.r0 + row0;
                 ts.rows = rows;
                 if (!alt) {
                     ts.blk0 = first;
@@ -813,20 +818,20 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
                 alt ? su_bar<256>(1) : su_bar<128>(2 + s);
                 if (s_odd[who] == 2) serve_slow_rows<D, F16, false>(a, ts, BN, thread >> 5, threads >> 5, sees, row_of);
             }
-            if (TREE && t.parts > 1) {
+            if (TREE && u.parts > 1) {
                 // the tile's last split to finish joins them all
                 __threadfence();
                 su_bar<256>(1);
                 if (threadIdx.x == 128) {
-                    int *count = a.counters + ((size_t)blockIdx.z * a.hkv + t.kvh) * a.row_tiles + blockIdx.x % a.row_tiles;
-                    const bool last = atomicAdd(count, 1) == t.parts - 1;
+                    int *count = a.counters + ((size_t)blockIdx.z * a.hkv + u.kvh) * a.row_tiles + blockIdx.x % a.row_tiles;
+                    const bool last = atomicAdd(count, 1) == u.parts - 1;
                     if (last) *count = 0;
                     s_odd[0] = last;
                 }
                 su_bar<256>(1);
                 if (s_odd[0]) {
                     __threadfence();
-                    sa_join<D, F16, false>(a, t, reinterpret_cast<float *>(ks), threadIdx.x - 128, 256, [] { su_bar<256>(1); });
+                    sa_join<D, F16, false>(a, u, reinterpret_cast<float *>(ks), threadIdx.x - 128, 256, [] { su_bar<256>(1); });
                 }
             }
         }
