@@ -30,7 +30,7 @@
 // of 128 query rows do not fit shared memory. Measured with 64 fp32 heads of
 // 512 dims: 6 trees over up to 9000 tokens 206 us (51 GFLOP in three terms: 250
 // TFLOP/s; of a block's time 0.30 in each product, 0.18 in the softmax); 301
-// prompt tokens in a window of 128, 71 us (a third of it set-up and output of
+// prompt tokens in a window of 128, 70 us (a third of it set-up and output of
 // 602 tiles of two or three blocks). Copies of 16 bytes instead of whole rows
 // cost 0.14 of a block's time.
 //
@@ -228,7 +228,7 @@ struct SaTile {
 // ceil(len * G / 2^LOG) tiles, and a later tile has more keys: CTAs start in the
 // order of falling tile numbers over all sequences, so the short ones fill the
 // end (29 prompts of 16001 tokens, 16 heads over 4, 64 dims: 75 us, sequence
-// after sequence 91 us). For that a warp holds the tile counts of up to
+// after sequence 91 us; 69 us since). For that a warp holds the tile counts of up to
 // SA_SORTED sequences and searches for the tile number whose CTAs include `id`.
 // More sequences come one after the other, in reverse, and so do tiles that a
 // window of up to SA_EVEN keys makes nearly equal: there the search only costs

@@ -28,8 +28,8 @@
 // Bound by latency: a request's sums come one after the other (1.6 on average
 // over sampled trees of 8, up to 4), each a few batches of loads, a conversion
 // of every element to double (16 a clock and SM) and a cluster barrier. 64
-// trees over 129280 tokens: 29 us, where the bytes of one row of p and one of
-// draft each take 10 us; one chain of 5 over 32000: 7.7 us. Four CTAs of 256
+// trees over 129280 tokens: 30 us, where the bytes of one row of p and one of
+// draft each take 10 us; one chain of 5 over 32000: 8.3 us. Four CTAs of 256
 // threads per SM keep all 64 clusters resident; asking for a row's slice in L2
 // ahead of its loads changed nothing (31.7 us).
 #include <math.h>

@@ -102,6 +102,18 @@ def test_prompt_many_sequences(dev, kind, dim):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dim", [64, 128, 512])
+@pytest.mark.parametrize("seqs,window", [(32, 0), (33, 1025), (120, 0), (128, 1024), (129, 0), (300, 0), (300, 40)])
+def test_prompt_order_of_tiles(dev, kind, dim, seqs, window):
+    """Every way to deal tiles out: few and many sequences, all heads together and one after the other, windows that
+    make tiles equal."""
+    rng = random.Random(seqs)
+    lens = [rng.choice([0, 1, 7, 20, 60, 110]) for _ in range(seqs)]
+    lens[rng.randrange(seqs)] = 400
+    _prompt(dev, lens, 16, 2, dim, kind, window=window, seed=seqs)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 512])
 def test_prompt_nonfinite_values_stay_behind_the_mask(dev, kind, dim):
     """NaN and infinite values and keys of later tokens and of other sequences reach only the rows that see them."""
     import torch
