@@ -205,7 +205,7 @@ struct SuShared {
     int16_t par[SA_MAX_NODES];
     uint8_t depth[SA_MAX_NODES];
 };
-constexpr int SU_SHARED = 3072;
+constexpr int SU_SHARED = 3 * 1024;
 static_assert(sizeof(SuShared) <= SU_SHARED, "the tiles start on the swizzle's period");
 
 template <int D, bool F16, bool TREE>
