@@ -311,7 +311,8 @@ __global__ void __cluster_dims__(VER_CL, 1, 1) __launch_bounds__(VER_THREADS, 4)
         }
     }
     if (!have_total) total = row_sum();
-    if (!(total > 0.0)) {                        // nothing left (or not a number): the target's row itself
+    auto draws = [](double t) { return t > 0.0 && t < (double)INFINITY; };   // a sum that a token can be drawn from
+    if (!draws(total)) {                         // nothing left, or no number: the target's row itself
         r.k = 0;
         total = row_sum();
     }
@@ -320,7 +321,7 @@ __global__ void __cluster_dims__(VER_CL, 1, 1) __launch_bounds__(VER_THREADS, 4)
     const double *sums = slots[set];
     int owner = -1;
     double before = 0.0;
-    if (total > 0.0) {
+    if (draws(total)) {
         int last = -1;
         double run = 0.0, last_before = 0.0;
         for (int c = 0; c < VER_CL && owner < 0; c++) {

@@ -751,9 +751,9 @@ int dsv4cu_tree_attn(dsv4cu_ctx *ctx, const dsv4cu_tree_attn_args *args, void *s
  * u * mass * draft[cur][x] < rest[x]; refused, rest = max(rest - mass *
  * draft[cur], 0) and mass = sum(rest) (certain drafts: mass -= rest[x],
  * rest[x] = 0). next = the first x whose running sum of rest passes
- * u * sum(rest); an empty rest falls back to p[cur], and -1 where that has no
- * positive finite sum. In doubles. ldp / ldd: floats between rows; vocab at
- * most 2^30. */
+ * u * sum(rest); a rest that is empty or not finite falls back to p[cur], and
+ * next is -1 where that has no positive finite sum. In doubles. ldp / ldd:
+ * floats between rows; vocab at most 2^30. */
 int dsv4cu_verify_greedy(dsv4cu_ctx *ctx, int *accepted, int *next, int *path, const int *tokens, const int *parent,
                          const int *cu, const int *best, const int *slot, int *slot_out, int n_req, int nt,
                          void *stream);

@@ -220,3 +220,31 @@ def test_rows_with_strides_and_other_streams(dev):
         torch.cuda.synchronize()
         want = servefix.verify(tokens, parent, cu, probs=p, u=u2, draft=q)
         assert [x.tolist() for x in out] == list(want[:3])
+
+
+@pytest.mark.parametrize("vocab,at", [(300, 0), (300, 299), (4099, 2048), (129280, 77777)])
+def test_rows_without_a_finite_sum_give_no_token(dev, vocab, at):
+    """An infinite probability is no distribution: next is -1, with and without drafts, refused or not, whatever u is.
+    The walk itself goes on by its comparisons."""
+    import torch
+    p = torch.full((3, vocab), 1.0 / vocab)
+    p[1, at] = float("inf")
+    top = 1 - 2.0 ** -24
+    one = lambda rows, parent, tokens, u, q=None: _sample(  # noqa: E731
+        dev, [0, len(rows)], parent, tokens, p[rows], None if q is None else q[rows], torch.tensor(u),
+        list(range(len(rows))))
+    other = (at + 1) % vocab
+    q = torch.full((3, vocab), 1.0 / vocab)
+    q[:, other] = 0.5
+    for u in (0.0, 0.5, top):
+        assert one([1], [-1], [0], [u])[1] == [-1]                      # the root's row
+        assert one([1], [-1], [0], [u], q)[1] == [-1]
+        assert one([0, 1], [-1, 0], [0, 5], [u, 0.0])[:2] == [[1], [-1]]    # the row behind an accepted node
+        # a refused draft leaves an infinite remainder of an infinite row
+        assert one([1, 0], [-1, 0], [0, other], [u, 0.9])[:2] == [[0], [-1]]
+        assert one([1, 0], [-1, 0], [0, other], [u, 0.9], q)[:2] == [[0], [-1]]
+        # the infinite entry itself is taken, and the finite row behind it gives a token
+        assert one([1, 2], [-1, 0], [0, at], [u, top])[0] == [1]
+        assert 0 <= one([1, 2], [-1, 0], [0, at], [u, top])[1][0] < vocab
+    # a finite row whose draft was refused: the first token that is left
+    assert one([2, 0], [-1, 0], [0, other], [0.0, top])[1] == [0 if other else 1]
