@@ -187,19 +187,20 @@ DSV4CU_DEV uint32_t sa_pack(float x, float y)
         return *reinterpret_cast<const uint32_t *>(&h);
     }
 }
-// Two values as TERMS packed words (bf16 terms, each the rounding of what the
-// ones before left over; the subtractions are exact).
+// Two values as TERMS packed words (bf16 terms). Every term but the last is
+// what the ones before left over, cut to bf16's 8 significand bits: cutting
+// cannot pass the largest bf16 as rounding up does for the largest floats, the
+// subtractions are exact, and three terms of 8 bits hold all 24.
 template <int TERMS, bool F16>
 DSV4CU_DEV void sa_split(float x, float y, uint32_t (&w)[TERMS])
 {
 #pragma unroll
-    for (int t = 0; t < TERMS; t++) {
-        w[t] = sa_pack<F16>(x, y);
-        if (t + 1 < TERMS) {
-            x -= __uint_as_float(w[t] << 16);
-            y -= __uint_as_float(w[t] & 0xFFFF0000u);
-        }
+    for (int t = 0; t + 1 < TERMS; t++) {
+        w[t] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+        x -= __uint_as_float(w[t] << 16);
+        y -= __uint_as_float(w[t] & 0xFFFF0000u);
     }
+    w[TERMS - 1] = sa_pack<F16>(x, y);
 }
 template <bool F16>
 DSV4CU_DEV float sa_float(uint16_t b)

@@ -493,3 +493,20 @@ def test_prompt_windows_of_wide_tiles(dev, dim):
     """One query head per key head: a tile's strips start blocks apart, each in its own part of the window."""
     for window in (1, 30, 64, 127, 128, 129, 300):
         _prompt(dev, [900, 40], 2, 2, dim, KINDS[0], window=window)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+@pytest.mark.parametrize("shared", [False, True])
+def test_largest_fp32_queries(dev, dim, shared):
+    """Finite fp32 queries above the largest bf16: their products with small keys are finite, and so are the outputs."""
+    import torch
+    big = torch.finfo(torch.float32).max
+    kind = KINDS[2]
+
+    def edit(q, k, v, *cache):
+        q[:, :, 0], q[:, :, 1] = big, -big
+        for x in (k,) + cache[:1]:
+            x[..., :2] *= 2.0 ** -127                      # products of at most about 10
+
+    _prompt(dev, [90, 5], 4, 1, dim, kind, shared=shared, edit=edit)
+    _tree(dev, [200, 70], [3, 9], 4, 1, dim, kind, shared=shared, edit=edit)
