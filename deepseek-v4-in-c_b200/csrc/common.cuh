@@ -17,6 +17,7 @@
 #include <stdint.h>
 
 #include "../../include/dsv4cu.h"
+#include "smem_limit.h"
 
 #if defined(__CUDA_ARCH__) && (__CUDA_ARCH__ < 1000)
 #error "dsv4cu is written for sm_100a (B200) only"
@@ -177,24 +178,7 @@ namespace dsv4cu {
 DSV4CU_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 DSV4CU_DEV void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// Host-side per-device caches, so a call costs no attribute queries after
-// the first: SmemLimit (one per call site) remembers the largest dynamic
-// shared-memory limit set for a kernel on each device; device_sms() the SM
-// count of the current device.
-struct SmemLimit {
-    int set[64];
-};
-static inline cudaError_t smem_limit(SmemLimit &c, const void *kernel, int bytes)
-{
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    const bool cache = dev >= 0 && dev < 64;
-    if (cache && c.set[dev] >= bytes) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && cache) c.set[dev] = bytes;
-    return e;
-}
+// SM count of the current device, kept per device.
 static inline int device_sms()
 {
     static int n[64];
