@@ -382,8 +382,9 @@ class TreeAttnArgs(C.Structure):
                [("scale", C.c_float), ("sink", C.c_void_p)]
 
 
-# The same layouts for struct.pack_into: filling a ctypes.Structure of this many
-# fields costs a serving step a few microseconds per call.
+# The same layouts for struct.pack: filling a ctypes.Structure of this many
+# fields costs a serving step a few microseconds per call. Every call packs a
+# buffer of its own, so calls of several threads do not touch each other's.
 _PLAN = struct.Struct("@5i12Q")
 _PROMPT = struct.Struct("@4Q4q2iQ6ifQ")
 _TREE = struct.Struct("@6Q4q2i4Q11ifQ")
@@ -404,7 +405,6 @@ class Device:
         check(self.L.dsv4cu_ctx_create(C.byref(h), device), "ctx_create")
         self.ctx = h
         self._elem = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-        self._args = C.create_string_buffer(256)     # argument structure of the call being made
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
     def close(self):
@@ -800,10 +800,10 @@ class Device:
             if t.dtype is not i64 or t.numel() != 2 or t.get_device() != device or not t.is_contiguous():
                 raise DSV4CUError("page_plan: ring_pos needs two contiguous int64 on this device")
         width = table.shape[1]
-        _PLAN.pack_into(self._args, 0, n, page_size, pages, width, cap, seq, new, h, h_out,
-                        *self._ints("page_plan", n * width, table), *self._ints("page_plan", pages, ring),
-                        ring_pos.data_ptr(), ring_pos_out.data_ptr(), *self._ints("page_plan", n + 1, cu), *out)
-        rc = self.L.dsv4cu_page_plan(self.ctx, self._args, self.stream())
+        a = _PLAN.pack(n, page_size, pages, width, cap, seq, new, h, h_out, *self._ints("page_plan", n * width, table),
+                       *self._ints("page_plan", pages, ring), ring_pos.data_ptr(), ring_pos_out.data_ptr(),
+                       *self._ints("page_plan", n + 1, cu), *out)
+        rc = self.L.dsv4cu_page_plan(self.ctx, a, self.stream())
         if rc:
             check(rc, "dsv4cu_page_plan")
 
@@ -837,10 +837,10 @@ class Device:
         if o.shape[0] != nt or k.shape[0] != nt or (v is not None and v.shape[0] != nt):
             raise DSV4CUError(f"{what}: q, k, v and o must have the same number of tokens")
         n = cu.numel()
-        _PROMPT.pack_into(self._args, 0, o.data_ptr(), q.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr(), ldo,
-                          ldq, ldk, ldv, self._elem[q.dtype], self._elem[k.dtype], self._ints(what, n, cu)[0], n - 1, nt,
-                          heads, kv, dim, window, scale, self._sink(what, sink, heads))
-        rc = self.L.dsv4cu_prompt_attn(self.ctx, self._args, self.stream())
+        a = _PROMPT.pack(o.data_ptr(), q.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr(), ldo, ldq, ldk, ldv,
+                         self._elem[q.dtype], self._elem[k.dtype], self._ints(what, n, cu)[0], n - 1, nt, heads, kv,
+                         dim, window, scale, self._sink(what, sink, heads))
+        rc = self.L.dsv4cu_prompt_attn(self.ctx, a, self.stream())
         if rc:
             check(rc, "dsv4cu_prompt_attn")
 
@@ -860,13 +860,12 @@ class Device:
         if table.dim() != 2 or table.shape[0] != n:
             raise DSV4CUError(f"{what}: table needs {n} rows, got {tuple(table.shape)}")
         width = table.shape[1]
-        _TREE.pack_into(self._args, 0, o.data_ptr(), q.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr(),
-                        k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), ldo, ldq, ldk, ldv,
-                        self._elem[q.dtype], self._elem[k.dtype], *self._ints(what, n * width, table),
-                        *self._ints(what, n, ctx_len), *self._ints(what, n + 1, cu), *self._ints(what, nt, parent), n,
-                        nt, heads, kv, dim, page, pages, width, max_nodes, max_ctx, window, scale,
-                        self._sink(what, sink, heads))
-        return self._args
+        return _TREE.pack(o.data_ptr(), q.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr(),
+                          k_cache.data_ptr(), 0 if v_cache is None else v_cache.data_ptr(), ldo, ldq, ldk, ldv,
+                          self._elem[q.dtype], self._elem[k.dtype], *self._ints(what, n * width, table),
+                          *self._ints(what, n, ctx_len), *self._ints(what, n + 1, cu), *self._ints(what, nt, parent), n,
+                          nt, heads, kv, dim, page, pages, width, max_nodes, max_ctx, window, scale,
+                          self._sink(what, sink, heads))
 
     def tree_attn(self, o, q, k, v, k_cache, v_cache, table, ctx_len, cu, parent, scale: float, max_nodes: int,
                   max_ctx: int, window: int = 0, sink=None):

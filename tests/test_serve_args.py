@@ -155,3 +155,67 @@ def test_row_numbers_and_vocabularies_past_32_bits_are_refused(L, ctx):
     assert L.dsv4cu_tree_attn_workspace(ctx, C.byref(a)) == 0
     v = (1 << 30) + 1
     assert L.dsv4cu_verify_sample(ctx, P, P, P, P, P, P, P, v, None, 0, P, v, None, None, 1, 1, None) == ARG
+
+
+class _TwoThreads:
+    """Stands in for the library: every call reads its arguments, lets the other thread make its call, reads again."""
+
+    def __init__(self):
+        import threading
+        self.meet = threading.Barrier(2, timeout=20)
+        self.torn = []
+
+    def _call(self, ctx, args, stream):
+        size = len(bytes(args))
+        first = C.string_at(args, size)
+        self.meet.wait()                       # both have packed their arguments and are inside the library
+        if C.string_at(args, size) != first:
+            self.torn.append(first)
+        self.meet.wait()
+        return 0
+
+    dsv4cu_page_plan = dsv4cu_prompt_attn = dsv4cu_tree_attn = _call
+
+
+@pytest.mark.parametrize("op", ["plan", "prompt", "tree"])
+def test_calls_of_two_threads_keep_their_arguments(op):
+    """A call's arguments are its own: a second thread's call on the same Device does not change them under the first."""
+    import threading
+
+    import torch
+
+    import dsv4cu
+    dev = object.__new__(dsv4cu.Device)
+    dev.torch, dev.L, dev.device, dev.ctx = torch, _TwoThreads(), -1, None       # tensors of the CPU count as device -1
+    dev._elem = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    dev._raw_stream = lambda device: 0
+
+    def call(n):
+        i32 = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+        row = lambda h: torch.zeros(n, h, 64, dtype=torch.bfloat16)  # noqa: E731
+        cache = torch.zeros(2, 8, 2, 64, dtype=torch.bfloat16)
+        if op == "plan":
+            dev.page_plan(i32(n, 3), i32(n), i32(8), torch.zeros(2, dtype=torch.int64), i32(n), i32(n), 8, i32(n + 1),
+                          i32(5))
+        elif op == "prompt":
+            dev.prompt_attn(row(4), row(4), row(2), row(2), i32(2), 0.125)
+        else:
+            dev.tree_attn(row(4), row(4), row(2), row(2), cache, cache, i32(n, 3), i32(n), i32(n + 1), i32(n), 0.125, 4,
+                          16)
+
+    start = threading.Barrier(2, timeout=20)
+    failed = []
+
+    def run(n):
+        try:
+            start.wait()
+            for _ in range(20):
+                call(n)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+    threads = [threading.Thread(target=run, args=(n,)) for n in (1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed and not dev.L.torn
