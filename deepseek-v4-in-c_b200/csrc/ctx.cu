@@ -106,17 +106,54 @@ extern "C" int dsv4cu_ctx_inject(dsv4cu_ctx *c, int what)
     return DSV4CU_OK;
 }
 
+// "free pages ran out (71), ..." for every bit.
+static void refused_text(unsigned bits, char *text, size_t size)
+{
+    static const struct {
+        int code;
+        const char *what;
+    } names[] = {{DSV4CU_NO_PAGES, "page_plan: free pages ran out"},
+                 {DSV4CU_NO_ROWS, "page_plan: more tokens than nt_cap"},
+                 {DSV4CU_NO_ENTRIES, "page_plan: a request needs more than max_pages pages"},
+                 {DSV4CU_TREE_NODES, "tree_attn: a request has more than max_nodes nodes"},
+                 {DSV4CU_VERIFY_NODES, "verify: a request has more than 128 nodes"}};
+    size_t n = 0;
+    text[0] = 0;
+    for (const auto &x : names)
+        if (bits >> (x.code - DSV4CU_NO_PAGES) & 1 && n < size)
+            n += (size_t)snprintf(text + n, size - n, "%s%s (%d)", n ? ", " : "", x.what, x.code);
+}
+
 extern "C" int dsv4cu_ctx_status(dsv4cu_ctx *c, void *stream, int *code)
 {
     if (!c || !code) return dsv4cu_set_error(DSV4CU_ERR_ARG, "ctx_status: NULL argument");
     DSV4CU_CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
-    DSV4CU_CUDA_TRY(cudaMemcpy(code, c->status, sizeof(int), cudaMemcpyDeviceToHost));
+    int words[2];
+    DSV4CU_CUDA_TRY(cudaMemcpy(words, c->status, sizeof words, cudaMemcpyDeviceToHost));
+    *code = words[0];
     if (*code) {
         // A kernel that gave up may have left its last-arriver counts behind.
         DSV4CU_CUDA_TRY(cudaMemset(c->counters, 0, DSV4CU_MAX_COUNTERS * sizeof(int)));
         DSV4CU_CUDA_TRY(cudaMemset(c->status, 0, sizeof(int)));
-        return dsv4cu_set_error(DSV4CU_ERR_TIMEOUT, "a bounded device wait timed out (code 0x%x)", *code);
+        return dsv4cu_set_error(DSV4CU_ERR_TIMEOUT, "a bounded device wait timed out (code %d)", *code);
     }
+    if (words[1]) {
+        DSV4CU_CUDA_TRY(cudaMemset(c->status + 1, 0, sizeof(int)));
+        char text[400];
+        refused_text((unsigned)words[1], text, sizeof text);
+        *code = DSV4CU_NO_PAGES;
+        while (!(words[1] >> (*code - DSV4CU_NO_PAGES) & 1)) (*code)++;
+        return dsv4cu_set_error(DSV4CU_ERR_REFUSED, "work was left out: %s", text);
+    }
+    return DSV4CU_OK;
+}
+
+extern "C" int dsv4cu_ctx_refused(dsv4cu_ctx *c, void *stream, unsigned *codes)
+{
+    if (!c || !codes) return dsv4cu_set_error(DSV4CU_ERR_ARG, "ctx_refused: NULL argument");
+    DSV4CU_CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
+    DSV4CU_CUDA_TRY(cudaMemcpy(codes, c->status + 1, sizeof *codes, cudaMemcpyDeviceToHost));
+    if (*codes) DSV4CU_CUDA_TRY(cudaMemset(c->status + 1, 0, sizeof(int)));
     return DSV4CU_OK;
 }
 

@@ -14,7 +14,8 @@ struct dsv4cu_ctx {
     void  *ws;          // device workspace
     size_t ws_bytes;
     int   *counters;    // [DSV4CU_MAX_COUNTERS], zero between calls
-    int   *status;      // device word: first bounded-wait timeout code, 0 = none
+    int   *status;      // two device words: first bounded-wait timeout code, 0 = none; and
+                        // the work left out, a bit per code from DSV4CU_NO_PAGES on
     int    inject;      // one-shot test fault for the next dsv4cu_gemv (DSV4CU_INJECT_*), 0 = none
 };
 

@@ -13,9 +13,6 @@ constexpr int PLAN_ITEM_THREADS = 256;
 constexpr int PLAN_SOLO_ITEMS = 4096;    // tokens one block handles by itself
 constexpr int PLAN_FUSED_REQ = 1024;     // requests whose sums every block keeps in shared memory
 
-// Status words of dsv4cu_ctx_status.
-enum { PLAN_NO_PAGES = 71, PLAN_TOKENS = 72, PLAN_TABLE = 73 };
-
 struct PlanWs {           // what the scan leaves for the items, per request; in the workspace or in shared memory
     int *held;            // pages held before the call (clamped)
     int *seq;             // tokens before the call (clamped)
@@ -41,8 +38,6 @@ static size_t plan_ws_layout(int n_req, char *base, PlanWs *w)
     w->ring_at = (int *)take(8);
     return off;
 }
-
-DSV4CU_DEV void plan_status(int *status, int code) { atomicCAS(status, 0, code); }
 
 // Inclusive sum of three values over the block's threads; total[] receives the
 // block's sums.
@@ -224,10 +219,10 @@ DSV4CU_DEV void plan_scan(const dsv4cu_page_plan_args &a, const PlanWs &w, bool 
         if (tid == 0) {
             a.ring_pos_out[0] = head + min(carry[1], avail);
             a.ring_pos_out[1] = tail + carry[2];
-            if (carry[0] > a.nt_cap) plan_status(status, PLAN_TOKENS);
+            if (carry[0] > a.nt_cap) serve_refuse(status, DSV4CU_NO_ROWS);
         }
-        if (no_pages) plan_status(status, PLAN_NO_PAGES);
-        if (narrow) plan_status(status, PLAN_TABLE);
+        if (no_pages) serve_refuse(status, DSV4CU_NO_PAGES);
+        if (narrow) serve_refuse(status, DSV4CU_NO_ENTRIES);
     }
 }
 

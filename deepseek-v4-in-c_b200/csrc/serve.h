@@ -26,6 +26,10 @@ struct DeviceGuard {
     }
 };
 
+// Work that a kernel leaves out: a bit beside the watchdog's word, so neither
+// hides the other and no code hides another.
+DSV4CU_DEV void serve_refuse(int *status, int code) { atomicOr(status + 1, 1 << (code - DSV4CU_NO_PAGES)); }
+
 static inline int elem_bytes(int type) { return type == DSV4CU_F32 ? 4 : 2; }
 static inline bool elem_known(int type) { return type == DSV4CU_F32 || type == DSV4CU_BF16 || type == DSV4CU_F16; }
 static inline bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }

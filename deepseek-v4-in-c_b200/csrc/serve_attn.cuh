@@ -54,7 +54,7 @@ namespace dsv4cu {
 
 constexpr int SA_MAX_NODES = 128;
 constexpr float SA_LOG2E = 1.4426950408889634f;
-enum { SA_BAD_NODES = 75, SA_COPY = 77 };   // dsv4cu_ctx_status: more nodes than max_nodes, a copy that did not arrive
+enum { SA_COPY = 77 };                // dsv4cu_ctx_status: a copy that did not arrive
 
 struct SaArgs {
     const void *q, *k, *v;            // packed rows; v == NULL: the key rows are the values
@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(32 * sa_warps(D), 1) serve_attn_kernel(const _
         t.begin = sp.begin;
         t.len = sp.len;
         if (t.len > a.max_nodes) {                       // refused whole: its rows are left as they were
-            if (tid == 0) atomicCAS(a.status, 0, SA_BAD_NODES);
+            if (tid == 0) serve_refuse(a.status, DSV4CU_TREE_NODES);
             return;
         }
         if (t.split >= sp.used) return;

@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(SU_THREADS, SuShape<D>::CTAS) serve_umma_kerne
         t.begin = sp.begin;
         t.len = sp.len;
         if (t.len > a.max_nodes) {
-            if (threadIdx.x == 0) atomicCAS(a.status, 0, SA_BAD_NODES);
+            if (threadIdx.x == 0) serve_refuse(a.status, DSV4CU_TREE_NODES);
             return;
         }
         if (t.split >= sp.used) return;

@@ -47,7 +47,6 @@ constexpr int VER_THREADS = 256;
 constexpr int VER_BATCH = 32;         // elements a lane has in flight, of one row or of both
 constexpr int VER_WARPS = VER_THREADS / 32;
 constexpr int VER_CL = 8;             // CTAs per request: the largest portable cluster
-enum { VER_BAD_TREE = 76 };           // more than VER_MAX_NODES nodes (dsv4cu_ctx_status)
 
 struct VerifyArgs {
     int *accepted, *next, *path, *slot_out;
@@ -76,7 +75,7 @@ DSV4CU_DEV void ver_refuse(const VerifyArgs &a, int b, int begin, int n)
         a.path[begin + i] = -1;
         if (a.slot_out) a.slot_out[begin + i] = -1;
     }
-    if (n > VER_MAX_NODES) atomicCAS(a.status, 0, VER_BAD_TREE);
+    if (n > VER_MAX_NODES) serve_refuse(a.status, DSV4CU_VERIFY_NODES);
 }
 
 // Writes path and slot_out of one request from the accepted line (line[0] = 0).

@@ -70,6 +70,7 @@ def lib() -> C.CDLL:
             "dsv4cu_ctx_reserve": (i, [vp, sz]),
             "dsv4cu_ctx_workspace_bytes": (sz, [vp]),
             "dsv4cu_ctx_status": (i, [vp, vp, C.POINTER(i)]),
+            "dsv4cu_ctx_refused": (i, [vp, vp, C.POINTER(C.c_uint)]),
             "dsv4cu_ctx_inject": (i, [vp, i]),
             "dsv4cu_mmq_workspace": (sz, [vp, i]),
             "dsv4cu_mmq": (i, [vp, vp, vp, vp, i, vp]),
@@ -424,15 +425,24 @@ class Device:
         check(self.L.dsv4cu_ctx_inject(self.ctx, what), "dsv4cu_ctx_inject")
 
     def status_code(self) -> int:
-        """Synchronise and return (and clear) the context's device status word."""
+        """Synchronise and return (and clear) the context's device status: a timeout's code, or the lowest code of
+        work left out (dsv4cu_ctx_status)."""
         code = C.c_int(0)
         self.L.dsv4cu_ctx_status(self.ctx, self.stream(), C.byref(code))
         return code.value
 
     def check_status(self):
-        """Raise if a kernel of this context hit a bounded-wait timeout."""
+        """Raise if a kernel of this context hit a bounded-wait timeout or left work out."""
         code = C.c_int(0)
         check(self.L.dsv4cu_ctx_status(self.ctx, self.stream(), C.byref(code)), "device status")
+
+    NO_PAGES, NO_ROWS, NO_ENTRIES, TREE_NODES, VERIFY_NODES = 71, 72, 73, 75, 76
+
+    def refused(self) -> set:
+        """Synchronise, return and clear the codes of work that paged serving calls left out (dsv4cu_ctx_refused)."""
+        bits = C.c_uint(0)
+        check(self.L.dsv4cu_ctx_refused(self.ctx, self.stream(), C.byref(bits)), "dsv4cu_ctx_refused")
+        return {self.NO_PAGES + i for i in range(32) if bits.value >> i & 1}
 
     @staticmethod
     def ptr(t):

@@ -32,7 +32,8 @@ enum {
     DSV4CU_ERR_NOMEM = -4,        /* device allocation failed                 */
     DSV4CU_ERR_TIMEOUT = -5,      /* a bounded device wait expired            */
     DSV4CU_ERR_COMM = -6,         /* collective / peer exchange failed        */
-    DSV4CU_ERR_IO = -7            /* pack file missing, malformed or short    */
+    DSV4CU_ERR_IO = -7,           /* pack file missing, malformed or short    */
+    DSV4CU_ERR_REFUSED = -8       /* a kernel left work out (dsv4cu_ctx_status) */
 };
 
 /* Weight storage tags; same values as the reference enum
@@ -71,11 +72,27 @@ int  dsv4cu_ctx_create(dsv4cu_ctx **out, int device);
 void dsv4cu_ctx_destroy(dsv4cu_ctx *ctx);
 int  dsv4cu_ctx_reserve(dsv4cu_ctx *ctx, size_t bytes);
 size_t dsv4cu_ctx_workspace_bytes(const dsv4cu_ctx *ctx);
-/* Synchronise `stream` and report whether any kernel of this context hit a
- * bounded-wait timeout since the last check (*code = 0: none; otherwise the
- * call returns DSV4CU_ERR_TIMEOUT, clears the word and resets the context's
- * cross-CTA counters, so the next call runs normally). */
+/* What the paged serving kernels leave out instead of failing: ordinary events
+ * of a server, found on the device. */
+enum {
+    DSV4CU_NO_PAGES = 71,      /* page_plan: the free pages ran out            */
+    DSV4CU_NO_ROWS = 72,       /* page_plan: more tokens than nt_cap           */
+    DSV4CU_NO_ENTRIES = 73,    /* page_plan: a request needs over max_pages    */
+    DSV4CU_TREE_NODES = 75,    /* tree_attn: a request over max_nodes nodes    */
+    DSV4CU_VERIFY_NODES = 76   /* verify_*: a request over 128 nodes           */
+};
+/* Synchronise `stream` and report what the kernels of this context met since
+ * the last check (*code = 0: nothing). The first bounded-wait timeout or other
+ * broken expectation comes before all else: the call returns
+ * DSV4CU_ERR_TIMEOUT with its code, clears it and resets the context's
+ * cross-CTA counters, so the next call runs normally. Without one, work left
+ * out (the codes above) makes it return DSV4CU_ERR_REFUSED with the lowest of
+ * the codes, all of them named by dsv4cu_last_error, and clears them. */
 int  dsv4cu_ctx_status(dsv4cu_ctx *ctx, void *stream, int *code);
+/* Synchronise `stream`, hand out and clear the work left out alone: bit
+ * (code - DSV4CU_NO_PAGES) of *codes for every code met since the last check.
+ * Timeouts stay for dsv4cu_ctx_status. */
+int  dsv4cu_ctx_refused(dsv4cu_ctx *ctx, void *stream, unsigned *codes);
 /* Test-only fault, consumed by the next dsv4cu_gemv call on the streamed
  * path: WITHHOLD_STAGE makes its first CTA skip its third weight stage (no
  * copy is issued and nothing arrives on the stage's barrier), so that CTA's
@@ -650,11 +667,11 @@ enum { DSV4CU_F32 = 0, DSV4CU_BF16 = 1, DSV4CU_F16 = 2 };   /* element types */
  * request (pos and req may be NULL); rows behind the last token get -1.
  * held_out / ring_pos_out may be held / ring_pos. Only table entries of newly
  * granted pages and ring entries of released ones are written, so the same
- * call on the same held and ring_pos writes the same again. Status codes
- * (dsv4cu_ctx_status): 71 the ring ran out (requests in order got what was
- * there, slots on missing pages are -1), 72 more tokens than nt_cap (the rest
- * has no row), 73 a request needs more than max_pages pages (slots behind
- * them are -1). */
+ * call on the same held and ring_pos writes the same again. Left out, and said
+ * so (dsv4cu_ctx_status, dsv4cu_ctx_refused): pages where the ring ran out
+ * (DSV4CU_NO_PAGES; requests in order got what was there, slots on missing
+ * pages are -1), rows of more tokens than nt_cap (DSV4CU_NO_ROWS), pages past
+ * max_pages (DSV4CU_NO_ENTRIES; slots behind them are -1). */
 typedef struct {
     int n_req, page_size, n_pages, max_pages, nt_cap;
     const int *seq_len, *new_len;       /* [n_req] */
@@ -714,7 +731,7 @@ int dsv4cu_prompt_attn(dsv4cu_ctx *ctx, const dsv4cu_prompt_attn_args *args, voi
  * Types, heads, head dims, sink, v NULL (then v_cache NULL as well) and
  * non-finite values as in dsv4cu_prompt_attn. max_ctx, an upper estimate of
  * ctx_len, only chooses how many ways a cache is split. A request with more
- * than max_nodes nodes is left out and sets status code 75. */
+ * than max_nodes nodes is left out (DSV4CU_TREE_NODES). */
 typedef struct {
     void *o;
     const void *q, *k, *v, *k_cache, *v_cache;
@@ -731,11 +748,12 @@ size_t dsv4cu_tree_attn_workspace(const dsv4cu_ctx *ctx, const dsv4cu_tree_attn_
 int dsv4cu_tree_attn(dsv4cu_ctx *ctx, const dsv4cu_tree_attn_args *args, void *stream);
 
 /* Verification of drafted trees (cu, parent as in dsv4cu_tree_attn, at most
- * 128 nodes per request; more sets status code 76). The current node starts
- * at node 0; a node in index order whose parent is the current node is tested
- * and becomes the current node when accepted. accepted[b] = accepted nodes
- * (node 0 not counted), next[b] = the token behind the last of them, path
- * [nt]: rows cu[b] + i hold node 0 (i = 0) and the i-th accepted node, then -1.
+ * 128 nodes per request; one with more is left out, accepted 0 and next -1:
+ * DSV4CU_VERIFY_NODES). The current node starts at node 0; a node in index
+ * order whose parent is the current node is tested and becomes the current
+ * node when accepted. accepted[b] = accepted nodes (node 0 not counted),
+ * next[b] = the token behind the last of them, path [nt]: rows cu[b] + i hold
+ * node 0 (i = 0) and the i-th accepted node, then -1.
  * With slot [nt] (a page plan's slots for the request's rows) and slot_out
  * [nt], slot_out of the d-th node of the path is slot[cu[b] + d] and -1 for
  * every other node: the rows dsv4cu_paged_write commits. A request without

@@ -229,3 +229,54 @@ def test_binding_refuses_wrong_tensors(dev):
                 lambda: dev.paged_write(cache, cache, rows, rows.float(), slot)):
         with pytest.raises(dsv4cu.DSV4CUError):
             bad()
+
+
+def _leave_out_everything(dev):
+    """One call of each kind that leaves work out."""
+    import torch
+    zero = torch.zeros(132, dtype=torch.int32, device="cuda")
+    cu = _i([0, 129, 132])
+    out = [torch.empty(m, dtype=torch.int32, device="cuda") for m in (2, 2, 132)]
+    rp = _i([0, 1], torch.int64)
+    # one free page for a request of 3 pages over a table of 2; 40 tokens for 8 rows
+    dev.page_plan(_i([[-1, -1]]), _i([0]), _i([0, 0]), rp, _i([0]), _i([40]), 16, _i([0, 0]), _i([0] * 8))
+    dev.verify_greedy(*out, zero, zero, cu, zero)
+    rows = torch.zeros(132, 1, 64, dtype=torch.bfloat16, device="cuda")
+    cache = torch.zeros(1, 16, 1, 64, dtype=torch.bfloat16, device="cuda")
+    dev.tree_attn(torch.empty_like(rows), rows, rows, rows, cache, cache, _i([[0], [0]]), _i([4, 4]), cu, zero, 0.1, 8, 4)
+
+
+def test_work_left_out_is_told_apart(dev):
+    """Every kind is remembered, none as a timeout; the status call gives the lowest and clears all."""
+    import dsv4cu
+    assert dev.refused() == set()
+    _leave_out_everything(dev)
+    assert dev.refused() == {71, 72, 73, 75, 76}
+    assert dev.refused() == set() and dev.status_code() == 0
+    _leave_out_everything(dev)
+    with pytest.raises(dsv4cu.DSV4CUError, match=r"status -8: .*free pages.*\(71\).*\(75\)"):
+        dev.check_status()
+    assert dev.status_code() == 0
+
+
+@pytest.mark.parametrize("first", [False, True])
+def test_work_left_out_and_a_timeout_do_not_hide_each_other(dev, first):
+    """A wait that runs out (a stage withheld in a streamed GEMV) before or after work is left out: both are told."""
+    import numpy as np
+    import torch
+    rows = cols = 7168                         # as many stages per CTA as the withheld one takes
+    w = torch.zeros(rows, cols, dtype=torch.uint8, device="cuda")
+    s = torch.full((rows // 128, cols // 128), 127, dtype=torch.uint8, device="cuda")
+    m = dev.qmat(w, s, 2, rows, cols, 128, 128)
+    x = torch.from_numpy(np.ones((1, cols), np.float32)).cuda()
+    y = torch.empty((1, rows), dtype=torch.float32, device="cuda")
+    if first:
+        _leave_out_everything(dev)
+    dev.inject(dev.INJECT_WITHHOLD_STAGE)
+    dev.gemv(y, x, m, 1)
+    if not first:
+        _leave_out_everything(dev)
+    assert 0 < dev.status_code() < 71          # the timeout, whichever came first
+    assert dev.refused() == {71, 72, 73, 75, 76}
+    dev.gemv(y, x, m, 1)
+    assert dev.status_code() == 0 and not bool(y.any())
