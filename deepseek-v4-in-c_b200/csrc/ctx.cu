@@ -6,6 +6,7 @@
 
 #include "common.cuh"
 #include "ctx.h"
+#include "serve.h"
 
 namespace dsv4cu {
 const float *router_table_get();
@@ -67,6 +68,8 @@ extern "C" int dsv4cu_ctx_create(dsv4cu_ctx **out, int device)
 extern "C" void dsv4cu_ctx_destroy(dsv4cu_ctx *c)
 {
     if (!c) return;
+    dsv4cu::DeviceGuard guard;
+    guard.enter(c->device);
     if (c->ws) cudaFree(c->ws);
     if (c->counters) cudaFree(c->counters);
     free(c);
@@ -76,6 +79,8 @@ extern "C" int dsv4cu_ctx_reserve(dsv4cu_ctx *c, size_t bytes)
 {
     if (!c) return dsv4cu_set_error(DSV4CU_ERR_ARG, "ctx_reserve: NULL ctx");
     if (bytes <= c->ws_bytes) return DSV4CU_OK;
+    dsv4cu::DeviceGuard guard;               // the kernels of this context read it on its device
+    DSV4CU_CUDA_TRY(guard.enter(c->device));
     // The old buffer may still be read by queued work: wait before freeing.
     DSV4CU_CUDA_TRY(cudaDeviceSynchronize());
     if (c->ws) cudaFree(c->ws);
@@ -127,6 +132,8 @@ static void refused_text(unsigned bits, char *text, size_t size)
 extern "C" int dsv4cu_ctx_status(dsv4cu_ctx *c, void *stream, int *code)
 {
     if (!c || !code) return dsv4cu_set_error(DSV4CU_ERR_ARG, "ctx_status: NULL argument");
+    dsv4cu::DeviceGuard guard;               // a NULL stream is the current device's
+    DSV4CU_CUDA_TRY(guard.enter(c->device));
     DSV4CU_CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
     int words[2];
     DSV4CU_CUDA_TRY(cudaMemcpy(words, c->status, sizeof words, cudaMemcpyDeviceToHost));
@@ -151,6 +158,8 @@ extern "C" int dsv4cu_ctx_status(dsv4cu_ctx *c, void *stream, int *code)
 extern "C" int dsv4cu_ctx_refused(dsv4cu_ctx *c, void *stream, unsigned *codes)
 {
     if (!c || !codes) return dsv4cu_set_error(DSV4CU_ERR_ARG, "ctx_refused: NULL argument");
+    dsv4cu::DeviceGuard guard;
+    DSV4CU_CUDA_TRY(guard.enter(c->device));
     DSV4CU_CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
     DSV4CU_CUDA_TRY(cudaMemcpy(codes, c->status + 1, sizeof *codes, cudaMemcpyDeviceToHost));
     if (*codes) DSV4CU_CUDA_TRY(cudaMemset(c->status + 1, 0, sizeof(int)));

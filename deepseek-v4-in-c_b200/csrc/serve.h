@@ -6,8 +6,8 @@
 
 namespace dsv4cu {
 
-// The calling thread's current device for the length of a call: the operator
-// runs on its context's device whichever device is current.
+// The calling thread's current device for the length of a call: the call
+// works on its context's device whichever device is current.
 struct DeviceGuard {
     int prev = -1;
     bool moved = false;

@@ -66,7 +66,8 @@ int dsv4cu_set_error(int code, const char *fmt, ...);
 
 /* Library context: owns a device workspace (grown on demand, or reserved up
  * front with dsv4cu_ctx_reserve so later calls allocate nothing). One context
- * per device; not shared between threads without external locking. */
+ * per device; not shared between threads without external locking. The
+ * dsv4cu_ctx_* calls work on the context's device whichever device is current. */
 typedef struct dsv4cu_ctx dsv4cu_ctx;
 int  dsv4cu_ctx_create(dsv4cu_ctx **out, int device);
 void dsv4cu_ctx_destroy(dsv4cu_ctx *ctx);

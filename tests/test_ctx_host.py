@@ -103,3 +103,37 @@ int main()
     assert out[4] == "0 0 "
     assert out[5].startswith("-8 71 ") and "pages" in out[5] and out[6] == "3"
     assert out[7] == "0 17" and out[8].startswith("-5 5 ") and out[9] == "0 0 " and out[10] == "-1 -1"
+
+
+def test_context_calls_run_on_the_contexts_device(tmp_path):
+    """Reserving, looking and growing work on the context's device whichever device is current, and leave that current."""
+    out, calls = _run(tmp_path, r"""
+int main()
+{
+    dsv4cu_ctx *c;
+    dsv4cu_ctx_create(&c, 1);
+    fprintf(stderr, "--\n");
+    int code;
+    unsigned bits;
+    void *ws;
+    dsv4cu_ctx_reserve(c, 1 << 20);
+    printf("%d\n", current);
+    dsv4cu_ws_get(c, 5 << 20, &ws);
+    printf("%d\n", current);
+    c->status[0] = 9;
+    dsv4cu_ctx_status(c, nullptr, &code);
+    printf("%d\n", current);
+    c->status[1] = 2;
+    dsv4cu_ctx_status(c, nullptr, &code);
+    c->status[1] = 2;
+    dsv4cu_ctx_refused(c, nullptr, &bits);
+    printf("%d %u\n", current, bits);
+    dsv4cu_ctx_destroy(c);
+    printf("%d\n", current);
+    return 0;
+}
+""")
+    assert out == ["0", "0", "0", "0 2", "0"]
+    calls = calls[calls.index("--") + 1:]
+    assert {x.split()[0] for x in calls} >= {"malloc", "free", "memset", "memcpy", "stream", "device"}
+    assert all(x.split()[1] == "1" for x in calls), calls
