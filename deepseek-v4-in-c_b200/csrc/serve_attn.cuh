@@ -463,9 +463,13 @@ __device__ __noinline__ void serve_slow_rows(const SaArgs &a, const SaTile &t, i
 
 // Joins the splits of a tile's rows: the partial outputs rescaled to the row's
 // largest maximum and divided by the joint exp-sum (with the sink), in split
-// order whichever split came last. First the maxima and sums into sm (2 parts
+// order whichever split came last. No factor is below SA_LEAST, which adds nothing
+// to a finite sum but keeps a visible infinity or NaN of a split that weighs next
+// to nothing (a row of NaN scores alone has no maximum; a split without a visible
+// key has sums of exactly 0). First the maxima and sums into sm (2 parts
 // + 1 numbers a row), a row's factors by a thread; then the outputs, four
 // columns per thread.
+constexpr float SA_LEAST = 1.1754944e-38f;   // 2^-126
 template <int D, bool F16, bool QF32, class Sync>
 DSV4CU_DEV void sa_join(const SaArgs &a, const SaTile &t, float *sm, int tid, int threads, Sync sync)
 {
@@ -488,9 +492,9 @@ DSV4CU_DEV void sa_join(const SaArgs &a, const SaTile &t, float *sm, int tid, in
         }
         const float use = m == -INFINITY ? 0.0f : m;
         for (int s = 0; s < parts; s++) {
-            const float f = sa_exp2(sm[s * rows + r] - use);
+            const float f = fmaxf(sa_exp2(sm[s * rows + r] - use), SA_LEAST);
             sm[s * rows + r] = f;
-            if (f != 0.0f) l = fmaf(ls[s * rows + r], f, l);   // factor 0: a split without a visible key
+            l = fmaf(ls[s * rows + r], f, l);
         }
         inv[r] = sa_inv(l, m, a.sink, t.kvh * a.G + t.r0 + r - sa_token(a, t.r0 + r) * a.G);
     }
@@ -524,12 +528,10 @@ DSV4CU_DEV void sa_join(const SaArgs &a, const SaTile &t, float *sm, int tid, in
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     const float f = s0 + s < parts ? sm[(s0 + s) * rows + row[u]] : 0.0f;
-                    if (f != 0.0f) {
-                        o[u].x = fmaf(y[u][s].x, f, o[u].x);
-                        o[u].y = fmaf(y[u][s].y, f, o[u].y);
-                        o[u].z = fmaf(y[u][s].z, f, o[u].z);
-                        o[u].w = fmaf(y[u][s].w, f, o[u].w);
-                    }
+                    o[u].x = fmaf(y[u][s].x, f, o[u].x);
+                    o[u].y = fmaf(y[u][s].y, f, o[u].y);
+                    o[u].z = fmaf(y[u][s].z, f, o[u].z);
+                    o[u].w = fmaf(y[u][s].w, f, o[u].w);
                 }
         }
 #pragma unroll

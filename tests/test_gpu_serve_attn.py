@@ -510,3 +510,30 @@ def test_largest_fp32_queries(dev, dim, shared):
 
     _prompt(dev, [90, 5], 4, 1, dim, kind, shared=shared, edit=edit)
     _tree(dev, [200, 70], [3, 9], 4, 1, dim, kind, shared=shared, edit=edit)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,sink", [(64, False), (128, True), (256, True), (512, False)])
+def test_tree_nonfinite_in_one_split_of_many(dev, kind, dim, sink):
+    """A cache read in many splits: what is no number in one of them is not lost when they are joined - a query, the one
+    key of a split that a row sees, a value whose split weighs next to nothing."""
+    import torch
+
+    def query(q, k, v, kc, vc, where):
+        q[2, 1, 3] = float("nan")
+
+    def key(q, k, v, kc, vc, where):
+        k[1, 0, 0] = float("nan")
+
+    def value(q, k, v, kc, vc, where):
+        q[:, :, 0] = 8.0
+        keys, values = (c.view(-1, *c.shape[2:]) for c in (kc, vc))
+        keys[where[0][10], :, 0] = 25.0 * dim ** 0.5       # score 200: every other split's factor is below 2^-126
+        values[where[0][4000], 0, 5], values[where[0][4000], 0, 9] = float("nan"), float("inf")
+
+    for edit in (query, key, value):
+        (o, *_), _ = _tree(dev, [5003, 0], [4, 2], 4, 2, dim, kind, page=64, edit=edit, sink=sink)
+    assert bool(torch.isnan(o[:4, :2, 5]).all()) and bool(torch.isposinf(o[:4, :2, 9]).all())
+    assert bool(torch.isfinite(o[:4, :, 10:]).all())
+    _tree(dev, [5000], [1], 4, 2, dim, kind, page=64, window=1, edit=lambda q, k, *x: k.fill_(float("nan")), sink=sink)
+    _tree(dev, [5003, 900], [3, 2], 4, 2, dim, kind, page=64, edit=lambda q, *x: q.fill_(float("nan")), sink=sink)
