@@ -385,7 +385,8 @@ class TreeAttnArgs(C.Structure):
 
 # The same layouts for struct.pack: filling a ctypes.Structure of this many
 # fields costs a serving step a few microseconds per call. Every call packs a
-# buffer of its own, so calls of several threads do not touch each other's.
+# buffer of its own, so calls of several threads do not touch each other's; those
+# that use the context's workspace (page_plan, tree_attn) want a Device per thread.
 _PLAN = struct.Struct("@5i12Q")
 _PROMPT = struct.Struct("@4Q4q2iQ6ifQ")
 _TREE = struct.Struct("@6Q4q2i4Q11ifQ")

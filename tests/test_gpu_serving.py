@@ -135,3 +135,31 @@ def test_serving_loop(dev, how):
         assert not bool(used[at].any())
         used[at] = True
     assert bool(torch.isnan(kc.view(-1, KV, DIM)[~used]).all())
+
+
+@pytest.mark.parametrize("how", ["bfloat16", "float16"])
+def test_fp32_projections_reach_the_prompt_and_the_cache(dev, how):
+    """The way from fp32 projections: rounded into packed 16-bit rows by a write with the slots 0 .. n - 1, attended
+    there, and written from there into the cache - the same rows as by rounding them elsewhere."""
+    import torch
+    ct = getattr(torch, how)
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    n, pages = 77, 8
+    fused = torch.randn(n, HEADS + 2 * KV, DIM, generator=gen, device="cuda")      # one product's output
+    q, k, v = fused[:, :HEADS].to(ct), fused[:, HEADS:HEADS + KV], fused[:, HEADS + KV:]
+    k16, v16 = (torch.empty(n, KV, DIM, dtype=ct, device="cuda") for _ in range(2))
+    iota = torch.arange(n, dtype=torch.int32, device="cuda")
+    dev.paged_write(k16.view(1, n, KV, DIM), v16.view(1, n, KV, DIM), k, v, iota)
+    assert torch.equal(k16, k.to(ct)) and torch.equal(v16, v.to(ct))
+    cu = torch.tensor([0, 30, n], dtype=torch.int32, device="cuda")
+    o = torch.empty(n, HEADS, DIM, dtype=ct, device="cuda")
+    dev.prompt_attn(o, q, k16, v16, cu, DIM ** -0.5)
+    for at in (slice(0, 30), slice(30, n)):
+        want, bound = servefix.attend(q[at], k16[at], v16[at], servefix.causal_seen(at.stop - at.start, 0).cuda(),
+                                      DIM ** -0.5)
+        servefix.check_close(o[at], want, bound(ct, ct))
+    kc, vc = (torch.zeros(pages, PAGE, KV, DIM, dtype=ct, device="cuda") for _ in range(2))
+    slot = torch.randperm(pages * PAGE, generator=gen, device="cuda")[:n].to(torch.int32)
+    dev.paged_write(kc, vc, k16, v16, slot)
+    for c, x in ((kc, k16), (vc, v16)):
+        assert torch.equal(c.view(-1, KV, DIM)[slot.long()], x)
