@@ -263,9 +263,10 @@ __global__ void __launch_bounds__(PLAN_ITEM_THREADS) plan_item_kernel(const dsv4
 
 // ---------------------------------------------------------------- writes
 // cache[slot[t]] = rows[t], rounded to the cache's type, eight elements per
-// thread; blockIdx.y 0 the keys, 1 the values. Bound by memory: every row is
-// read once and written once (65111 fp32 rows of 512 into bf16: 35 us, 5.7 TB/s,
-// 0.87 of the measured copy rate; 48 rows of 8 x 128: 2.0 us).
+// thread; blockIdx.y 0 the keys, 1 the values. Bound by memory: every row with a
+// slot is read once and written once, a row without one is not read (65111 fp32
+// rows of 512 into bf16: 38.6 us, 5.2 TB/s, 0.79 of the measured copy rate; one in
+// nine skipped 35.2 us, 5.1 TB/s; 48 rows of 8 x 128: 2.0 us).
 struct WriteArgs {
     const void *src[2];
     void *dst[2];
@@ -347,9 +348,10 @@ extern "C" int dsv4cu_page_plan(dsv4cu_ctx *ctx, const dsv4cu_page_plan_args *a,
         return DSV4CU_OK;
     }
     // One launch up to 1024 requests: as many blocks as the tokens take, one
-    // where the outputs lie over the inputs. 24 requests of 8 tokens: 3.4 us
-    // against 4.5 us by one block of 1024 threads; 300 prompts of 195,000 tokens:
-    // 7.0 us against 7.9 us in two launches.
+    // where the outputs lie over the inputs. 24 requests of 8 tokens: 3.6 us
+    // against 4.5 us by one block of 1024 threads (in place, by one block of 256:
+    // 5.5 us); 300 prompts of 195,000 tokens: 7.1 us against 7.9 us in two launches
+    // (in place: 10.5 us).
     const bool solo = a->nt_cap <= PLAN_SOLO_ITEMS, over = a->held_out == a->held || a->ring_pos_out == a->ring_pos;
     const int blocks = max(1, min((a->nt_cap + PLAN_ITEM_THREADS - 1) / PLAN_ITEM_THREADS, ctx->sm_count * 2));
     if (a->n_req <= PLAN_FUSED_REQ && (solo || !over)) {

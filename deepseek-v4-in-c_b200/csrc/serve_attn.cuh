@@ -20,15 +20,16 @@
 // fp32 queries (TERMS = 3) over a bf16 cache enter as three bf16 terms
 // q = t0 + t1 + t2, which carry all 24 significand bits, and so do the
 // weights: products are those of fp32. 16-bit queries use the weights rounded
-// to the cache's type (2^-9 of each weight in bf16, 2^-12 in f16: the size of
-// the output's own rounding). The tensor core's own additions cut off low bits
+// to the cache's type (up to 2^-8 of each weight in bf16, 2^-11 in f16: the size
+// of the output's own rounding). The tensor core's own additions cut off low bits
 // (toward zero, so they do not average out), therefore it only adds within a
 // block; blocks are added in fp32 with rounding to nearest.
 //
 // Bound by mma.sync: 556 TFLOP/s at most on a B200, a third of tcgen05's, but
 // 512 output columns and the scores do not fit TMEM together, and three terms
-// of 128 query rows do not fit shared memory. Measured with 64 fp32 heads of
-// 512 dims: 6 trees over up to 9000 tokens 206 us (51 GFLOP in three terms: 250
+// of 128 query rows do not fit shared memory; 256 dims in 16 bits would fit
+// tcgen05 and have no kernel there. Measured with 64 fp32 heads of
+// 512 dims: 6 trees over up to 9000 tokens 201 us (51 GFLOP in three terms: 255
 // TFLOP/s; of a block's time 0.30 in each product, 0.18 in the softmax); 301
 // prompt tokens in a window of 128, 70 us (a third of it set-up and output of
 // 602 tiles of two or three blocks). Copies of 16 bytes instead of whole rows

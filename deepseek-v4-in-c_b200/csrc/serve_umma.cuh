@@ -29,16 +29,16 @@
 // the turns overlap; at head dim 64 the exponentials; for trees of few rows the
 // cache's bytes. Measured on one B200:
 //   32768 causal tokens, 64 heads over 8, 128 dims: 13.6 ms in a short run
-//   (1290 TFLOP/s, 0.77 of the measured bf16 rate), 15.5 to 15.9 ms repeated at
+//   (1290 TFLOP/s, 0.77 of the measured bf16 rate), 15.5 to 16.2 ms repeated at
 //   the power limit; products and copies alone take 11.8 ms.
 //   29 prompts, 16001 tokens, 16 heads over 4, 64 dims: 69 us. (Before tiles
 //   started longest first: 92 us, 107 us with one CTA of 128-key blocks per SM.)
 //   A strip's block takes 2700 clocks, 2050 of them at the exponential unit's
 //   rate for the four strips of an SM; a polynomial for a quarter to a half of
 //   the exponentials: 73 to 77 us.
-//   32 trees of 8 to 16 nodes over up to 32000 tokens, 64 heads over 8: 500 us
-//   in a short run (5.8 TB/s, 0.89 of the measured copy rate), 580 us repeated;
-//   606 us with two stages instead of three.
+//   32 trees of 8 to 16 nodes over up to 32000 tokens, 64 heads over 8: 511 us
+//   (5.7 TB/s, 0.87 of the measured copy rate), 590 us with other work between the
+//   calls; with two stages instead of three a fifth more.
 #pragma once
 
 #include <cuda.h>

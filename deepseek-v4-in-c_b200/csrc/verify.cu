@@ -93,8 +93,8 @@ DSV4CU_DEV void ver_write(const VerifyArgs &a, int b, int begin, int n, const in
 }
 
 // Greedy: a node is accepted when its token is the target's pick at the
-// current node. One warp per request, the walk in registers of lane 0's
-// shared arrays.
+// current node. One warp per request: the warp loads its nodes into shared
+// memory, lane 0 walks them there.
 __global__ void __launch_bounds__(128) verify_greedy_kernel(const VerifyArgs a)
 {
     __shared__ int s_par[4][VER_MAX_NODES], s_tok[4][VER_MAX_NODES], s_best[4][VER_MAX_NODES];
